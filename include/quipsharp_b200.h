@@ -39,7 +39,8 @@ typedef enum qs_status {
   QS_ERR_ALIGNMENT = 6,   /* pointer not aligned as the kernel requires           */
   QS_ERR_CUDA = 7,        /* a CUDA runtime call or launch failed                 */
   QS_ERR_WORKSPACE = 8,   /* workspace missing or smaller than *_bytes() asked for */
-  QS_ERR_TIMEOUT = 9      /* a kernel gave up a bounded pipeline wait (see qs_device_status) */
+  QS_ERR_TIMEOUT = 9,     /* a kernel gave up a bounded pipeline wait (see qs_device_status) */
+  QS_ERR_PAGES = 10       /* a cache ran out of pages (reported by qs_device_status)  */
 } qs_status;
 
 /* Codebook kinds (one per RVQ stage). */
@@ -63,7 +64,10 @@ const char *qs_last_error(void);
  * up a bounded wait inside its pipeline since the last call (QS_ERR_TIMEOUT;
  * the results of that launch are invalid).  The kernels never spin without a
  * limit: a stalled pipeline ends the kernel with this flag set instead of
- * hanging the GPU.  No counterpart in the reference (pure Python). */
+ * hanging the GPU.  Also reports, and clears, what the cache operators found
+ * on the device since the last call: QS_ERR_PAGES (no free page, or a table row
+ * outgrown) and QS_ERR_INDEX (a parent or token count out of range).  No
+ * counterpart in the reference (pure Python). */
 int qs_device_status(qs_stream_t stream);
 
 /* Limit, in nanoseconds, of the bounded waits between the warps of the
@@ -334,6 +338,109 @@ int qs_linear_matmul_tp(const void *x2_workspace, int64_t batch, int64_t n, int6
 int qs_linear_output_peers(const qs_tp_peers *peers, int64_t batch, int64_t m, int transform,
                            const float *su, const void *phase_u, const float *bias, void *y,
                            int y_dtype, qs_stream_t stream);
+
+/* ---- paged key-value cache ---------------------------------------------------
+ * No counterpart in the reference (it leaves decoding to transformers).  A cache
+ * keeps the keys and values of every layer in pages of `page` tokens; a row (one
+ * sequence, or one beam) is a line of page numbers in `table` (rows x width,
+ * int32) with its length in tokens in `lengths`; only the first ceil(length /
+ * page) entries of a line count, and the operators write -1 into the others.
+ * refcount[p] counts the references to page p (a caller may add its own); a page
+ * is free while it is 0, and the lowest free page is taken first.  All int32, on
+ * the device.  Page numbers outside [0, pages) are absent pages: they are never
+ * read or written. */
+typedef struct qs_kv_pool {
+  void *k, *v;          /* (layers, pages, heads, page, dim), 16-byte aligned */
+  int dtype;            /* QS_F16 or QS_BF16 */
+  int64_t layers, pages, heads;
+  int64_t page;         /* tokens per page: a power of two, 16 to 256 */
+  int64_t dim;          /* head dimension: a multiple of 8, at most 256 */
+  int64_t k_stride[4];  /* elements: layer, page, head, token (each a multiple of 8); */
+  int64_t v_stride[4];  /* the last dimension is contiguous */
+} qs_kv_pool;
+
+/* Workspace of qs_cache_fork / qs_cache_compact / qs_cache_extend (256-byte
+ * aligned; rows at most 8192). */
+int64_t qs_cache_workspace_bytes(int64_t rows, int64_t pages);
+
+/* Row i becomes a copy of row parents[i] of the input tables (-1: an empty row;
+ * its pages are freed unless others hold them): fork, free and reorder in one.
+ * Whole pages are shared.  A part-filled last page stays with the lowest child of
+ * a row, and each other child gets the lowest free page, in row order, with the
+ * filled tokens of all layers copied into it.  The new counts are the old ones
+ * plus references after minus references before, taken before pages are handed
+ * out, so pages freed by this call serve it.  The outputs must not overlap the
+ * inputs.  A row that finds no free page gets -1 there (QS_ERR_PAGES from
+ * qs_device_status); a parent outside [-1, rows) makes an empty row
+ * (QS_ERR_INDEX). */
+int qs_cache_fork(const qs_kv_pool *pool, int64_t rows, int64_t width, const int *table, const int *lengths,
+                  const int *refcount, const int *parents, int *table_out, int *lengths_out, int *refcount_out,
+                  void *workspace, int64_t workspace_bytes, qs_stream_t stream);
+/* Moves the pages in use to the lowest numbers: with U of them, those from U on
+ * go to the holes below U, both in ascending order, contents of all layers with
+ * them.  used_out (one int32, device) gets U.  The table and count outputs may be
+ * the inputs. */
+int qs_cache_compact(const qs_kv_pool *pool, int64_t rows, int64_t width, const int *table, const int *lengths,
+                     const int *refcount, int *table_out, int *refcount_out, int *used_out, void *workspace,
+                     int64_t workspace_bytes, qs_stream_t stream);
+/* Row i grows by add[i] (>= 0) tokens: the pages that it needs are the lowest
+ * free ones, in row and then column order.  The outputs may be the inputs.  Where
+ * pages run out or a line is full, the length grows all the same and the missing
+ * entries are -1 (QS_ERR_PAGES from qs_device_status). */
+int qs_cache_extend(int64_t page, int64_t pages, int64_t rows, int64_t width, const int *table, const int *lengths,
+                    const int *refcount, const int *add, int *table_out, int *lengths_out, int *refcount_out,
+                    void *workspace, int64_t workspace_bytes, qs_stream_t stream);
+/* Writes the keys and values of new tokens of one layer (pool->layers == 1): k and
+ * v are (tokens, heads, dim) of the pool's type, packed by row; row r's are
+ * [cu[r], cu[r+1]) and take its last places (lengths already count them).  cu
+ * NULL: one token per row.  Strides in elements, multiples of 8.  Tokens whose
+ * page is absent are left out. */
+int qs_cache_write(const qs_kv_pool *pool, int64_t rows, int64_t width, const int *table, const int *lengths,
+                   const int *cu, const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v,
+                   int64_t v_token_stride, int64_t v_head_stride, int64_t tokens, qs_stream_t stream);
+
+/* ---- attention over the paged cache ------------------------------------------
+ * o = sum_j p_j v_j with p = softmax_j(scale * q . k_j) over the keys that the
+ * query's token sees: with the token in place i of its row (places count from 0)
+ * those j <= i with j > i - window or j < sinks (window 0: every j <= i).  Query
+ * head h reads key head h / (q_heads / heads).  Keys that a query does not see do
+ * not enter, whatever they hold; a query that sees none gives 0 (and lse -inf).
+ * q and out have the pool's type, lse is float32: log sum_j exp(scale q . k_j),
+ * or NULL.  pool is one layer (layers == 1) with dim at most 128. */
+
+/* One token per row, the newest: q (rows, q_heads, dim) with strides in elements
+ * (multiples of 8), out (rows, q_heads, dim) and lse (rows, q_heads) contiguous.
+ * Rows of length 0 see nothing.  workspace: 256-byte aligned. */
+int64_t qs_attn_decode_workspace_bytes(int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t dim);
+int qs_attn_decode(const void *q, int64_t q_row_stride, int64_t q_head_stride, const qs_kv_pool *pool, int64_t rows,
+                   int64_t q_heads, int64_t width, const int *table, const int *lengths, float scale, int64_t window,
+                   int64_t sinks, void *out, float *lse, void *workspace, int64_t workspace_bytes,
+                   qs_stream_t stream);
+/* Many tokens per row, packed: row r's are [cu[r], cu[r+1]) of q (tokens, q_heads,
+ * dim) and take its last places, their keys and values already written (lengths
+ * count them).  Tokens past cu[rows] give 0. */
+int64_t qs_attn_window_workspace_bytes(int64_t tokens, int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t dim);
+int qs_attn_window(const void *q, int64_t q_token_stride, int64_t q_head_stride, const qs_kv_pool *pool,
+                   int64_t tokens, int64_t rows, int64_t q_heads, int64_t width, const int *table, const int *lengths,
+                   const int *cu, float scale, int64_t window, int64_t sinks, void *out, float *lse, void *workspace,
+                   int64_t workspace_bytes, qs_stream_t stream);
+
+/* ---- beam search: selection ---------------------------------------------------
+ * For each of `batch` searches the best n continuations of its `beams` beams:
+ * score[b] + log_softmax(logits[b])[token].  A beam's tokens rank by logit (ties:
+ * the lower token first); the beams' lists then merge by score (ties: the lower
+ * beam first, then by rank).  A NaN logit counts as -inf; a beam all of -inf has
+ * scores of -inf; +inf logits share the whole probability.  finished (batch,
+ * beams) bytes or NULL: an ended beam has the one continuation `pad` with its
+ * score as it is (and then -inf).  A NaN score counts as -inf.  logits: QS_F32 /
+ * QS_F16 / QS_BF16, strides in elements, the vocabulary contiguous.  Outputs
+ * (batch, n): scores float32, parents (the beam, 0 to beams - 1) and tokens
+ * int32.  n at most 64 and at most vocab, beams at most 64. */
+int64_t qs_beam_workspace_bytes(int64_t batch, int64_t beams, int64_t vocab, int64_t n);
+int qs_beam_select(const void *logits, int dtype, int64_t batch_stride, int64_t beam_stride, int64_t batch,
+                   int64_t beams, int64_t vocab, const float *scores, const uint8_t *finished, int64_t n, int pad,
+                   float *scores_out, int *parents_out, int *tokens_out, void *workspace, int64_t workspace_bytes,
+                   qs_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -6,6 +6,7 @@ is missing, every CUDA entry point raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -24,6 +25,7 @@ QS_ERR_ALIGNMENT = 6
 QS_ERR_CUDA = 7
 QS_ERR_WORKSPACE = 8
 QS_ERR_TIMEOUT = 9
+QS_ERR_PAGES = 10
 
 QS_CB_E8P = 0
 QS_CB_E8_1BIT = 1
@@ -73,6 +75,17 @@ _SIGS = {
     "qs_linear_output_peers": (_I, [_P, _L, _L, _I, _P, _P, _P, _P, _I, _P]),
     "qs_linear_fwd_tp": (_I, [_P, _I, _L, _L, _L, _P, _I, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P, _P, _L, _P,
                               _P]),
+    "qs_cache_workspace_bytes": (_L, [_L, _L]),
+    "qs_cache_fork": (_I, [_P, _L, _L, _P, _P, _P, _P, _P, _P, _P, _P, _L, _P]),
+    "qs_cache_compact": (_I, [_P, _L, _L, _P, _P, _P, _P, _P, _P, _P, _L, _P]),
+    "qs_cache_extend": (_I, [_L, _L, _L, _L, _P, _P, _P, _P, _P, _P, _P, _P, _L, _P]),
+    "qs_attn_decode_workspace_bytes": (_L, [_L, _L, _L, _L]),
+    "qs_attn_decode": (_I, [_P, _L, _L, _P, _L, _L, _L, _P, _P, ctypes.c_float, _L, _L, _P, _P, _P, _L, _P]),
+    "qs_attn_window_workspace_bytes": (_L, [_L, _L, _L, _L, _L]),
+    "qs_attn_window": (_I, [_P, _L, _L, _P, _L, _L, _L, _L, _P, _P, _P, ctypes.c_float, _L, _L, _P, _P, _P, _L, _P]),
+    "qs_beam_workspace_bytes": (_L, [_L, _L, _L, _L]),
+    "qs_beam_select": (_I, [_P, _I, _L, _L, _L, _L, _L, _P, _P, _L, _I, _P, _P, _P, _P, _L, _P]),
+    "qs_cache_write": (_I, [_P, _L, _L, _P, _P, _P, _P, _L, _L, _P, _L, _L, _L, _P]),
 }
 
 QS_TP_MAX_RANKS = 8
@@ -101,6 +114,14 @@ class LinearLayer(ctypes.Structure):
                 ("phase_u", ctypes.c_void_p), ("phase_v", ctypes.c_void_p),
                 ("bias", ctypes.c_void_p), ("y", ctypes.c_void_p),
                 ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64)]
+
+
+class KVPool(ctypes.Structure):
+    """qs_kv_pool (include/quipsharp_b200.h): the keys and values of a paged cache."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("dtype", ctypes.c_int),
+                ("layers", ctypes.c_int64), ("pages", ctypes.c_int64), ("heads", ctypes.c_int64),
+                ("page", ctypes.c_int64), ("dim", ctypes.c_int64),
+                ("k_stride", ctypes.c_int64 * 4), ("v_stride", ctypes.c_int64 * 4)]
 
 
 EXPORTS = tuple(_SIGS)
@@ -152,12 +173,44 @@ def check(status: int) -> None:
     raise RuntimeError(f"quipsharp_b200 error {status}: {msg}")
 
 
+ref = ctypes.byref
+
+
 def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 
 
 def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def raw_stream(index: int) -> int:
+    """The current stream of a device, without a Stream object."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def device_guard(device: torch.device):
+    """Makes `device` current, at no cost where it is already."""
+    return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def refuse_grad(name: str, *tensors) -> None:
+    """The decoding operators have no backward pass: refuse inputs whose
+    gradient autograd would silently lose."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} has no backward pass; call it under torch.no_grad() or detach its inputs")
+
+
+def rows_of_8(t: torch.Tensor) -> torch.Tensor:
+    """t as the kernels read it in 16-byte pieces (two-byte elements): the last
+    dimension contiguous, other strides multiples of 8, the start aligned; a
+    contiguous copy where it is not."""
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1]):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def require_cuda(*tensors) -> None:

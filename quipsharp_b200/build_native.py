@@ -113,7 +113,8 @@ def _write_if_changed(path: str, text: str) -> None:
 
 SOURCES = ["qs_abi.cu", "qs_decode.cu", "qs_transform.cu", "qs_pack.cu", "qs_gemv.cu",
            "qs_xform_a.cu", "qs_xform_b.cu", "qs_xform_c.cu", "qs_xform_d.cu", "qs_xform_e.cu", "qs_xform_f.cu",
-           "qs_noalloc.cu", "qs_gemm_tc.cu", "qs_xform2.cu", "qs_tp.cu", "qs_fit.cu", "qs_xsmall.cu"]
+           "qs_noalloc.cu", "qs_gemm_tc.cu", "qs_xform2.cu", "qs_tp.cu", "qs_fit.cu", "qs_xsmall.cu",
+           "qs_cache.cu", "qs_beam.cu", "qs_attn_decode.cu", "qs_attn_window.cu"]
 
 
 def _compile(src: str, obj: str, verbose: bool) -> None:

@@ -493,3 +493,205 @@ QS_API int qs_linear_fwd_group(const void *x, int x_dtype, int64_t batch, int64_
       st = fail(QS_ERR_CUDA, "group join failed");
   return st;
 }
+
+// ---- paged key-value cache --------------------------------------------------------
+static int check_pool(const qs_kv_pool *p) {
+  if (!p) return fail(QS_ERR_INVALID_ARG, "null pool");
+  if (p->dtype != QS_F16 && p->dtype != QS_BF16) return fail(QS_ERR_INVALID_ARG, "a cache holds float16 or bfloat16 (dtype %d)", p->dtype);
+  if (p->layers < 1 || p->heads < 1 || p->pages < 1 || p->dim < 1 || p->layers > (1 << 20) || p->heads > (1 << 20))
+    return fail(QS_ERR_INVALID_ARG, "bad pool shape");
+  if (p->pages > (1 << 28)) return fail(QS_ERR_UNSUPPORTED, "more than 2^28 pages");
+  if (p->page < 16 || p->page > 256 || (p->page & (p->page - 1)))
+    return fail(QS_ERR_UNSUPPORTED, "page size must be a power of two of 16 to 256, got %lld", (long long)p->page);
+  if (p->dim % 8 || p->dim > 256)
+    return fail(QS_ERR_UNSUPPORTED, "head dimension must be a multiple of 8 up to 256, got %lld", (long long)p->dim);
+  if (!p->k || !p->v) return fail(QS_ERR_INVALID_ARG, "null pointer");
+  if (!aligned(p->k, 16) || !aligned(p->v, 16)) return fail(QS_ERR_ALIGNMENT, "pools must be 16-byte aligned");
+  for (int i = 0; i < 4; ++i)
+    if (p->k_stride[i] < 0 || p->v_stride[i] < 0 || p->k_stride[i] % 8 || p->v_stride[i] % 8)
+      return fail(QS_ERR_ALIGNMENT, "pool strides must be multiples of 8 elements");
+  return QS_OK;
+}
+
+static int check_rows(int64_t rows, int64_t width, const int *table, const int *lengths) {
+  if (rows < 0 || width < 0) return fail(QS_ERR_INVALID_ARG, "bad table shape");
+  if (width > (1 << 24)) return fail(QS_ERR_UNSUPPORTED, "more than 2^24 pages in a row");
+  if (rows && (!lengths || (width && !table))) return fail(QS_ERR_INVALID_ARG, "null pointer");
+  return QS_OK;
+}
+
+static int check_cache_work(int64_t rows, int64_t pages, const void *ws, int64_t bytes) {
+  if (rows > kCacheMaxRows) return fail(QS_ERR_UNSUPPORTED, "more than %d rows", kCacheMaxRows);
+  if (!ws || bytes < cache_workspace_bytes(rows, pages)) return fail(QS_ERR_WORKSPACE, "workspace missing or too small");
+  if (!aligned(ws, 256)) return fail(QS_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
+  return QS_OK;
+}
+
+QS_API int64_t qs_cache_workspace_bytes(int64_t rows, int64_t pages) {
+  if (rows < 0 || rows > kCacheMaxRows || pages < 1 || pages > (1 << 28)) return -1;
+  return cache_workspace_bytes(rows, pages);
+}
+
+QS_API int qs_cache_fork(const qs_kv_pool *pool, int64_t rows, int64_t width, const int *table, const int *lengths,
+                         const int *refcount, const int *parents, int *table_out, int *lengths_out, int *refcount_out,
+                         void *workspace, int64_t workspace_bytes, qs_stream_t stream) {
+  int st = check_pool(pool);
+  if (st || (st = check_rows(rows, width, table, lengths))) return st;
+  if ((st = check_cache_work(rows, pool->pages, workspace, workspace_bytes))) return st;
+  if (!refcount || !refcount_out || (rows && (!parents || !lengths_out || (width && !table_out))))
+    return fail(QS_ERR_INVALID_ARG, "null pointer");
+  if (overlaps(table, rows * width * 4, table_out, rows * width * 4) || overlaps(lengths, rows * 4, lengths_out, rows * 4) ||
+      overlaps(refcount, pool->pages * 4, refcount_out, pool->pages * 4))
+    return fail(QS_ERR_INVALID_ARG, "fork's outputs must not overlap its inputs");
+  return launch_cache_fork(*pool, (int)rows, (int)width, table, lengths, refcount, parents, table_out, lengths_out,
+                           refcount_out, workspace, (cudaStream_t)stream);
+}
+
+QS_API int qs_cache_compact(const qs_kv_pool *pool, int64_t rows, int64_t width, const int *table, const int *lengths,
+                            const int *refcount, int *table_out, int *refcount_out, int *used_out, void *workspace,
+                            int64_t workspace_bytes, qs_stream_t stream) {
+  int st = check_pool(pool);
+  if (st || (st = check_rows(rows, width, table, lengths))) return st;
+  if ((st = check_cache_work(rows, pool->pages, workspace, workspace_bytes))) return st;
+  if (!refcount || !refcount_out || !used_out || (rows && width && !table_out))
+    return fail(QS_ERR_INVALID_ARG, "null pointer");
+  return launch_cache_compact(*pool, (int)rows, (int)width, table, lengths, refcount, table_out, refcount_out, used_out,
+                              workspace, (cudaStream_t)stream);
+}
+
+QS_API int qs_cache_extend(int64_t page, int64_t pages, int64_t rows, int64_t width, const int *table,
+                           const int *lengths, const int *refcount, const int *add, int *table_out, int *lengths_out,
+                           int *refcount_out, void *workspace, int64_t workspace_bytes, qs_stream_t stream) {
+  if (page < 16 || page > 256 || (page & (page - 1)))
+    return fail(QS_ERR_UNSUPPORTED, "page size must be a power of two of 16 to 256, got %lld", (long long)page);
+  if (pages < 1) return fail(QS_ERR_INVALID_ARG, "bad pool shape");
+  if (pages > (1 << 28)) return fail(QS_ERR_UNSUPPORTED, "more than 2^28 pages");
+  int st = check_rows(rows, width, table, lengths);
+  if (st || (st = check_cache_work(rows, pages, workspace, workspace_bytes))) return st;
+  if (!refcount || !refcount_out || (rows && (!add || !lengths_out || (width && !table_out))))
+    return fail(QS_ERR_INVALID_ARG, "null pointer");
+  return launch_cache_extend(page, pages, (int)rows, (int)width, table, lengths, refcount, add, table_out, lengths_out,
+                             refcount_out, workspace, (cudaStream_t)stream);
+}
+
+QS_API int qs_cache_write(const qs_kv_pool *pool, int64_t rows, int64_t width, const int *table, const int *lengths,
+                          const int *cu, const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v,
+                          int64_t v_token_stride, int64_t v_head_stride, int64_t tokens, qs_stream_t stream) {
+  int st = check_pool(pool);
+  if (st || (st = check_rows(rows, width, table, lengths))) return st;
+  if (pool->layers != 1) return fail(QS_ERR_INVALID_ARG, "a write takes one layer's pool");
+  if (rows > (1 << 28) || tokens > (int64_t(1) << 30)) return fail(QS_ERR_UNSUPPORTED, "too many rows or tokens");
+  if (tokens < 0 || (!cu && tokens != rows)) return fail(QS_ERR_INVALID_ARG, "without cu there is one token per row");
+  if (tokens == 0 || rows == 0 || width == 0) return QS_OK;
+  if (!k || !v) return fail(QS_ERR_INVALID_ARG, "null pointer");
+  if (!aligned(k, 16) || !aligned(v, 16) || k_token_stride < 0 || k_head_stride < 0 || v_token_stride < 0 ||
+      v_head_stride < 0 || k_token_stride % 8 || k_head_stride % 8 || v_token_stride % 8 || v_head_stride % 8)
+    return fail(QS_ERR_ALIGNMENT, "keys and values must be 16-byte aligned, their strides multiples of 8 elements");
+  return launch_cache_write(*pool, (int)rows, (int)width, table, lengths, cu, k, k_token_stride, k_head_stride, v,
+                            v_token_stride, v_head_stride, tokens, (cudaStream_t)stream);
+}
+
+// ---- beam search ---------------------------------------------------------------------
+QS_API int64_t qs_beam_workspace_bytes(int64_t batch, int64_t beams, int64_t vocab, int64_t n) {
+  if (batch < 0 || beams < 1 || beams > kBeamMaxBeams || vocab < 1 || n < 1 || n > kBeamMaxN || n > vocab) return -1;
+  return beam_workspace_bytes(batch, beams, vocab, n);
+}
+
+QS_API int qs_beam_select(const void *logits, int dtype, int64_t batch_stride, int64_t beam_stride, int64_t batch,
+                          int64_t beams, int64_t vocab, const float *scores, const uint8_t *finished, int64_t n,
+                          int pad, float *scores_out, int *parents_out, int *tokens_out, void *workspace,
+                          int64_t workspace_bytes, qs_stream_t stream) {
+  if (!valid_io_dtype(dtype)) return fail(QS_ERR_INVALID_ARG, "bad dtype %d", dtype);
+  if (batch < 0 || beams < 1 || vocab < 1 || n < 1 || n > vocab || batch_stride < 0 || beam_stride < 0)
+    return fail(QS_ERR_INVALID_ARG, "bad shape: n must be between 1 and the vocabulary");
+  if (beams > kBeamMaxBeams || n > kBeamMaxN)
+    return fail(QS_ERR_UNSUPPORTED, "up to %d beams and n up to %d, got %lld and %lld", kBeamMaxBeams, kBeamMaxN,
+                (long long)beams, (long long)n);
+  if (vocab > (1 << 30) || batch * beams > 65535) return fail(QS_ERR_UNSUPPORTED, "vocabulary or batch x beams too large");
+  if (batch == 0) return QS_OK;
+  if (!logits || !scores || !scores_out || !parents_out || !tokens_out) return fail(QS_ERR_INVALID_ARG, "null pointer");
+  if (!aligned(logits, dtype == QS_F32 ? 4 : 2)) return fail(QS_ERR_ALIGNMENT, "logits must be aligned to their type");
+  if (!workspace || workspace_bytes < beam_workspace_bytes(batch, beams, vocab, n))
+    return fail(QS_ERR_WORKSPACE, "workspace missing or too small");
+  if (!aligned(workspace, 256)) return fail(QS_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
+  return launch_beam_select(logits, dtype, batch_stride, beam_stride, batch, beams, vocab, scores, finished, (int)n, pad,
+                            scores_out, parents_out, tokens_out, workspace, (cudaStream_t)stream);
+}
+
+// ---- attention over the paged cache ----------------------------------------------------
+static int check_attn(AttnArgs *a, const void *q, int64_t q_token, int64_t q_head, const qs_kv_pool *pool, int64_t tokens,
+                      int64_t rows, int64_t q_heads, int64_t width, const int *table, const int *lengths, float scale,
+                      int64_t window, int64_t sinks, void *out, float *lse, void *ws) {
+  int st = check_pool(pool);
+  if (st || (st = check_rows(rows, width, table, lengths))) return st;
+  if (pool->layers != 1) return fail(QS_ERR_INVALID_ARG, "attention reads one layer's pool");
+  if (pool->dim > 128) return fail(QS_ERR_UNSUPPORTED, "head dimension up to 128, got %lld", (long long)pool->dim);
+  if (q_heads < 1 || q_heads % pool->heads)
+    return fail(QS_ERR_INVALID_ARG, "%lld query heads do not share %lld key heads evenly", (long long)q_heads,
+                (long long)pool->heads);
+  if (tokens < 0 || window < 0 || sinks < 0) return fail(QS_ERR_INVALID_ARG, "negative tokens, window or sinks");
+  if (!(scale > 0.f) || scale > 3e38f) return fail(QS_ERR_INVALID_ARG, "scale must be positive and finite");
+  if (rows > (1 << 24) || tokens > (1 << 30) || q_heads > (1 << 20) || rows * q_heads > (int64_t(1) << 30) ||
+      (width << 8) > (int64_t(1) << 30))
+    return fail(QS_ERR_UNSUPPORTED, "too many rows, tokens, heads or pages in a row");
+  if (tokens == 0) return QS_OK;
+  if (!q || !out) return fail(QS_ERR_INVALID_ARG, "null pointer");
+  if (!aligned(q, 16) || !aligned(out, 16) || q_token < 0 || q_head < 0 || q_token % 8 || q_head % 8)
+    return fail(QS_ERR_ALIGNMENT, "queries must be 16-byte aligned, their strides multiples of 8 elements");
+  int shift = 4;
+  while ((int64_t(1) << shift) < pool->page) ++shift;
+  *a = AttnArgs{q, q_token, q_head, pool->k, pool->v,
+                {pool->k_stride[1], pool->k_stride[2], pool->k_stride[3]},
+                {pool->v_stride[1], pool->v_stride[2], pool->v_stride[3]},
+                pool->dtype, (int)pool->dim, (int)q_heads, (int)pool->heads, (int)pool->pages, shift,
+                (int)rows, (int)width, tokens, table, lengths, nullptr, scale, window, sinks, out, lse, ws};
+  return QS_OK;
+}
+
+static bool attn_shape_ok(int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t dim) {
+  return rows >= 0 && q_heads >= 1 && kv_heads >= 1 && q_heads % kv_heads == 0 && dim >= 8 && dim <= 128 && dim % 8 == 0 &&
+         rows <= (1 << 24) && q_heads <= (1 << 20);
+}
+
+QS_API int64_t qs_attn_decode_workspace_bytes(int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t dim) {
+  return attn_shape_ok(rows, q_heads, kv_heads, dim) ? attn_decode_workspace_bytes(rows, q_heads, kv_heads, dim) : -1;
+}
+
+QS_API int qs_attn_decode(const void *q, int64_t q_row_stride, int64_t q_head_stride, const qs_kv_pool *pool, int64_t rows,
+                          int64_t q_heads, int64_t width, const int *table, const int *lengths, float scale,
+                          int64_t window, int64_t sinks, void *out, float *lse, void *workspace,
+                          int64_t workspace_bytes, qs_stream_t stream) {
+  AttnArgs a;
+  const int st = check_attn(&a, q, q_row_stride, q_head_stride, pool, rows, rows, q_heads, width, table, lengths, scale,
+                            window, sinks, out, lse, workspace);
+  if (st || rows == 0) return st;
+  if (!workspace || workspace_bytes < attn_decode_workspace_bytes(rows, q_heads, pool->heads, pool->dim))
+    return fail(QS_ERR_WORKSPACE, "workspace missing or too small");
+  if (!aligned(workspace, 256)) return fail(QS_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
+  return launch_attn_decode(a, (cudaStream_t)stream);
+}
+
+QS_API int64_t qs_attn_window_workspace_bytes(int64_t tokens, int64_t rows, int64_t q_heads, int64_t kv_heads,
+                                              int64_t dim) {
+  if (tokens < 0 || !attn_shape_ok(rows, q_heads, kv_heads, dim)) return -1;
+  return attn_window_workspace_bytes(tokens, rows, q_heads, kv_heads, dim);
+}
+
+QS_API int qs_attn_window(const void *q, int64_t q_token_stride, int64_t q_head_stride, const qs_kv_pool *pool,
+                          int64_t tokens, int64_t rows, int64_t q_heads, int64_t width, const int *table,
+                          const int *lengths, const int *cu, float scale, int64_t window, int64_t sinks, void *out,
+                          float *lse, void *workspace, int64_t workspace_bytes, qs_stream_t stream) {
+  AttnArgs a;
+  const int st = check_attn(&a, q, q_token_stride, q_head_stride, pool, tokens, rows, q_heads, width, table, lengths,
+                            scale, window, sinks, out, lse, workspace);
+  if (st || tokens == 0) return st;
+  if (!cu) return fail(QS_ERR_INVALID_ARG, "null pointer");
+  if (q_heads / pool->heads > 128 || pool->heads > 65535)
+    return fail(QS_ERR_UNSUPPORTED, "up to 128 query heads per key head and 65535 key heads");
+  if (workspace_bytes < attn_window_workspace_bytes(tokens, rows, q_heads, pool->heads, pool->dim) ||
+      (workspace_bytes && !workspace))
+    return fail(QS_ERR_WORKSPACE, "workspace missing or too small");
+  if (!aligned(workspace, 256)) return fail(QS_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
+  a.cu = cu;
+  return launch_attn_window(a, (cudaStream_t)stream);
+}

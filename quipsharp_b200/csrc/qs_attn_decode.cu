@@ -1,0 +1,464 @@
+// Attention of one new token per row over the paged cache.
+//
+// The query heads that share a key head form the 16 rows of mma.sync m16n8k16 (more
+// than 16 take further blocks of 16), so each key and value is read once for all of
+// them.  A warp works alone: it streams groups of 16 keys (one page each) through its
+// own cp.async ring, keeps the running maximum, sum and output of a softmax in
+// registers, and meets the other warps of its CTA only when a segment ends.
+//
+// Rows differ in length, so the work is cut by keys, not by rows: the groups of all
+// (row, key head) segments form one line that is dealt to the CTAs in equal ranges,
+// whatever the lengths.  A segment that several ranges share leaves partial results
+// (maximum, sum, output in float32), which attn_join_kernel puts together in order.
+//
+// Bound: the keys and values seen, once, at HBM rate.
+#include <cmath>
+#include <type_traits>
+
+#include "qs_attn.cuh"
+
+namespace qs {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kStages = 3;
+constexpr int kKeys = 16;       // keys of a group
+constexpr int kRows = 16;       // query heads of a block
+constexpr int kCtasPerSm = 2;
+constexpr int kMinRange = 16;   // groups of a range at least: 4 per warp, or the joins cost more than the split saves
+
+// The groups of 16 keys that a row's newest token sees: the first `sink` groups, then
+// those from `from` on.
+struct Seen {
+  int n, lo, sink_keys;  // keys in places >= lo or < sink_keys are seen
+  int sink, from, count;
+};
+
+__device__ __forceinline__ Seen seen_of(int length, const AttnArgs &a) {
+  Seen s;
+  const int64_t cap = static_cast<int64_t>(a.width) << a.page_shift;
+  s.n = static_cast<int>(min(cap, static_cast<int64_t>(max(0, length))));
+  s.lo = a.window > 0 && length > a.window ? static_cast<int>(length - a.window) : 0;
+  s.lo = min(s.lo, s.n);
+  s.sink_keys = static_cast<int>(min(static_cast<int64_t>(s.lo), a.sinks));
+  s.sink = (s.sink_keys + kKeys - 1) / kKeys;
+  s.from = max(s.lo / kKeys, s.sink);
+  s.count = s.sink + max(0, (s.n + kKeys - 1) / kKeys - s.from);
+  return s;
+}
+
+// How the line of groups is dealt (the same in every CTA and in the join).
+struct Deal {
+  int64_t total;  // padded groups of all segments
+  int range;      // groups per range
+  int pad;        // segments take multiples of this many groups
+};
+
+__device__ __forceinline__ int padded(int count, int pad) { return (count + pad - 1) / pad * pad; }
+
+struct Ws {
+  int64_t *start;  // [rows + 1]: padded groups of one head before the row
+  int *deal;       // range, pad
+  float *ml;       // [slot][16][2]
+  float *o;        // [slot][16][DP]
+};
+
+template <typename T, int DP>
+struct Smem {
+  T kv[kWarps][kStages][2][kKeys * DP];
+  float ml[kWarps][kRows][2];
+  int64_t sums[kThreads + 1][2];
+};
+
+// One warp's softmax state over 16 query rows (R8: only the first 8 are real).
+template <typename T, int DP, bool R8>
+struct Warp {
+  uint32_t q[DP / 16][4];
+  float o[DP / 8][4];
+  float m[2], l[2];
+
+  __device__ __forceinline__ void load_q(const AttnArgs &a, int64_t row, int head0, int heads, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    const T *base = static_cast<const T *>(a.q) + row * a.q_token;
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = g + (i & 1) * 8, d = k * 16 + (i >> 1) * 8 + 2 * t;
+        q[k][i] = r < heads && d < a.dim
+                      ? *reinterpret_cast<const uint32_t *>(base + (head0 + r) * a.q_head + d) : 0u;
+      }
+  }
+  __device__ __forceinline__ void reset() {
+#pragma unroll
+    for (int j = 0; j < DP / 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[j][i] = 0.f;
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
+  }
+  // 16 keys at kv (keys, then values, swizzled rows); bit i of `mask`: key i is seen.
+  __device__ __forceinline__ void step(uint32_t ks, uint32_t vs, uint32_t mask, float scale2, int lane) {
+    float s[2][4] = {};
+    const int r8 = lane & 7, hi = (lane >> 3) & 1, top = lane >> 4;
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k) {
+      uint32_t b[4];
+      ldmatrix_x4(b, ks + swizzled<DP>(r8 + 8 * top, 2 * k + hi));
+      mma16816<T>(s[0], q[k], b[0], b[1]);
+      mma16816<T>(s[1], q[k], b[2], b[3]);
+    }
+    const int t = lane & 3;
+    float top_s[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < (R8 ? 2 : 4); ++i) {
+        s[j][i] = (mask >> (8 * j + 2 * t + (i & 1))) & 1 ? s[j][i] * scale2 : -INFINITY;
+        top_s[i >> 1] = fmaxf(top_s[i >> 1], s[j][i]);
+      }
+    bool grew = false;
+    float mn[2], alpha[2];
+#pragma unroll
+    for (int h = 0; h < (R8 ? 1 : 2); ++h) {
+      top_s[h] = fmaxf(top_s[h], __shfl_xor_sync(0xffffffffu, top_s[h], 1));
+      top_s[h] = fmaxf(top_s[h], __shfl_xor_sync(0xffffffffu, top_s[h], 2));
+      mn[h] = fmaxf(m[h], top_s[h]);
+      grew |= mn[h] > m[h];
+      alpha[h] = mn[h] == -INFINITY ? 1.f : ex2(m[h] - mn[h]);
+      m[h] = mn[h];
+    }
+    if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+      for (int h = 0; h < (R8 ? 1 : 2); ++h) {
+        l[h] *= alpha[h];
+#pragma unroll
+        for (int j = 0; j < DP / 8; ++j) o[j][2 * h] *= alpha[h], o[j][2 * h + 1] *= alpha[h];
+      }
+    }
+    // The weights enter the second product as the sum of two 16-bit values (what the
+    // first leaves of 24 bits, the second takes), so they lose nothing that the output's
+    // rounding would show; the extra products are hidden behind the loads.
+    uint32_t ph[4] = {}, pl[4] = {};
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int h = 0; h < (R8 ? 1 : 2); ++h) {
+        const float base = m[h] == -INFINITY ? 0.f : m[h];
+        const float x = ex2(s[j][2 * h] - base), y = ex2(s[j][2 * h + 1] - base);
+        l[h] += x + y;
+        const float2 back = split16<T>(x, y, ph[2 * j + h]);
+        float2 unused;
+        unused = split16<T>(x - back.x, y - back.y, pl[2 * j + h]);
+        (void)unused;
+      }
+#pragma unroll
+    for (int j = 0; j < DP / 16; ++j) {
+      uint32_t b[4];
+      ldmatrix_x4_trans(b, vs + swizzled<DP>(r8 + 8 * hi, 2 * j + top));
+      mma16816<T>(o[2 * j], ph, b[0], b[1]);
+      mma16816<T>(o[2 * j + 1], ph, b[2], b[3]);
+      mma16816<T>(o[2 * j], pl, b[0], b[1]);
+      mma16816<T>(o[2 * j + 1], pl, b[2], b[3]);
+    }
+  }
+};
+
+template <typename T, int DP, bool R8>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_decode_kernel(AttnArgs a, Ws ws, int blocks, int share) {
+  extern __shared__ __align__(128) uint8_t dsm[];
+  Smem<T, DP> &sm = *reinterpret_cast<Smem<T, DP> *>(dsm);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // ---- the line of groups: counts per thread's rows, then their prefix
+  const int heads = a.kv_heads * blocks;  // segments per row
+  const int per = (a.rows + kThreads - 1) / kThreads;
+  const int first_row = min(a.rows, tid * per), last_row = min(a.rows, first_row + per);
+  {
+    int64_t c = 0, p = 0;
+    for (int r = first_row; r < last_row; ++r) {
+      const int n = seen_of(a.lengths[r], a).count;
+      c += n;
+      p += padded(n, kMinRange);
+    }
+    sm.sums[tid + 1][0] = c;
+    sm.sums[tid + 1][1] = p;
+    if (tid == 0) sm.sums[0][0] = sm.sums[0][1] = 0;
+    __syncthreads();
+    for (int d = 1; d < kThreads; d <<= 1) {
+      int64_t x = 0, y = 0;
+      if (tid >= d) x = sm.sums[tid + 1 - d][0], y = sm.sums[tid + 1 - d][1];
+      __syncthreads();
+      sm.sums[tid + 1][0] += x;
+      sm.sums[tid + 1][1] += y;
+      __syncthreads();
+    }
+  }
+  // Enough groups for every CTA: one unpadded line in equal ranges.  Else short ranges
+  // that begin with their segments, so that most segments need no join.
+  Deal d;
+  const int64_t groups = sm.sums[kThreads][0] * heads;
+  const bool dense = groups >= static_cast<int64_t>(gridDim.x) * kMinRange;
+  const int col = dense ? 0 : 1;
+  d.pad = dense ? 1 : kMinRange;
+  d.total = sm.sums[kThreads][col] * heads;
+  d.range = dense ? static_cast<int>((d.total + gridDim.x - 1) / gridDim.x) : kMinRange;
+  if (blockIdx.x == 0) {  // for the join
+    int64_t at = sm.sums[tid][col];
+    for (int r = first_row; r < last_row; ++r) {
+      ws.start[r] = at;
+      at += padded(seen_of(a.lengths[r], a).count, d.pad);
+    }
+    if (tid == 0) {
+      ws.start[a.rows] = sm.sums[kThreads][col];
+      ws.deal[0] = d.range;
+      ws.deal[1] = d.pad;
+    }
+  }
+
+  const T *kbase = static_cast<const T *>(a.k), *vbase = static_cast<const T *>(a.v);
+  const float scale2 = a.scale * kLog2e;
+  constexpr int CPR = DP / 8;            // 16-byte pieces of a key
+  constexpr int RPI = 32 / CPR;          // keys per warp-wide copy
+  const int piece = lane % CPR, sub = lane / CPR;
+  const uint32_t ring = smem_u32(&sm.kv[warp][0][0][0]);
+  Warp<T, DP, R8> w;
+
+  const int64_t ranges = (d.total + d.range - 1) / d.range;
+  for (int64_t range = blockIdx.x; range < ranges; range += gridDim.x) {
+    const int64_t r0 = range * d.range, r1 = min(d.total, r0 + d.range);
+    // the row that holds group r0: the thread's block of rows by its prefix, then row by row
+    int lo = 0, hi = kThreads;
+    while (lo + 1 < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (sm.sums[mid][col] * heads <= r0) lo = mid;
+      else hi = mid;
+    }
+    int row = lo * per;
+    int64_t at = sm.sums[lo][col] * heads;  // the row's first group
+    while (row < a.rows) {
+      const int c = padded(seen_of(a.lengths[row], a).count, d.pad);
+      if (at + static_cast<int64_t>(c) * heads > r0) break;
+      at += static_cast<int64_t>(c) * heads;
+      ++row;
+    }
+    int64_t pos = r0;
+    while (pos < r1 && row < a.rows) {
+      const Seen seen = seen_of(a.lengths[row], a);
+      const int c = padded(seen.count, d.pad);
+      if (c == 0 || at + static_cast<int64_t>(c) * heads <= pos) {
+        at += static_cast<int64_t>(c) * heads;
+        ++row;
+        continue;
+      }
+      const int head = static_cast<int>((pos - at) / c);
+      const int64_t seg = at + static_cast<int64_t>(head) * c;  // the segment's first group
+      const int u0 = static_cast<int>(pos - seg);
+      const int u1 = static_cast<int>(min(static_cast<int64_t>(seen.count), r1 - seg));
+      pos = min(r1, seg + c);
+      if (u0 >= u1) continue;  // padding only
+      const int kvh = head / blocks, h0 = kvh * share + (head % blocks) * kRows;
+      const int hn = min(kRows, share - (head % blocks) * kRows);
+      const int *table = a.table + static_cast<int64_t>(row) * a.width;
+
+      const int mine = u1 - u0 - warp > 0 ? (u1 - u0 - warp + kWarps - 1) / kWarps : 0;
+      auto group_of = [&](int it) {
+        const int u = u0 + warp + it * kWarps;
+        return u < seen.sink ? u : seen.from + (u - seen.sink);
+      };
+      int page_ids = -1;  // lane i: the page of this warp's group 32 * block + i
+      auto mask_of = [&](int g, int page) {  // bits of the group's keys that are seen
+        if (page < 0 || page >= a.pages) return 0u;
+        const int k0 = g * kKeys;
+        const uint32_t below = seen.n - k0 >= kKeys ? 0xffffu : (1u << (seen.n - k0)) - 1u;
+        const int lo_k = seen.lo - k0, sink_k = seen.sink_keys - k0;
+        const uint32_t recent = lo_k <= 0 ? 0xffffu : lo_k >= kKeys ? 0u : 0xffffu & ~((1u << lo_k) - 1u);
+        const uint32_t sinks = sink_k <= 0 ? 0u : sink_k >= kKeys ? 0xffffu : (1u << sink_k) - 1u;
+        return below & (recent | sinks);
+      };
+      auto issue = [&](int it) {
+        if (it < mine) {
+          if ((it & 31) == 0) {
+            page_ids = -1;
+            if (it + lane < mine) page_ids = table[(group_of(it + lane) * kKeys) >> a.page_shift];
+          }
+          const int page = __shfl_sync(0xffffffffu, page_ids, it & 31);
+          const int g = group_of(it);
+          const uint32_t mask = mask_of(g, page);
+          const int slot = (g * kKeys) & ((1 << a.page_shift) - 1);
+          const int64_t pg = mask ? page : 0;
+          const T *kp = kbase + pg * a.ks[0] + kvh * a.ks[1] + slot * a.ks[2] + piece * 8;
+          const T *vp = vbase + pg * a.vs[0] + kvh * a.vs[1] + slot * a.vs[2] + piece * 8;
+          const uint32_t st = ring + (it % kStages) * (2 * kKeys * DP * 2);
+          const bool real = piece * 8 < a.dim;
+#pragma unroll
+          for (int i = 0; i < kKeys / RPI; ++i) {
+            const int key = sub + i * RPI;
+            // a key that is not seen is not read: its place is zero, so nothing it holds can enter
+            const bool in = real && ((mask >> key) & 1);
+            const uint32_t dst = st + swizzled<DP>(key, piece);
+            cp_async16(dst, in ? kp + key * a.ks[2] : kbase, in);
+            cp_async16(dst + kKeys * DP * 2, in ? vp + key * a.vs[2] : vbase, in);
+          }
+        }
+        cp_async_commit();
+      };
+
+      w.load_q(a, row, h0, hn, lane);
+      w.reset();
+      int masks_page = -1;  // the pages of the groups being computed trail those being loaded
+#pragma unroll
+      for (int it = 0; it < kStages - 1; ++it) issue(it);
+      for (int it = 0; it < mine; ++it) {
+        if ((it & 31) == 0) {
+          masks_page = -1;
+          if (it + lane < mine) masks_page = table[(group_of(it + lane) * kKeys) >> a.page_shift];
+        }
+        issue(it + kStages - 1);
+        cp_async_wait<kStages - 1>();
+        __syncwarp();
+        const uint32_t st = ring + (it % kStages) * (2 * kKeys * DP * 2);
+        const uint32_t mask = mask_of(group_of(it), __shfl_sync(0xffffffffu, masks_page, it & 31));
+        w.step(st, st + kKeys * DP * 2, mask, scale2, lane);
+        __syncwarp();
+      }
+      cp_async_wait<0>();
+
+      // ---- the CTA's warps meet: outputs through shared memory (their own rings)
+      float *mine_o = reinterpret_cast<float *>(&sm.kv[warp][0][0][0]);
+      const int g = lane >> 2, t = lane & 3;
+      __syncwarp();
+#pragma unroll
+      for (int h = 0; h < (R8 ? 1 : 2); ++h) {
+        float l = w.l[h];
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        if (t == 0) sm.ml[warp][g + 8 * h][0] = w.m[h], sm.ml[warp][g + 8 * h][1] = l;
+#pragma unroll
+        for (int j = 0; j < DP / 8; ++j)
+          *reinterpret_cast<float2 *>(mine_o + (g + 8 * h) * DP + 8 * j + 2 * t) =
+              make_float2(w.o[j][2 * h], w.o[j][2 * h + 1]);
+      }
+      __syncthreads();
+      const bool whole = u0 == 0 && u1 == seen.count;
+      const int64_t slot = dense ? 2 * range + (seg > r0 ? 1 : 0) : range;
+      for (int i = tid; i < hn * DP; i += kThreads) {
+        const int r = i / DP, c2 = i % DP;
+        float m = -INFINITY, l = 0.f, o = 0.f;
+#pragma unroll
+        for (int v = 0; v < kWarps; ++v) m = fmaxf(m, sm.ml[v][r][0]);
+#pragma unroll
+        for (int v = 0; v < kWarps; ++v) {
+          const float f = weight(sm.ml[v][r][0], m);
+          l += f * sm.ml[v][r][1];
+          o += f * reinterpret_cast<const float *>(&sm.kv[v][0][0][0])[r * DP + c2];
+        }
+        if (whole) {
+          const int64_t out = static_cast<int64_t>(row) * a.q_heads + h0 + r;
+          if (c2 < a.dim) store1(static_cast<T *>(a.out) + out * a.dim + c2, l == 0.f ? 0.f : o / l);
+          if (c2 == 0 && a.lse) a.lse[out] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+        } else {
+          ws.o[(slot * kRows + r) * DP + c2] = o;
+          if (c2 == 0) ws.ml[(slot * kRows + r) * 2] = m, ws.ml[(slot * kRows + r) * 2 + 1] = l;
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// Joins the partial results of one segment's ranges, in their order; segments that no
+// range covers (rows that see nothing) get zeros.
+template <typename T, int DP>
+__global__ void __launch_bounds__(128) attn_join_kernel(AttnArgs a, Ws ws, int blocks, int share) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int heads = a.kv_heads * blocks;
+  const int row = blockIdx.x / heads, head = blockIdx.x % heads;
+  const int range = ws.deal[0], pad = ws.deal[1];
+  const int kvh = head / blocks, h0 = kvh * share + (head % blocks) * kRows;
+  const int hn = min(kRows, share - (head % blocks) * kRows);
+  const int count = seen_of(a.lengths[row], a).count;
+  const int64_t seg = ws.start[row] * heads + static_cast<int64_t>(head) * padded(count, pad);
+  const int64_t f = seg / range, e = count ? (seg + count - 1) / range : f;
+  if (count && f == e) return;  // one range had it whole
+  for (int i = threadIdx.x; i < hn * DP; i += 128) {
+    const int r = i / DP, c = i % DP;
+    float m = -INFINITY, l = 0.f, o = 0.f;
+    if (count)
+      for (int64_t x = f; x <= e; ++x) {
+        const int64_t slot = pad == 1 ? 2 * x + (x == f && seg > x * range ? 1 : 0) : x;
+        const float m2 = ws.ml[(slot * kRows + r) * 2], l2 = ws.ml[(slot * kRows + r) * 2 + 1];
+        const float o2 = ws.o[(slot * kRows + r) * DP + c];
+        const float mn = fmaxf(m, m2);
+        const float p = weight(m, mn), q = weight(m2, mn);
+        l = l * p + l2 * q;
+        o = o * p + o2 * q;
+        m = mn;
+      }
+    const int64_t out = static_cast<int64_t>(row) * a.q_heads + h0 + r;
+    if (c < a.dim) store1(static_cast<T *>(a.out) + out * a.dim + c, l == 0.f ? 0.f : o / l);
+    if (c == 0 && a.lse) a.lse[out] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+  }
+}
+
+struct Shape {
+  int64_t heads, slots;
+  int dp;
+};
+
+Shape shape_of(int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t dim) {
+  Shape s;
+  s.heads = kv_heads * ceil_div(q_heads / kv_heads, kRows);
+  // equal ranges leave up to two partial results each; short ranges one, and there are
+  // no more of them than the CTAs plus one for each segment's last
+  const int64_t grid = 148 * kCtasPerSm;
+  s.slots = 2 * grid > grid + rows * s.heads ? 2 * grid : grid + rows * s.heads;
+  s.dp = dim <= 64 ? 64 : 128;
+  return s;
+}
+
+template <typename T, int DP, bool R8>
+int run(const AttnArgs &a, const Ws &ws, int blocks, int share, cudaStream_t s) {
+  auto kern = attn_decode_kernel<T, DP, R8>;
+  static const cudaError_t attr =
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(Smem<T, DP>)));
+  if (attr != cudaSuccess) return fail(QS_ERR_CUDA, "attention (decode): %s", cudaGetErrorString(attr));
+  const int grid = 148 * kCtasPerSm;
+  int st = launch_pdl("attention (decode)", kern, dim3(grid), dim3(kThreads), sizeof(Smem<T, DP>), s, a, ws, blocks,
+                      share);
+  if (st) return st;
+  return launch_pdl("attention (join)", attn_join_kernel<T, DP>,
+                    dim3(static_cast<unsigned>(a.rows * a.kv_heads * blocks)), dim3(128), 0, s, a, ws, blocks, share);
+}
+
+template <typename T>
+int run_type(const AttnArgs &a, const Ws &ws, int blocks, int share, cudaStream_t s) {
+  if (a.dim <= 64)
+    return share <= 8 ? run<T, 64, true>(a, ws, blocks, share, s) : run<T, 64, false>(a, ws, blocks, share, s);
+  return share <= 8 ? run<T, 128, true>(a, ws, blocks, share, s) : run<T, 128, false>(a, ws, blocks, share, s);
+}
+
+}  // namespace
+
+int64_t attn_decode_workspace_bytes(int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t dim) {
+  const Shape s = shape_of(rows, q_heads, kv_heads, dim);
+  return round_up((rows + 1) * 8 + 8, 256) + s.slots * kRows * (s.dp + 2) * 4;
+}
+
+int launch_attn_decode(const AttnArgs &a, cudaStream_t s) {
+  const int share = a.q_heads / a.kv_heads, blocks = static_cast<int>(ceil_div(share, kRows));
+  const Shape sh = shape_of(a.rows, a.q_heads, a.kv_heads, a.dim);
+  Ws ws;
+  ws.start = static_cast<int64_t *>(a.ws);
+  ws.deal = reinterpret_cast<int *>(ws.start + a.rows + 1);
+  ws.ml = reinterpret_cast<float *>(static_cast<char *>(a.ws) + round_up((a.rows + 1) * int64_t(8) + 8, 256));
+  ws.o = ws.ml + sh.slots * kRows * 2;
+  return a.dtype == QS_F16 ? run_type<__half>(a, ws, blocks, share, s)
+                           : run_type<__nv_bfloat16>(a, ws, blocks, share, s);
+}
+
+}  // namespace qs

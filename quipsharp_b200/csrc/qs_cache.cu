@@ -1,0 +1,543 @@
+// Pages of a key-value cache: fork (share, copy, free, reorder), compact, extend
+// and the write of new tokens' keys and values.
+//
+// State: a page table (rows x width page numbers), the rows' lengths, and a
+// reference count per page.  A page is free when its count is 0; the lowest free
+// page is taken first, so every result is a function of the inputs alone (no
+// free list, no order of arrival).  The bookkeeping of one call is one launch of
+// one thread-block cluster (its phases follow one another through cluster
+// barriers, a microsecond each, where separate launches or a grid barrier cost
+// more); the page contents then move in a second launch over the whole GPU.
+//
+// Nothing here computes: the bound is the bytes moved (the rows copied, once in
+// and once out) plus the two launches.
+#include "qs_common.cuh"
+#include "qs_launch.h"
+
+namespace qs {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+
+// Raised by the kernels, read and cleared by qs_device_status.
+__device__ int g_cache_error;
+
+__device__ __forceinline__ void flag_error(int bit) { atomicOr(&g_cache_error, bit); }
+
+__device__ __forceinline__ int cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return static_cast<int>(r);
+}
+__device__ __forceinline__ int cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return static_cast<int>(r);
+}
+// Barrier of every thread of the cluster; global writes before it are seen after it.
+__device__ __forceinline__ void cluster_barrier() {
+  __threadfence();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Exclusive prefix of v over the block's threads; *total gets the sum.
+__device__ __forceinline__ int block_prefix(int v, int *total, int *tmp) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, d);
+    if (lane >= d) x += y;
+  }
+  if (lane == 31) tmp[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int w = lane < kWarps ? tmp[lane] : 0;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, w, d);
+      if (lane >= d) w += y;
+    }
+    if (lane < kWarps) tmp[lane] = w;
+  }
+  __syncthreads();
+  const int before = (warp ? tmp[warp - 1] : 0) + x - v;
+  *total = tmp[kWarps - 1];
+  __syncthreads();
+  return before;
+}
+
+// Workspace of a bookkeeping launch (int32 words).
+struct Work {
+  int *head;    // [64]: 0 = entries of list, 1 = moves of a compaction, 8.. = one count per CTA
+  int *a, *b;   // [pages] each
+  int *map;     // [pages]
+  int4 *list;   // copies: source page, destination page, tokens
+};
+
+Work split_work(void *ws, int64_t rows, int64_t pages) {
+  Work w;
+  w.head = static_cast<int *>(ws);
+  w.list = reinterpret_cast<int4 *>(w.head + 64);
+  w.a = w.head + 64 + 4 * (rows + pages);
+  w.b = w.a + pages;
+  w.map = w.b + pages;
+  return w;
+}
+
+// This CTA's pages [lo, hi): equal shares in page order.
+__device__ __forceinline__ void share_of(int pages, int *lo, int *hi) {
+  const int each = (pages + cluster_size() - 1) / cluster_size();
+  *lo = min(pages, each * cluster_rank());
+  *hi = min(pages, *lo + each);
+}
+
+// Sum of the counts of the CTAs before this one (and of all), after every CTA wrote head[8 + rank].
+__device__ __forceinline__ int counts_before(const int *head, int *total) {
+  int before = 0, all = 0;
+  for (int r = 0; r < cluster_size(); ++r) {
+    const int c = __ldcg(head + 8 + r);
+    if (r < cluster_rank()) before += c;
+    all += c;
+  }
+  *total = all;
+  return before;
+}
+
+// Numbers this CTA's share of the pages with pred true, in page order, from the
+// cluster-wide prefix: emit(page, rank) for each.  All threads call it; the first
+// pass counts, a cluster barrier exchanges the counts, the second pass numbers.
+template <class Pred, class Emit>
+__device__ __forceinline__ int number_pages(int pages, int *head, int *tmp, Pred pred, Emit emit) {
+  int lo, hi;
+  share_of(pages, &lo, &hi);
+  int mine = 0;
+  for (int p = lo + threadIdx.x; p < hi; p += kThreads) mine += pred(p) ? 1 : 0;
+  int total;
+  block_prefix(mine, &total, tmp);
+  if (threadIdx.x == 0) head[8 + cluster_rank()] = total;
+  cluster_barrier();
+  int all;
+  int base = counts_before(head, &all);
+  for (int p0 = lo; p0 < hi; p0 += kThreads) {
+    const int p = p0 + threadIdx.x;
+    const bool is = p < hi && pred(p);
+    int n;
+    const int r = base + block_prefix(is ? 1 : 0, &n, tmp);
+    if (p < hi) emit(p, r, is, all);
+    base += n;
+  }
+  return all;
+}
+
+struct Tables {
+  int rows, width, pages, page_shift;
+  const int *table, *lengths, *refcount;
+  int *table_out, *lengths_out, *refcount_out;
+};
+
+__device__ __forceinline__ int pages_of(int64_t n, int shift, int width) {
+  return static_cast<int>(min(static_cast<int64_t>(width), (n + (1 << shift) - 1) >> shift));
+}
+
+// ---- fork ------------------------------------------------------------------------
+// Row i becomes a copy of row parent[i] of the input tables (-1: empty).  Whole
+// pages are shared; a part-filled last page stays with the first child, and the
+// other children get a page of their own, whose filled tokens the second launch
+// copies.  Counts change by references after minus references before, so counts
+// that the caller holds besides the table's stay.
+__global__ void __launch_bounds__(kThreads) fork_kernel(Tables t, const int *parents, Work w) {
+  extern __shared__ int sm[];
+  __shared__ int tmp[32];
+  int *first = sm, *kids = sm + t.rows, *rank = sm + 2 * t.rows;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int nthreads = kThreads * cluster_size(), tid = cluster_rank() * kThreads + threadIdx.x;
+  auto parent = [&](int i) {
+    const int p = parents[i];
+    return p >= 0 && p < t.rows ? p : -1;
+  };
+  auto length = [&](int i) { return max(0, t.lengths[i]); };
+  for (int i = threadIdx.x; i < t.rows; i += kThreads) first[i] = t.rows, kids[i] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < t.rows; i += kThreads) {
+    const int p = parent(i);
+    if (p >= 0) {
+      atomicAdd(&kids[p], 1);
+      atomicMin(&first[p], i);
+    } else if (parents[i] != -1 && cluster_rank() == 0) {
+      flag_error(kCacheErrParent);
+    }
+  }
+  __syncthreads();
+  // rows that need a page of their own, numbered in row order
+  int want = 0;
+  for (int i0 = 0; i0 < t.rows; i0 += kThreads) {
+    const int i = i0 + threadIdx.x;
+    bool dup = false;
+    if (i < t.rows) {
+      const int p = parent(i);
+      if (p >= 0 && first[p] != i) {
+        const int n = length(p);
+        dup = (n & ((1 << t.page_shift) - 1)) != 0 && (n >> t.page_shift) < t.width;
+      }
+    }
+    int n;
+    const int r = want + block_prefix(dup ? 1 : 0, &n, tmp);
+    if (i < t.rows) rank[i] = dup ? r : -1;
+    want += n;
+  }
+  int lo, hi;
+  share_of(t.pages, &lo, &hi);
+  for (int p = lo + threadIdx.x; p < hi; p += kThreads) t.refcount_out[p] = t.refcount[p];
+  cluster_barrier();
+  const int lane = threadIdx.x & 31;
+  for (int i = tid >> 5; i < t.rows; i += nthreads >> 5) {
+    {  // references of the old row that go or come
+      const int n = length(i), used = pages_of(n, t.page_shift, t.width), delta = kids[i] - 1;
+      const int whole = min(used, n >> t.page_shift);
+      const int *row = t.table + static_cast<int64_t>(i) * t.width;
+      for (int c = lane; c < used; c += 32) {
+        const int d = c < whole ? delta : (kids[i] ? 0 : -1);
+        const int p = row[c];
+        if (d != 0 && p >= 0 && p < t.pages) atomicAdd(t.refcount_out + p, d);
+      }
+    }
+    const int p = parent(i), n = p < 0 ? 0 : length(p), used = pages_of(n, t.page_shift, t.width);
+    const int *row = t.table + static_cast<int64_t>(p) * t.width;
+    int *out = t.table_out + static_cast<int64_t>(i) * t.width;
+    const int keep = used - (rank[i] >= 0 ? 1 : 0);  // the last entry of a copying row follows below
+    for (int c = lane; c < t.width; c += 32)
+      if (c < keep || c >= used) out[c] = c < used ? row[c] : -1;
+    if (lane == 0) t.lengths_out[i] = n;
+  }
+  cluster_barrier();
+  const int free_pages = number_pages(
+      t.pages, w.head, tmp, [&](int p) { return __ldcg(t.refcount_out + p) == 0; },
+      [&](int p, int r, bool is, int) {
+        if (is && r < want) w.a[r] = p;
+      });
+  cluster_barrier();
+  for (int i = tid; i < t.rows; i += nthreads) {
+    const int r = rank[i];
+    if (r < 0) continue;
+    const int p = parent(i), n = length(p), last = n >> t.page_shift;
+    const int page = r < free_pages ? __ldcg(w.a + r) : -1;
+    t.table_out[static_cast<int64_t>(i) * t.width + last] = page;
+    if (page >= 0) t.refcount_out[page] = 1;
+    else flag_error(kCacheErrPages);
+    w.list[r] = make_int4(t.table[static_cast<int64_t>(p) * t.width + last], page, n & ((1 << t.page_shift) - 1), 0);
+  }
+  if (tid == 0) w.head[0] = want;
+}
+
+// ---- compact ---------------------------------------------------------------------
+// With U pages in use, the used pages from U on move to the holes below U, both in
+// ascending order; tables and counts follow.
+__global__ void __launch_bounds__(kThreads) compact_kernel(Tables t, int *used_out, Work w) {
+  __shared__ int tmp[32];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int nthreads = kThreads * cluster_size(), tid = cluster_rank() * kThreads + threadIdx.x;
+  if (tid == 0) w.head[1] = 0;
+  // rank = used pages before p.  A hole p < U is number p - rank among the holes; a
+  // used page p >= U goes by its rank, and those ranks end at U - 1.
+  const int used = number_pages(
+      t.pages, w.head, tmp, [&](int p) { return t.refcount[p] > 0; },
+      [&](int p, int r, bool is, int all) {
+        t.refcount_out[p] = t.refcount[p];
+        w.map[p] = p;
+        if (is && p >= all) w.a[r] = p;
+        if (!is && p < all) w.b[p - r] = p;
+        if (p == all) w.head[1] = all - r;  // holes below U
+      });
+  cluster_barrier();
+  const int moves = __ldcg(w.head + 1);
+  for (int m = tid; m < moves; m += nthreads) {
+    const int src = __ldcg(w.a + used - moves + m), dst = __ldcg(w.b + m);
+    w.map[src] = dst;
+    t.refcount_out[dst] = t.refcount[src];
+    t.refcount_out[src] = 0;
+    w.list[m] = make_int4(src, dst, 1 << t.page_shift, 0);
+  }
+  if (tid == 0) {
+    w.head[0] = moves;
+    used_out[0] = used;
+  }
+  cluster_barrier();
+  const int lane = threadIdx.x & 31;
+  for (int i = tid >> 5; i < t.rows; i += nthreads >> 5) {
+    const int n = pages_of(max(0, t.lengths[i]), t.page_shift, t.width);
+    for (int c = lane; c < t.width; c += 32) {
+      const int64_t at = static_cast<int64_t>(i) * t.width + c;
+      const int p = c < n ? t.table[at] : -1;
+      t.table_out[at] = p >= 0 && p < t.pages ? __ldcg(w.map + p) : -1;
+    }
+  }
+}
+
+// ---- extend ----------------------------------------------------------------------
+// Row i grows by add[i] tokens; its new pages are the lowest free ones, numbered in
+// row and then column order.
+__global__ void __launch_bounds__(kThreads) extend_kernel(Tables t, const int *add, Work w) {
+  extern __shared__ int sm[];
+  __shared__ int tmp[32];
+  int *start = sm, *had_s = sm + t.rows, *len_s = sm + 2 * t.rows;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int nthreads = kThreads * cluster_size(), tid = cluster_rank() * kThreads + threadIdx.x;
+  int want = 0;
+  for (int i0 = 0; i0 < t.rows; i0 += kThreads) {
+    const int i = i0 + threadIdx.x;
+    int need = 0;
+    if (i < t.rows) {
+      const int n = max(0, t.lengths[i]), a = add[i];
+      const int64_t m = static_cast<int64_t>(n) + max(0, a);
+      const int had = pages_of(n, t.page_shift, t.width);
+      need = pages_of(m, t.page_shift, t.width) - had;
+      had_s[i] = had;
+      len_s[i] = static_cast<int>(min(m, static_cast<int64_t>(0x7fffffff)));
+      if (cluster_rank() == 0) {
+        if (a < 0) flag_error(kCacheErrParent);
+        if (m > (static_cast<int64_t>(t.width) << t.page_shift)) flag_error(kCacheErrPages);
+      }
+    }
+    int n;
+    const int before = want + block_prefix(need, &n, tmp);
+    if (i < t.rows) start[i] = before;
+    want += n;
+  }
+  const int free_pages = number_pages(
+      t.pages, w.head, tmp, [&](int p) { return t.refcount[p] == 0; },
+      [&](int p, int r, bool is, int) {
+        const bool take = is && r < want;
+        if (take) w.a[r] = p;
+        w.b[p] = take ? 1 : t.refcount[p];
+      });
+  if (tid == 0 && want > free_pages) flag_error(kCacheErrPages);
+  cluster_barrier();
+  // the outputs may be the inputs: every input value was read before the last barrier,
+  // except the table entries that stay where they are
+  for (int p = tid; p < t.pages; p += nthreads) t.refcount_out[p] = __ldcg(w.b + p);
+  const int lane = threadIdx.x & 31;
+  for (int i = tid >> 5; i < t.rows; i += nthreads >> 5) {
+    const int had = had_s[i], has = pages_of(len_s[i], t.page_shift, t.width);
+    for (int c = lane; c < t.width; c += 32) {
+      const int64_t at = static_cast<int64_t>(i) * t.width + c;
+      int p = -1;
+      if (c < had) p = t.table[at];
+      else if (c < has && start[i] + c - had < free_pages) p = __ldcg(w.a + start[i] + c - had);
+      t.table_out[at] = p;
+    }
+    if (lane == 0) t.lengths_out[i] = len_s[i];
+  }
+}
+
+// ---- moving page contents ------------------------------------------------------------
+struct Pool {
+  char *k, *v;
+  int layers, pages, heads, chunks;  // chunks: 16-byte pieces of one token's row of one head
+  int64_t ks[4], vs[4];              // strides in bytes: layer, page, head, token
+};
+
+Pool make_pool(const qs_kv_pool &p) {
+  Pool q;
+  q.k = static_cast<char *>(p.k);
+  q.v = static_cast<char *>(p.v);
+  q.layers = static_cast<int>(p.layers);
+  q.pages = static_cast<int>(p.pages);
+  q.heads = static_cast<int>(p.heads);
+  q.chunks = static_cast<int>(p.dim / 8);
+  for (int i = 0; i < 4; ++i) q.ks[i] = p.k_stride[i] * 2, q.vs[i] = p.v_stride[i] * 2;
+  return q;
+}
+
+// A warp takes one (copy, layer, K or V, head): `tokens` rows of `chunks` 16-byte pieces.
+constexpr int kCopyUnroll = 8;
+__global__ void __launch_bounds__(256) copy_pages_kernel(Pool p, const int *head, const int4 *list) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const int64_t units = static_cast<int64_t>(head[0]) * p.layers * 2 * p.heads;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
+  for (int64_t u = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5); u < units; u += step) {
+    const int h = static_cast<int>(u % p.heads);
+    int64_t r = u / p.heads;
+    const bool is_v = r & 1;
+    r >>= 1;
+    const int layer = static_cast<int>(r % p.layers);
+    const int4 e = list[r / p.layers];
+    if (e.x < 0 || e.x >= p.pages || e.y < 0 || e.y >= p.pages) continue;
+    const int64_t *st = is_v ? p.vs : p.ks;
+    char *base = (is_v ? p.v : p.k) + layer * st[0] + h * st[2];
+    const char *src = base + e.x * st[1];
+    char *dst = base + e.y * st[1];
+    const int n = e.z * p.chunks;
+    for (int i0 = lane; i0 < n; i0 += 32 * kCopyUnroll) {
+      uint4 x[kCopyUnroll];
+      int64_t off[kCopyUnroll];
+#pragma unroll
+      for (int j = 0; j < kCopyUnroll; ++j) {
+        const int i = i0 + 32 * j;
+        if (i < n) {
+          off[j] = (i / p.chunks) * st[3] + (i % p.chunks) * 16;
+          x[j] = *reinterpret_cast<const uint4 *>(src + off[j]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kCopyUnroll; ++j)
+        if (i0 + 32 * j < n) *reinterpret_cast<uint4 *>(dst + off[j]) = x[j];
+    }
+  }
+}
+
+// ---- writing new tokens ------------------------------------------------------------
+struct WriteArgs {
+  Pool p;
+  int rows, width, page_shift, tokens;
+  const int *table, *lengths, *cu;  // cu null: token t is the newest of row t
+  const char *k, *v;
+  int64_t k_token, k_head, v_token, v_head;  // bytes
+};
+
+// A warp per token: its place is its row's length before the call plus its number
+// among the row's new tokens.  Tokens without a page are left out.
+__global__ void __launch_bounds__(256) write_kernel(WriteArgs a) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const int tok = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (tok >= a.tokens) return;
+  int row = tok, back = 1;  // back: tokens from this one to the row's end
+  if (a.cu) {
+    int lo = 0, hi = a.rows;  // first row whose end is past tok
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (a.cu[mid + 1] > tok) hi = mid;
+      else lo = mid + 1;
+    }
+    row = lo;
+    if (row < a.rows) back = a.cu[row + 1] - tok;
+  }
+  if (row >= a.rows) return;
+  const int pos = a.lengths[row] - back;
+  if (pos < 0 || (pos >> a.page_shift) >= a.width) return;
+  const int page = a.table[static_cast<int64_t>(row) * a.width + (pos >> a.page_shift)];
+  if (page < 0 || page >= a.p.pages) return;
+  const int slot = pos & ((1 << a.page_shift) - 1);
+  const int n = a.p.heads * a.p.chunks;
+  for (int i = lane; i < n; i += 32) {
+    const int h = i / a.p.chunks, c = i % a.p.chunks;
+    const uint4 x = *reinterpret_cast<const uint4 *>(a.k + tok * a.k_token + h * a.k_head + c * 16);
+    const uint4 y = *reinterpret_cast<const uint4 *>(a.v + tok * a.v_token + h * a.v_head + c * 16);
+    *reinterpret_cast<uint4 *>(a.p.k + page * a.p.ks[1] + h * a.p.ks[2] + slot * a.p.ks[3] + c * 16) = x;
+    *reinterpret_cast<uint4 *>(a.p.v + page * a.p.vs[1] + h * a.p.vs[2] + slot * a.p.vs[3] + c * 16) = y;
+  }
+}
+
+// One CTA while a scan of the counts and the tables is short; a cluster of eight
+// shares longer ones.
+int cluster_for(int64_t rows, int64_t width, int64_t pages) { return rows * width + pages <= 32768 ? 1 : 8; }
+
+template <typename... KArgs, typename... Args>
+int launch_cluster(const char *what, void (*kern)(KArgs...), int ctas, size_t smem, cudaStream_t s, Args... args) {
+  if (smem > 48 * 1024)
+    QS_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ctas;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+  if (e != cudaSuccess) return fail(QS_ERR_CUDA, "%s launch failed: %s", what, cudaGetErrorString(e));
+  return QS_OK;
+}
+
+int log2_of(int64_t v) {
+  int s = 0;
+  while ((int64_t(1) << s) < v) ++s;
+  return s;
+}
+
+int launch_copy(const qs_kv_pool &pool, const Work &w, cudaStream_t s) {
+  return launch_pdl("copy_pages", copy_pages_kernel, dim3(device_sms() * 8), dim3(256), 0, s, make_pool(pool),
+                    static_cast<const int *>(w.head), static_cast<const int4 *>(w.list));
+}
+
+}  // namespace
+
+int64_t cache_workspace_bytes(int64_t rows, int64_t pages) { return (64 + 4 * (rows + pages) + 3 * pages) * 4; }
+
+int device_sms() {
+  static int cached[64] = {0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && cached[dev]) return cached[dev];
+  int n = 148;
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  if (dev >= 0 && dev < 64) cached[dev] = n;
+  return n;
+}
+
+int take_cache_errors(int *bits, cudaStream_t s) {
+  static const int zero = 0;
+  *bits = 0;
+  QS_CUDA_TRY(cudaMemcpyFromSymbolAsync(bits, g_cache_error, sizeof(int), 0, cudaMemcpyDeviceToHost, s));
+  QS_CUDA_TRY(cudaStreamSynchronize(s));
+  if (*bits) {
+    QS_CUDA_TRY(cudaMemcpyToSymbolAsync(g_cache_error, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s));
+    QS_CUDA_TRY(cudaStreamSynchronize(s));
+  }
+  return QS_OK;
+}
+
+int launch_cache_fork(const qs_kv_pool &pool, int rows, int width, const int *table, const int *lengths,
+                      const int *refcount, const int *parents, int *table_out, int *lengths_out, int *refcount_out,
+                      void *ws, cudaStream_t s) {
+  const Tables t{rows, width, static_cast<int>(pool.pages), log2_of(pool.page), table, lengths, refcount,
+                 table_out, lengths_out, refcount_out};
+  const Work w = split_work(ws, rows, pool.pages);
+  const int st = launch_cluster("cache fork", fork_kernel, cluster_for(rows, width, pool.pages),
+                                static_cast<size_t>(rows) * 12, s, t, parents, w);
+  return st ? st : launch_copy(pool, w, s);
+}
+
+int launch_cache_compact(const qs_kv_pool &pool, int rows, int width, const int *table, const int *lengths,
+                         const int *refcount, int *table_out, int *refcount_out, int *used_out, void *ws,
+                         cudaStream_t s) {
+  const Tables t{rows, width, static_cast<int>(pool.pages), log2_of(pool.page), table, lengths, refcount,
+                 table_out, nullptr, refcount_out};
+  const Work w = split_work(ws, rows, pool.pages);
+  const int st = launch_cluster("cache compact", compact_kernel, cluster_for(rows, width, pool.pages), 0, s, t,
+                                used_out, w);
+  return st ? st : launch_copy(pool, w, s);
+}
+
+int launch_cache_extend(int64_t page, int64_t pages, int rows, int width, const int *table, const int *lengths,
+                        const int *refcount, const int *add, int *table_out, int *lengths_out, int *refcount_out,
+                        void *ws, cudaStream_t s) {
+  const Tables t{rows, width, static_cast<int>(pages), log2_of(page), table, lengths, refcount,
+                 table_out, lengths_out, refcount_out};
+  return launch_cluster("cache extend", extend_kernel, cluster_for(rows, width, pages), static_cast<size_t>(rows) * 12,
+                        s, t, add, split_work(ws, rows, pages));
+}
+
+int launch_cache_write(const qs_kv_pool &pool, int rows, int width, const int *table, const int *lengths,
+                       const int *cu, const void *k, int64_t k_token, int64_t k_head, const void *v, int64_t v_token,
+                       int64_t v_head, int64_t tokens, cudaStream_t s) {
+  const WriteArgs a{make_pool(pool), rows, width, log2_of(pool.page), static_cast<int>(tokens), table, lengths, cu,
+                    static_cast<const char *>(k), static_cast<const char *>(v), k_token * 2, k_head * 2,
+                    v_token * 2, v_head * 2};
+  return launch_pdl("cache write", write_kernel, dim3(static_cast<unsigned>(ceil_div(tokens, 8))), dim3(256), 0, s, a);
+}
+
+}  // namespace qs

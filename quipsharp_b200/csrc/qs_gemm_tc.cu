@@ -572,20 +572,43 @@ using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_
                                    const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-int encode_fp16_rows_map(CUtensorMap *map, const void *x2h, int64_t n_pad, int64_t rows, int box_x, int box_y,
-                         bool swizzle128) {
+static int encode_tiled_fn(EncodeTiledFn *out) {
   static EncodeTiledFn fn = nullptr;
   static std::mutex mu;
-  {
-    std::lock_guard<std::mutex> lock(mu);
-    if (!fn) {
-      void *p = nullptr;
-      cudaDriverEntryPointQueryResult q;
-      QS_CUDA_TRY(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q));
-      if (!p || q != cudaDriverEntryPointSuccess) return fail(QS_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-    }
+  std::lock_guard<std::mutex> lock(mu);
+  if (!fn) {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    QS_CUDA_TRY(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q));
+    if (!p || q != cudaDriverEntryPointSuccess) return fail(QS_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+    fn = reinterpret_cast<EncodeTiledFn>(p);
   }
+  *out = fn;
+  return QS_OK;
+}
+
+int encode_16bit_map(CUtensorMap *map, const void *base, bool bf16, int rank, const int64_t *dims,
+                     const int64_t *strides, const int *box) {
+  EncodeTiledFn fn;
+  const int st = encode_tiled_fn(&fn);
+  if (st) return st;
+  cuuint64_t d[5], s[4];
+  cuuint32_t b[5], one[5];
+  for (int i = 0; i < rank; ++i) d[i] = dims[i], b[i] = box[i], one[i] = 1;
+  for (int i = 0; i + 1 < rank; ++i) s[i] = strides[i] * 2;
+  const CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
+                        const_cast<void *>(base), d, s, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(QS_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+  return QS_OK;
+}
+
+int encode_fp16_rows_map(CUtensorMap *map, const void *x2h, int64_t n_pad, int64_t rows, int box_x, int box_y,
+                         bool swizzle128) {
+  EncodeTiledFn fn;
+  const int st = encode_tiled_fn(&fn);
+  if (st) return st;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(n_pad), static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(n_pad * 2)};
   const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_x), static_cast<cuuint32_t>(box_y)};
@@ -698,6 +721,12 @@ int device_status(cudaStream_t s) {
     return fail(QS_ERR_TIMEOUT, "a bounded wait timed out (prefill matmul pipeline or tensor-parallel shard arrival); "
                 "the results of that launch are invalid");
   }
+  int bits = 0;
+  const int st = take_cache_errors(&bits, s);
+  if (st) return st;
+  if (bits & kCacheErrPages)
+    return fail(QS_ERR_PAGES, "a cache row found no free page, or outgrew its page table row; its new tokens have no page");
+  if (bits & kCacheErrParent) return fail(QS_ERR_INDEX, "a cache row's parent or token count was out of range");
   return QS_OK;
 }
 

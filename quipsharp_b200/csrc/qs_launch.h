@@ -107,6 +107,10 @@ int *device_error_flag();
 // a box of box_x elements x box_y rows; 128-byte swizzle or none.
 int encode_fp16_rows_map(::CUtensorMap_st *map, const void *x2h, int64_t n_pad, int64_t rows, int box_x, int box_y,
                          bool swizzle128);
+// Tensor map over 16-bit values, up to 5 dimensions (innermost first; strides in
+// elements of all but the innermost), 128-byte swizzle, zeros outside.
+int encode_16bit_map(::CUtensorMap_st *map, const void *base, bool bf16, int rank, const int64_t *dims,
+                     const int64_t *strides, const int *box);
 // Limit (ns) of every bounded wait between the warps of a pipelined kernel
 // (mbarrier waits); a wait that runs out sets the device error flag.  Drains of
 // a CTA's own asynchronous copies and tensor-core work keep a fixed 4 s limit.
@@ -117,5 +121,57 @@ void set_pipeline_wait_ns(uint64_t ns);
 // decoded weights in shared memory); smaller ones the mma.sync decode-regime
 // kernel (weights decoded in registers, passes of 8 or 16 tokens).
 constexpr int64_t kTcMinBatch = 33;
+
+// qs_cache.cu: pages of a key-value cache
+constexpr int kCacheErrPages = 1;   // a row found no free page, or outgrew its table row
+constexpr int kCacheErrParent = 2;  // a parent outside [-1, rows), or a negative token count
+constexpr int kCacheMaxRows = 8192;
+int64_t cache_workspace_bytes(int64_t rows, int64_t pages);
+int launch_cache_fork(const qs_kv_pool &pool, int rows, int width, const int *table, const int *lengths,
+                      const int *refcount, const int *parents, int *table_out, int *lengths_out, int *refcount_out,
+                      void *ws, cudaStream_t s);
+int launch_cache_compact(const qs_kv_pool &pool, int rows, int width, const int *table, const int *lengths,
+                         const int *refcount, int *table_out, int *refcount_out, int *used_out, void *ws,
+                         cudaStream_t s);
+int launch_cache_extend(int64_t page, int64_t pages, int rows, int width, const int *table, const int *lengths,
+                        const int *refcount, const int *add, int *table_out, int *lengths_out, int *refcount_out,
+                        void *ws, cudaStream_t s);
+int launch_cache_write(const qs_kv_pool &pool, int rows, int width, const int *table, const int *lengths,
+                       const int *cu, const void *k, int64_t k_token, int64_t k_head, const void *v, int64_t v_token,
+                       int64_t v_head, int64_t tokens, cudaStream_t s);
+// Reads and clears the kCacheErr bits raised on the device (synchronises s).
+int take_cache_errors(int *bits, cudaStream_t s);
+int device_sms();  // of the current device
+
+// Arguments of attention over one layer of the cache (strides in elements).
+struct AttnArgs {
+  const void *q;
+  int64_t q_token, q_head;
+  const void *k, *v;
+  int64_t ks[3], vs[3];  // page, head, token
+  int dtype, dim, q_heads, kv_heads, pages, page_shift;
+  int rows, width;
+  int64_t tokens;
+  const int *table, *lengths, *cu;
+  float scale;
+  int64_t window, sinks;  // window 0: none
+  void *out;
+  float *lse;
+  void *ws;
+};
+// qs_attn_decode.cu
+int64_t attn_decode_workspace_bytes(int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t dim);
+int launch_attn_decode(const AttnArgs &a, cudaStream_t s);
+// qs_attn_window.cu
+int64_t attn_window_workspace_bytes(int64_t tokens, int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t dim);
+int launch_attn_window(const AttnArgs &a, cudaStream_t s);
+
+// qs_beam.cu
+constexpr int kBeamMaxN = 64;
+constexpr int kBeamMaxBeams = 64;
+int64_t beam_workspace_bytes(int64_t batch, int64_t beams, int64_t vocab, int64_t n);
+int launch_beam_select(const void *logits, int dtype, int64_t batch_stride, int64_t beam_stride, int64_t batch,
+                       int64_t beams, int64_t vocab, const float *scores, const uint8_t *finished, int n, int pad,
+                       float *scores_out, int *parents_out, int *tokens_out, void *ws, cudaStream_t s);
 
 }  // namespace qs
