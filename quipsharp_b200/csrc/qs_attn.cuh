@@ -4,6 +4,7 @@
 
 #include "qs_common.cuh"
 #include "qs_launch.h"
+#include "qs_pair.cuh"
 
 namespace qs {
 namespace {

@@ -15,7 +15,8 @@
 // grown by more than 2^8: until then weights up to 2^8 are exact in the float32 sum
 // and lose nothing in the 16-bit ones, and most tiles rescale nothing.
 //
-// Warps: 0 loads, 1 issues the products, then four per query tile for the softmax.
+// Warps: 0 loads, 1 issues the products (2 and 3 only fill their warpgroup), then four
+// per query tile for the softmax, to which the first four leave most of the registers.
 #include <cuda.h>
 
 #include <cmath>
@@ -35,7 +36,7 @@ struct Cfg {
   static constexpr int halves = DP / 64;
   static constexpr int tile_bytes = halves * kHalf;
   static constexpr int stages = (224 * 1024 - NQ * tile_bytes) / tile_bytes > 8 ? 8 : (224 * 1024 - NQ * tile_bytes) / tile_bytes;
-  static constexpr int threads = 64 + NQ * 128;
+  static constexpr int threads = 128 + NQ * 128;
   static constexpr int tmem_cols = NQ * (kTile + DP) <= 256 ? 256 : 512;
   static constexpr int bars = 1 + 3 * stages + 3 * NQ + 1;
   static constexpr int smem = (NQ + stages) * tile_bytes + bars * 8 + 16 + 1024;
@@ -68,6 +69,14 @@ __device__ __forceinline__ void tmem_st_32(uint32_t addr, const uint32_t *v) {
       "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]),
       "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
       "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_16(uint32_t addr, const uint32_t *v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15};" ::"r"(v[0]),
+      "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(addr)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -125,6 +134,13 @@ struct Job {
   int sink_tiles;      // key tiles from 0
   int from, tiles;     // first key after them, tiles in all
 };
+
+// Registers per thread: 168 at launch (65536 / 384, in eights); the sum over the
+// warpgroups stays 3 x 168.
+template <int N>
+__device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return min(max(v, lo), hi); }
 
@@ -244,7 +260,9 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       store1(static_cast<T *>(a.out) + at * a.dim + i % a.dim, 0.f);
       if (i % a.dim == 0 && a.lse) a.lse[at] = -INFINITY;
     }
-  } else if (warp == 0) {
+  } else if (warp < 4) {
+    if (NQ == 2) registers_down<72>();
+    if (warp == 0) {
     // ---- loads: Q once, then K and V tiles through one ring.  Lane b takes box b.
     const int boxes = kTile / w.granule, mask = (1 << a.page_shift) - 1;
     if (lane == 0) {
@@ -313,7 +331,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       for (int x = issued > S ? issued - S : 0; x < issued; ++x)
         if (!sm100::mbar_wait_bounded(full(x % S), (x / S) & 1, kDrainNs)) *w.error = 1;
     }
-  } else if (warp == 1) {
+    } else if (warp == 1) {
     // ---- products
     if (lane == 0) {
       constexpr uint32_t id_s = idesc_of<T>(kTile, false), id_o = idesc_of<T>(DP, true);
@@ -362,9 +380,11 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       sm100::umma_commit(drain);
       if (!sm100::mbar_wait_bounded(drain, 0, kDrainNs)) *w.error = 1;
     }
+    }
   } else {
+    if (NQ == 2) registers_up<216>();
     // ---- softmax: one thread per query row
-    const int t = (warp - 2) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+    const int t = (warp - 4) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_at = tmem + lanes + t * kTile, o_at = tmem + lanes + NQ * kTile + t * DP;
     const int tok = r / w.share, token = j.t0 + t * w.tokens_per_tile + tok;
@@ -410,9 +430,13 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           }
         }
       }
-      float top = s[0];
+      float tops[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-      for (int c = 1; c < kTile; ++c) top = fmaxf(top, s[c]);
+      for (int c = 4; c < kTile; c += 8)
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          tops[x] = fmaxf(fmaxf(tops[x], s[c + x]), c + 4 + x < kTile ? s[c + 4 + x] : s[c + x]);
+      const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
       const float grown = (top - m) * scale2;
       const bool renew = m == -INFINITY ? top != -INFINITY : grown > 8.f;
       if (__any_sync(0xffffffffu, renew)) {
@@ -433,16 +457,21 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         m = mn;
       }
       const float mb = m == -INFINITY ? 0.f : m * scale2;
-      float sum = 0.f;
+      const uint64_t scale_2 = pack2(scale2, scale2), mb_2 = pack2(-mb, -mb);
+      uint64_t sums[2] = {0, 0};
 #pragma unroll
-      for (int c = 0; c < kTile; c += 2) {
-        const float x = ex2(fmaf(s[c], scale2, -mb)), y = ex2(fmaf(s[c + 1], scale2, -mb));
-        sum += x + y;
-        split16<T>(x, y, raw[c / 2]);
+      for (int c = 0; c < kTile; c += 32) {
+#pragma unroll
+        for (int x = 0; x < 32; x += 2) {
+          const float2 e = unpack2(fma2(pack2(s[c + x], s[c + x + 1]), scale_2, mb_2));
+          const float p0 = ex2(e.x), p1 = ex2(e.y);
+          sums[(x >> 1) & 1] = add2(sums[(x >> 1) & 1], pack2(p0, p1));
+          split16<T>(p0, p1, raw[(c + x) / 2]);
+        }
+        tmem_st_16(s_at + c / 2, raw + c / 2);
       }
-      l += sum;
-      tmem_st_32(s_at, raw);
-      tmem_st_32(s_at + 32, raw + 32);
+      const float2 sum = unpack2(add2(sums[0], sums[1]));
+      l += sum.x + sum.y;
       tmem_st_wait();
       sm100::tc_fence_before_sync();
       sm100::mbar_arrive(p_full(t));
