@@ -15,6 +15,12 @@
 // grown by more than 2^8: until then weights up to 2^8 are exact in the float32 sum
 // and lose nothing in the 16-bit ones, and most tiles rescale nothing.
 //
+// One CTA per SM stays and takes one group of tiles after another: the grid has a block
+// for each, and a running CTA cancels the next one that has not started and does its work
+// (so the longest are begun first and none waits for a fixed share).  The loads of a
+// group begin while the one before is still being summed; with a CTA per group instead,
+// 14 to 17 us of each went into starting, the first loads and the last stores.
+//
 // Warps: 0 loads, 1 issues the products (2 and 3 only fill their warpgroup), then four
 // per query tile for the softmax, to which the first four leave most of the registers.
 #include <cuda.h>
@@ -27,7 +33,12 @@
 namespace qs {
 namespace {
 
+#ifndef VPOLY
+#define VPOLY 0
+#endif
+constexpr int kPolyPairs = VPOLY;
 constexpr int kTile = 128;            // query rows of a tile, keys of a tile
+constexpr float kMaxSum = 32768.f;
 constexpr int kHalf = kTile * 128;    // bytes of 128 rows of 64 values
 constexpr uint64_t kDrainNs = kDefaultWaitNs;
 
@@ -38,7 +49,7 @@ struct Cfg {
   static constexpr int stages = (224 * 1024 - NQ * tile_bytes) / tile_bytes > 8 ? 8 : (224 * 1024 - NQ * tile_bytes) / tile_bytes;
   static constexpr int threads = 128 + NQ * 128;
   static constexpr int tmem_cols = NQ * (kTile + DP) <= 256 ? 256 : 512;
-  static constexpr int bars = 1 + 3 * stages + 3 * NQ + 1;
+  static constexpr int bars = 3 * stages + 5 * NQ + 8;
   static constexpr int smem = (NQ + stages) * tile_bytes + bars * 8 + 16 + 1024;
 };
 
@@ -71,15 +82,84 @@ __device__ __forceinline__ void tmem_st_32(uint32_t addr, const uint32_t *v) {
       "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(addr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st_16(uint32_t addr, const uint32_t *v) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15};" ::"r"(v[0]),
-      "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
-      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(addr)
-      : "memory");
-}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// 2^t for two t on the multiply-add pipe (16 special-function lanes per SM would
+// bound the kernel if they took every exponential): t is split into the nearest integer,
+// left in the low bits of t + 1.5 * 2^23 and added to the result's exponent, and a rest f
+// in [-1/2, 1/2], whose 2^f is a polynomial of degree 4 fitted to the least relative error
+// (2.7e-6, and 4e-8 on average: a float16 weight's rounding is a hundred times that).
+// t is taken as at least -125 and at most 120; NaN gives a huge number.
+__device__ __forceinline__ float2 exp2_poly(uint64_t t) {
+  float2 x = unpack2(t);
+  x.x = min_nan(max_nan(x.x, -125.f), 120.f);
+  x.y = min_nan(max_nan(x.y, -125.f), 120.f);
+  t = pack2(x.x, x.y);
+  const uint64_t magic = pack2(12582912.f, 12582912.f), minus = pack2(-12582912.f, -12582912.f);
+  const uint64_t r = add2(t, magic);
+  const uint64_t f = fma2(add2(r, minus), pack2(-1.f, -1.f), t);
+  uint64_t p = fma2(pack2(9.570101276e-3f, 9.570101276e-3f), f, pack2(5.591785908e-2f, 5.591785908e-2f));
+  p = fma2(p, f, pack2(2.402474433e-1f, 2.402474433e-1f));
+  p = fma2(p, f, pack2(6.931217909e-1f, 6.931217909e-1f));
+  p = fma2(p, f, pack2(9.999992847e-1f, 9.999992847e-1f));
+  const float2 q = unpack2(p), n = unpack2(r);
+  return make_float2(__uint_as_float(__float_as_uint(q.x) + (__float_as_uint(n.x) << 23)),
+                     __uint_as_float(__float_as_uint(q.y) + (__float_as_uint(n.y) << 23)));
+}
+
+// 64 scores of a row (float32 in raw) to weights 2^(s scale2 + shift), as 16-bit values in
+// raw's first half; returns their sum before that rounding.  POLY of every 16 pairs go
+// through exp2_poly.
+template <typename T, int POLY>
+__device__ __forceinline__ float weights(uint32_t *raw, float scale2, float shift) {
+  const uint64_t scale_2 = pack2(scale2, scale2), shift_2 = pack2(shift, shift);
+  uint64_t sums[2] = {0, 0};
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    const uint64_t e2 = fma2(pack2(__uint_as_float(raw[2 * j]), __uint_as_float(raw[2 * j + 1])), scale_2, shift_2);
+    float2 e;
+    if (j % 16 * POLY / 16 != (j % 16 + 1) * POLY / 16) {
+      e = exp2_poly(e2);
+    } else {
+      e = unpack2(e2);
+      e.x = ex2(e.x);
+      e.y = ex2(e.y);
+    }
+    sums[j & 1] = add2(sums[j & 1], pack2(e.x, e.y));
+    split16<T>(e.x, e.y, raw[j]);
+  }
+  const float2 sum = unpack2(add2(sums[0], sums[1]));
+  return sum.x + sum.y;
+}
+
+// The largest of three; NaN if one is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// The largest of 64 scores; NaN if one is.
+__device__ __forceinline__ float top_of(const uint32_t *raw) {
+  const float *s = reinterpret_cast<const float *>(raw);
+  float tops[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+  for (int c = 4; c < 64; c += 8)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) tops[x] = max3(tops[x], s[c + x], c + 4 + x < 64 ? s[c + 4 + x] : s[c + x]);
+  return max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[3]);
+}
 
 // D[tmem] (+)= A[tmem] * B[smem], issued by one thread.
 __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -124,15 +204,22 @@ constexpr uint32_t idesc_of(int n, bool b_mn_major) {
   return sm100::idesc_f16_f32(kTile, n) | (f << 7) | (f << 10) | ((b_mn_major ? 1u : 0u) << 16);
 }
 
-// What a CTA works on.
+// The lowest n bits (none for n <= 0, all for n >= 32).
+__device__ __forceinline__ uint32_t ones_below(int n) {
+  return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u;
+}
+
+// The tiles of one block of the grid.
 struct Job {
-  int row;             // -1: none
-  int q0, q1;          // the row's tokens in q
-  int t0;              // first token of this CTA (in q)
-  int pos0;            // its place in the row
-  int keys;            // keys that any token of the CTA sees end before this
-  int sink_tiles;      // key tiles from 0
-  int from, tiles;     // first key after them, tiles in all
+  int row;          // -1: none
+  int head;         // key head
+  int q0, q1;       // the row's tokens in q
+  int t0;           // first token (in q)
+  int pos0;         // its place in the row
+  int keys;         // keys that any of the tokens sees end before this
+  int sink_tiles;   // key tiles from 0
+  int from, tiles;  // first key after them, tiles in all (0: tokens to clear, -1: no more jobs)
+  int absent;       // a page among the keys is missing
 };
 
 // Registers per thread: 168 at launch (65536 / 384, in eights); the sum over the
@@ -144,6 +231,96 @@ __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sy
 
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return min(max(v, lo), hi); }
 
+// True in one thread of a warp that is here as a whole.  The compiler knows that it is
+// one: what the product instructions take from uniform registers stays there, where a
+// test of the lane number has every operand moved by way of a loop (155 cycles for each
+// product of 64, measured).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// Takes over the next block of the grid that has not started: the answer goes to `answer`
+// (16 bytes) and completes on the barrier.
+__device__ __forceinline__ void ask_next_block(uint32_t answer, uint32_t bar) {
+  sm100::mbar_arrive_expect_tx(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer),
+               "r"(bar)
+               : "memory");
+}
+// The block taken over, or false where none was left.
+__device__ __forceinline__ bool next_block(uint32_t answer, int &x, int &y) {
+  uint32_t taken, bx, by;
+  asm volatile(
+      "{\n\t.reg .b128 a;\n\t.reg .pred p;\n\t.reg .b32 z;\n\tld.shared.b128 a, [%3];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\tselp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+      "mov.u32 %2, 0;\n\t@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, %2, z, _}, a;\n\t}"
+      : "=r"(taken), "=r"(bx), "=r"(by)
+      : "r"(answer)
+      : "memory");
+  sm100::fence_proxy_async_smem();  // read before the next answer is written
+  x = static_cast<int>(bx);
+  y = static_cast<int>(by);
+  return taken != 0;
+}
+
+// Block (x, y) of the grid as a job (a whole warp): the rows' tiles in row order, a row's
+// last tile (the most keys) first.
+__device__ __forceinline__ Job job_of(const WindowArgs &w, int x, int y, int per, int lane) {
+  const AttnArgs &a = w.a;
+  const int total_tokens = static_cast<int>(a.tokens);
+  Job j;
+  j.row = -1;
+  j.head = y;
+  j.q0 = j.q1 = j.t0 = 0;
+  int end = 0, want = x;
+  for (int r0 = 0; r0 < a.rows && j.row < 0; r0 += 32) {
+    const int r = r0 + lane;
+    int q0 = 0, q1 = 0, n = 0;
+    if (r < a.rows) {
+      q0 = clampi(a.cu[r], 0, total_tokens);
+      q1 = clampi(a.cu[r + 1], q0, total_tokens);
+      n = (q1 - q0 + per - 1) / per;
+    }
+    int sum = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += v;
+    }
+    const uint32_t who = __ballot_sync(0xffffffffu, want >= sum - n && want < sum);
+    end = max(end, __reduce_max_sync(0xffffffffu, q1));
+    if (who) {
+      const int src = __ffs(who) - 1;
+      j.row = r0 + src;
+      j.q0 = __shfl_sync(0xffffffffu, q0, src);
+      j.q1 = __shfl_sync(0xffffffffu, q1, src);
+      const int local = __shfl_sync(0xffffffffu, want - (sum - n), src), all = __shfl_sync(0xffffffffu, n, src);
+      j.t0 = j.q0 + (all - 1 - local) * per;
+    } else {
+      want -= __shfl_sync(0xffffffffu, sum, 31);
+    }
+  }
+  if (j.row >= 0) {
+    const int length = max(0, a.lengths[j.row]);
+    const int cap = static_cast<int>(min(static_cast<int64_t>(a.width) << a.page_shift, static_cast<int64_t>(0x7ffffff0)));
+    const int back = length - (j.q1 - j.q0);
+    j.pos0 = back + (j.t0 - j.q0);
+    const int last = back + min(j.q1, j.t0 + per) - 1 - j.q0;
+    j.keys = clampi(last + 1, 0, min(length, cap));
+    const int lo = a.window > 0 && j.pos0 + 1 > a.window ? static_cast<int>(j.pos0 + 1 - a.window) : 0;
+    const int sinks = static_cast<int>(min(static_cast<int64_t>(min(lo, j.keys)), a.sinks));
+    j.sink_tiles = (sinks + kTile - 1) / kTile;
+    j.from = max(lo / w.granule * w.granule, j.sink_tiles * kTile);
+    j.tiles = j.sink_tiles + max(0, (j.keys - j.from + kTile - 1) / kTile);
+  } else {  // a block beyond the tiles clears its share of the tokens that belong to no row
+    j.t0 = end + want * per;
+    j.tiles = 0;
+  }
+  return j;
+}
+
 template <typename T, int DP, int NQ>
 __global__ void __launch_bounds__(Cfg<DP, NQ>::threads, 1)
 attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
@@ -151,26 +328,27 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   using C = Cfg<DP, NQ>;
   constexpr int S = C::stages;
   extern __shared__ uint8_t dsm[];
-  __shared__ Job job_s;
-  __shared__ volatile int absent;  // a page among the keys is missing: set before its tile's loads
+  __shared__ Job jobs[2];  // the current one and the next
+  __shared__ __align__(16) uint8_t answer_s[16];
   const AttnArgs &a = w.a;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   uint8_t *base = dsm + ((1024u - (smem_u32(dsm) & 1023u)) & 1023u);
   const uint32_t q_sm = smem_u32(base), ring = q_sm + NQ * C::tile_bytes;
   const uint32_t bar0 = ring + S * C::tile_bytes;
-  const uint32_t q_full = bar0;
-  auto full = [&](int s) { return bar0 + 8u * (1 + s); };
-  auto empty = [&](int s) { return bar0 + 8u * (1 + S + s); };
-  auto landed = [&](int s) { return bar0 + 8u * (1 + 2 * S + s); };  // loads of a tile that is then cleared in part
-  auto s_full = [&](int t) { return bar0 + 8u * (1 + 3 * S + t); };
-  auto p_full = [&](int t) { return bar0 + 8u * (1 + 3 * S + NQ + t); };
-  auto o_full = [&](int t) { return bar0 + 8u * (1 + 3 * S + 2 * NQ + t); };
-  const uint32_t drain = bar0 + 8u * (1 + 3 * S + 3 * NQ);
+  auto full = [&](int s) { return bar0 + 8u * s; };
+  auto empty = [&](int s) { return bar0 + 8u * (S + s); };
+  auto landed = [&](int s) { return bar0 + 8u * (2 * S + s); };  // loads of a tile that is then cleared in part
+  auto s_full = [&](int t) { return bar0 + 8u * (3 * S + t); };
+  auto p_full = [&](int t) { return bar0 + 8u * (3 * S + NQ + t); };
+  auto o_full = [&](int t) { return bar0 + 8u * (3 * S + 2 * NQ + t); };
+  auto p_half = [&](int t) { return bar0 + 8u * (3 * S + 3 * NQ + t); };    // the first 64 keys' weights are stored
+  auto half_done = [&](int t) { return bar0 + 8u * (3 * S + 4 * NQ + t); };  // and in O
+  auto job_full = [&](int s) { return bar0 + 8u * (3 * S + 5 * NQ + s); };
+  auto job_empty = [&](int s) { return bar0 + 8u * (3 * S + 5 * NQ + 2 + s); };
+  const uint32_t q_full = bar0 + 8u * (3 * S + 5 * NQ + 4), q_empty = q_full + 8, asked = q_full + 16, drain = q_full + 24;
   uint32_t *holder = reinterpret_cast<uint32_t *>(base + (NQ + S) * C::tile_bytes + C::bars * 8);
 
   if (tid == 0) {
-    absent = 0;
-    sm100::mbar_init(q_full, 1);
     for (int s = 0; s < S; ++s) {
       sm100::mbar_init(full(s), 1);
       sm100::mbar_init(empty(s), 1);
@@ -178,208 +356,227 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     }
     for (int t = 0; t < NQ; ++t) {
       sm100::mbar_init(s_full(t), 1);
-      sm100::mbar_init(p_full(t), 128);
+      sm100::mbar_init(p_full(t), 4);
+      sm100::mbar_init(p_half(t), 4);
+      sm100::mbar_init(half_done(t), 1);
       sm100::mbar_init(o_full(t), 1);
     }
+    for (int s = 0; s < 2; ++s) {
+      sm100::mbar_init(job_full(s), 1);
+      sm100::mbar_init(job_empty(s), 1 + NQ * 128);
+    }
+    sm100::mbar_init(q_full, 1);
+    sm100::mbar_init(q_empty, 1);
+    sm100::mbar_init(asked, 1);
     sm100::mbar_init(drain, 1);
     sm100::fence_barrier_init();
+    sm100::prefetch_tmap(&qmap);
+    sm100::prefetch_tmap(&kmap);
+    sm100::prefetch_tmap(&vmap);
   }
   if (warp == 1) sm100::tmem_alloc(smem_u32(holder), C::tmem_cols);
   pdl_wait();
   pdl_launch_dependents();
-
-  // ---- which tokens: CTAs deal the rows' tiles in row order, a row's last tile (the
-  // most keys) first
-  const int per = NQ * w.tokens_per_tile;
-  const int total_tokens = static_cast<int>(a.tokens);
-  if (warp == 0) {
-    int want = blockIdx.x;
-    Job j;
-    j.row = -1;
-    j.q0 = j.q1 = j.t0 = 0;
-    int end = 0;
-    for (int r0 = 0; r0 < a.rows && j.row < 0; r0 += 32) {
-      const int r = r0 + lane;
-      int q0 = 0, q1 = 0, n = 0;
-      if (r < a.rows) {
-        q0 = clampi(a.cu[r], 0, total_tokens);
-        q1 = clampi(a.cu[r + 1], q0, total_tokens);
-        n = (q1 - q0 + per - 1) / per;
-      }
-      int x = n;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, d);
-        if (lane >= d) x += y;
-      }
-      const bool mine = want >= x - n && want < x;
-      const uint32_t who = __ballot_sync(0xffffffffu, mine);
-      end = max(end, __reduce_max_sync(0xffffffffu, q1));
-      if (who) {
-        const int src = __ffs(who) - 1;
-        j.row = r0 + src;
-        j.q0 = __shfl_sync(0xffffffffu, q0, src);
-        j.q1 = __shfl_sync(0xffffffffu, q1, src);
-        const int local = __shfl_sync(0xffffffffu, want - (x - n), src), all = __shfl_sync(0xffffffffu, n, src);
-        j.t0 = j.q0 + (all - 1 - local) * per;
-      } else {
-        want -= __shfl_sync(0xffffffffu, x, 31);
-      }
-    }
-    if (j.row >= 0) {
-      const int length = max(0, a.lengths[j.row]);
-      const int cap = static_cast<int>(min(static_cast<int64_t>(a.width) << a.page_shift, static_cast<int64_t>(0x7ffffff0)));
-      const int back = length - (j.q1 - j.q0);
-      j.pos0 = back + (j.t0 - j.q0);
-      const int last = back + min(j.q1, j.t0 + per) - 1 - j.q0;
-      j.keys = clampi(last + 1, 0, min(length, cap));
-      const int lo = w.a.window > 0 && j.pos0 + 1 > a.window ? static_cast<int>(j.pos0 + 1 - a.window) : 0;
-      const int sinks = static_cast<int>(min(static_cast<int64_t>(min(lo, j.keys)), a.sinks));
-      j.sink_tiles = (sinks + kTile - 1) / kTile;
-      j.from = max(lo / w.granule * w.granule, j.sink_tiles * kTile);
-      j.tiles = j.sink_tiles + max(0, (j.keys - j.from + kTile - 1) / kTile);
-    } else {  // a CTA without a tile clears its share of the tokens that belong to no row
-      j.t0 = end + want * per;
-      j.tiles = 0;
-    }
-    if (lane == 0) job_s = j;
-  }
   sm100::tc_fence_before_sync();
   __syncthreads();
   sm100::tc_fence_after_sync();
   const uint32_t tmem = *holder;
-  const Job j = job_s;
-  const int kvh = blockIdx.y, n = j.tiles;
-  auto key_of_tile = [&](int i) { return i < j.sink_tiles ? i * kTile : j.from + (i - j.sink_tiles) * kTile; };
+  const int per = NQ * w.tokens_per_tile;
+  auto key_of_tile = [&](const Job &j, int i) {
+    return i < j.sink_tiles ? i * kTile : j.from + (i - j.sink_tiles) * kTile;
+  };
 
-  if (n == 0) {
-    const int end = j.row >= 0 ? min(j.q1, j.t0 + per) : min(total_tokens, j.t0 + per);
-    const int count = max(0, end - j.t0) * w.share;
-    for (int i = tid; i < count * a.dim; i += C::threads) {
-      const int64_t at = static_cast<int64_t>(j.t0 + i / a.dim / w.share) * a.q_heads + kvh * w.share + i / a.dim % w.share;
-      store1(static_cast<T *>(a.out) + at * a.dim + i % a.dim, 0.f);
-      if (i % a.dim == 0 && a.lse) a.lse[at] = -INFINITY;
-    }
-  } else if (warp < 4) {
+  if (warp < 4) {
     if (NQ == 2) registers_down<72>();
     if (warp == 0) {
-    // ---- loads: Q once, then K and V tiles through one ring.  Lane b takes box b.
-    const int boxes = kTile / w.granule, mask = (1 << a.page_shift) - 1;
-    if (lane == 0) {
-      const int bytes = C::halves * 128 * w.share * w.tokens_per_tile;
-      sm100::mbar_arrive_expect_tx(q_full, NQ * bytes);
-      for (int t = 0; t < NQ; ++t)
-        for (int h = 0; h < C::halves; ++h)
-          tma_load_3d(q_sm + t * C::tile_bytes + h * kHalf, &qmap, h * 64, kvh * w.share,
-                      j.t0 + t * w.tokens_per_tile, q_full);
-    }
-    const int *table = a.table + static_cast<int64_t>(j.row) * a.width;
-    auto page_at = [&](int i) {  // lane b: the page of box b of tile i, -1 where there is none
-      const int k = key_of_tile(i) + lane * w.granule;
-      if (i >= n || lane >= boxes || k >= j.keys) return -1;
-      const int p = table[k >> a.page_shift];
-      return p >= 0 && p < a.pages ? p : -1;
-    };
-    int issued = 0;
-    uint32_t landed_phase = 0;
-    int next_page = page_at(0);
-    bool ok = true;
-    for (int i = 0; i < n && ok; ++i) {
-      const int page = next_page;
-      next_page = page_at(i + 1);
-      const int k0 = key_of_tile(i), k = k0 + lane * w.granule;
-      const uint32_t have = __ballot_sync(0xffffffffu, page >= 0);
-      const int bytes = __popc(have) * w.granule * 128 * C::halves;
-      if (__any_sync(0xffffffffu, page < 0 && lane < boxes && k < j.keys) && lane == 0) absent = 1;
-      // values of absent pages and past the last key must be zero: their weights are,
-      // but zero times what stale memory may hold need not be
-      const bool partial = __popc(have) != boxes || k0 + kTile > j.keys;
-#pragma unroll
-      for (int kv = 0; kv < 2 && ok; ++kv) {
-        const int s = issued % S, use = issued / S;
-        if (use > 0) ok = sm100::mbar_wait_warp(empty(s), (use - 1) & 1, w.wait_ns);
+      // ---- jobs, and loads: Q, then K and V tiles through one ring.  Lane b takes box b.
+      const int boxes = kTile / w.granule, mask = (1 << a.page_shift) - 1;
+      const uint32_t answer = smem_u32(answer_s);
+      int issued = 0, q_loads = 0, asks = 0, answers = 0;
+      uint32_t landed_phase = 0;
+      bool ok = true;
+      int bx = blockIdx.x, by = blockIdx.y;
+      for (int num = 0; ok; ++num) {
+        const int slot = num & 1;
+        const Job j = job_of(w, bx, by, per, lane);
+        if (num >= 2) ok = sm100::mbar_wait_warp(job_empty(slot), ((num >> 1) - 1) & 1, w.wait_ns);
         if (!ok) break;
-        const bool clear = kv == 1 && partial;
-        const uint32_t bar = clear ? landed(s) : full(s), dst = ring + s * C::tile_bytes;
-        if (lane == 0) sm100::mbar_arrive_expect_tx(bar, bytes);
+        if (lane == 0) {
+          jobs[slot] = j;
+          jobs[slot].absent = 0;
+          sm100::mbar_arrive(job_full(slot));
+          ask_next_block(answer, asked);
+        }
+        ++asks;
         __syncwarp();
-        if (page >= 0)
-          for (int h = 0; h < C::halves; ++h)
-            tma_load_4d(dst + h * kHalf + lane * w.granule * 128, kv ? &vmap : &kmap, h * 64, k & mask, kvh, page, bar);
-        ++issued;
-        if (clear) {
-          ok = sm100::mbar_wait_warp(bar, (landed_phase >> s) & 1, w.wait_ns);
-          landed_phase ^= 1u << s;
-          for (int r = lane; r < kTile; r += 32) {
-            const int p = __shfl_sync(0xffffffffu, page, r / w.granule);
-            if (p < 0 || k0 + r >= j.keys)
+        const int n = j.tiles;
+        if (n > 0) {
+          if (q_loads > 0) ok = sm100::mbar_wait_warp(q_empty, (q_loads - 1) & 1, w.wait_ns);
+          if (!ok) break;
+          if (lane == 0) {
+            sm100::mbar_arrive_expect_tx(q_full, NQ * C::halves * 128 * w.share * w.tokens_per_tile);
+            for (int t = 0; t < NQ; ++t)
               for (int h = 0; h < C::halves; ++h)
-                for (int c = 0; c < 8; ++c)
-                  asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(dst + h * kHalf + r * 128 + c * 16), "r"(0)
-                               : "memory");
+                tma_load_3d(q_sm + t * C::tile_bytes + h * kHalf, &qmap, h * 64, j.head * w.share,
+                            j.t0 + t * w.tokens_per_tile, q_full);
           }
-          sm100::fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) sm100::mbar_arrive(full(s));
+          ++q_loads;
+        }
+        const int *table = a.table + static_cast<int64_t>(max(j.row, 0)) * a.width;
+        auto page_at = [&](int i) {  // lane b: the page of box b of tile i, -1 where there is none
+          const int k = key_of_tile(j, i) + lane * w.granule;
+          if (i >= n || lane >= boxes || k >= j.keys) return -1;
+          const int p = table[k >> a.page_shift];
+          return p >= 0 && p < a.pages ? p : -1;
+        };
+        int next_page = page_at(0);
+        for (int i = 0; i < n && ok; ++i) {
+          const int page = next_page;
+          next_page = page_at(i + 1);
+          const int k0 = key_of_tile(j, i), k = k0 + lane * w.granule;
+          const uint32_t have = __ballot_sync(0xffffffffu, page >= 0);
+          const int bytes = __popc(have) * w.granule * 128 * C::halves;
+          if (__any_sync(0xffffffffu, page < 0 && lane < boxes && k < j.keys) && lane == 0)
+            *const_cast<volatile int *>(&jobs[slot].absent) = 1;  // before the tile's loads: its scores come after
+          // values of absent pages and past the last key must be zero: their weights are,
+          // but zero times what stale memory may hold need not be
+          const bool partial = __popc(have) != boxes || k0 + kTile > j.keys;
+#pragma unroll
+          for (int kv = 0; kv < 2 && ok; ++kv) {
+            const int s = issued % S, use = issued / S;
+            if (use > 0) ok = sm100::mbar_wait_warp(empty(s), (use - 1) & 1, w.wait_ns);
+            if (!ok) break;
+            const bool clear = kv == 1 && partial;
+            const uint32_t bar = clear ? landed(s) : full(s), dst = ring + s * C::tile_bytes;
+            if (lane == 0) sm100::mbar_arrive_expect_tx(bar, bytes);
+            __syncwarp();
+            if (page >= 0)
+              for (int h = 0; h < C::halves; ++h)
+                tma_load_4d(dst + h * kHalf + lane * w.granule * 128, kv ? &vmap : &kmap, h * 64, k & mask, j.head, page,
+                            bar);
+            ++issued;
+            if (clear) {
+              ok = sm100::mbar_wait_warp(bar, (landed_phase >> s) & 1, w.wait_ns);
+              landed_phase ^= 1u << s;
+              for (int r = lane; r < kTile; r += 32) {
+                const int p = __shfl_sync(0xffffffffu, page, r / w.granule);
+                if (p < 0 || k0 + r >= j.keys)
+                  for (int h = 0; h < C::halves; ++h)
+                    for (int c = 0; c < 8; ++c)
+                      asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(dst + h * kHalf + r * 128 + c * 16),
+                                   "r"(0)
+                                   : "memory");
+              }
+              sm100::fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) sm100::mbar_arrive(full(s));
+            }
+          }
+        }
+        if (!ok) break;
+        ok = sm100::mbar_wait_warp(asked, num & 1, w.wait_ns);
+        if (ok) ++answers;
+        if (!ok || !next_block(answer, bx, by)) {
+          // no block is left: the job after this one says so
+          const int last = (num + 1) & 1;
+          if (ok && num >= 1) ok = sm100::mbar_wait_warp(job_empty(last), (((num + 1) >> 1) - 1) & 1, w.wait_ns);
+          if (ok && lane == 0) {
+            jobs[last].tiles = -1;
+            sm100::mbar_arrive(job_full(last));
+          }
+          break;
         }
       }
       if (!ok) *w.error = 1;
-    }
-    // wind down: every load must have landed before the CTA exits
-    if (lane == 0) {
-      if (!sm100::mbar_wait_bounded(q_full, 0, kDrainNs)) *w.error = 1;
-      for (int x = issued > S ? issued - S : 0; x < issued; ++x)
-        if (!sm100::mbar_wait_bounded(full(x % S), (x / S) & 1, kDrainNs)) *w.error = 1;
-    }
+      // wind down: every load and answer must have landed before the CTA exits
+      if (lane == 0) {
+        if (asks > answers && !sm100::mbar_wait_bounded(asked, answers & 1, kDrainNs)) *w.error = 1;
+        if (q_loads && !sm100::mbar_wait_bounded(q_full, (q_loads - 1) & 1, kDrainNs)) *w.error = 1;
+        for (int x = issued > S ? issued - S : 0; x < issued; ++x)
+          if (!sm100::mbar_wait_bounded(full(x % S), (x / S) & 1, kDrainNs)) *w.error = 1;
+      }
     } else if (warp == 1) {
-    // ---- products
-    if (lane == 0) {
+      // ---- products: the warp waits, one thread issues
       constexpr uint32_t id_s = idesc_of<T>(kTile, false), id_o = idesc_of<T>(DP, true);
       auto stage_of = [&](int x) { return ring + (x % S) * C::tile_bytes; };
-      auto wait_tile = [&](int x) { return sm100::mbar_wait_bounded(full(x % S), (x / S) & 1, w.wait_ns); };
+      auto wait_tile = [&](int x) { return sm100::mbar_wait_warp(full(x % S), (x / S) & 1, w.wait_ns); };
       auto scores = [&](int t, int x) {  // S of query tile t over the keys in ring place x
-        const uint32_t qa = q_sm + t * C::tile_bytes, kb = stage_of(x);
+        const uint64_t qd = sm100::sw128_kmajor_desc(q_sm + t * C::tile_bytes), kd = sm100::sw128_kmajor_desc(stage_of(x));
+        if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-          const uint32_t off = (k / 4) * kHalf + (k % 4) * 32;
-          sm100::umma_f16(tmem + t * kTile, sm100::sw128_kmajor_desc(qa + off), sm100::sw128_kmajor_desc(kb + off), id_s,
-                          k != 0);
+          for (int k = 0; k < DP / 16; ++k) {
+            const uint32_t off = ((k / 4) * kHalf + (k % 4) * 32) >> 4;
+            sm100::umma_f16(tmem + t * kTile, qd + off, kd + off, id_s, k != 0);
+          }
+          sm100::umma_commit(s_full(t));
         }
-        sm100::umma_commit(s_full(t));
+        __syncwarp();
       };
-      bool ok = sm100::mbar_wait_bounded(q_full, 0, w.wait_ns) && wait_tile(0);
-      if (ok) {
+      auto commit = [&](uint32_t bar) {
+        if (elect_one()) sm100::umma_commit(bar);
+        __syncwarp();
+      };
+      bool ok = true;
+      int q_loads = 0, place = 0, step = 0;  // place: of the job's first tile in the ring; step: key tiles so far
+      for (int num = 0; ok; ++num) {
+        const int slot = num & 1;
+        ok = sm100::mbar_wait_warp(job_full(slot), (num >> 1) & 1, w.wait_ns);
+        if (!ok) break;
+        const int n = __shfl_sync(0xffffffffu, jobs[slot].tiles, 0);
+        if (n < 0) break;
+        if (lane == 0) sm100::mbar_arrive(job_empty(slot));
+        __syncwarp();
+        if (n == 0) continue;
+        ok = sm100::mbar_wait_warp(q_full, q_loads & 1, w.wait_ns) && wait_tile(place);
+        ++q_loads;
+        if (!ok) break;
         sm100::tc_fence_after_sync();
-        for (int t = 0; t < NQ; ++t) scores(t, 0);
-        sm100::umma_commit(empty(0));
-      }
-      for (int i = 0; i < n && ok; ++i) {
-        ok = wait_tile(2 * i + 1);
-        for (int t = 0; t < NQ && ok; ++t) {
-          ok = sm100::mbar_wait_bounded(p_full(t), i & 1, w.wait_ns);
-          if (!ok) break;
-          sm100::tc_fence_after_sync();
-          const uint64_t vb = sw128_mnmajor_desc(stage_of(2 * i + 1));
-#pragma unroll
-          for (int k = 0; k < kTile / 16; ++k)
-            umma_ts(tmem + NQ * kTile + t * DP, tmem + t * kTile + k * 8, vb + k * (16 * 128 >> 4), id_o, (i | k) != 0);
-          if (i + 1 < n) {
-            if (t == 0) ok = wait_tile(2 * i + 2);
+        for (int t = 0; t < NQ; ++t) scores(t, place);
+        commit(empty(place % S));
+        if (n == 1) commit(q_empty);
+        for (int i = 0; i < n && ok; ++i) {
+          const int k_next = place + 2 * i + 2, v = place + 2 * i + 1;
+          ok = wait_tile(v);
+          for (int t = 0; t < NQ && ok; ++t) {
+            const uint64_t vb = sw128_mnmajor_desc(stage_of(v));
+            const uint32_t od = tmem + NQ * kTile + t * DP, pa = tmem + t * kTile;
+            ok = sm100::mbar_wait_warp(p_half(t), (step + i) & 1, w.wait_ns);
             if (!ok) break;
             sm100::tc_fence_after_sync();
-            scores(t, 2 * i + 2);
-          } else {
-            sm100::umma_commit(o_full(t));
+            if (elect_one()) {
+#pragma unroll
+              for (int k = 0; k < kTile / 32; ++k)
+                umma_ts(od, pa + k * 8, vb + k * (16 * 128 >> 4), id_o, k != 0 || i != 0);
+              sm100::umma_commit(half_done(t));
+            }
+            __syncwarp();
+            ok = sm100::mbar_wait_warp(p_full(t), (step + i) & 1, w.wait_ns);
+            if (!ok) break;
+            sm100::tc_fence_after_sync();
+            if (elect_one()) {
+#pragma unroll
+              for (int k = kTile / 32; k < kTile / 16; ++k) umma_ts(od, pa + k * 8, vb + k * (16 * 128 >> 4), id_o, 1);
+              if (i + 1 == n) sm100::umma_commit(o_full(t));
+            }
+            __syncwarp();
+            if (i + 1 < n) {
+              if (t == 0) ok = wait_tile(k_next);
+              if (!ok) break;
+              sm100::tc_fence_after_sync();
+              scores(t, k_next);
+            }
           }
+          if (!ok) break;
+          commit(empty(v % S));
+          if (i + 1 < n) commit(empty(k_next % S));
+          if (i + 2 == n) commit(q_empty);  // the last scores are under way
         }
-        if (!ok) break;
-        sm100::umma_commit(empty((2 * i + 1) % S));
-        if (i + 1 < n) sm100::umma_commit(empty((2 * i + 2) % S));
+        place += 2 * n;
+        step += n;
       }
       if (!ok) *w.error = 1;
-      sm100::umma_commit(drain);
-      if (!sm100::mbar_wait_bounded(drain, 0, kDrainNs)) *w.error = 1;
-    }
+      commit(drain);
+      if (!sm100::mbar_wait_warp(drain, 0, kDrainNs)) *w.error = 1;
     }
   } else {
     if (NQ == 2) registers_up<216>();
@@ -387,62 +584,59 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     const int t = (warp - 4) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_at = tmem + lanes + t * kTile, o_at = tmem + lanes + NQ * kTile + t * DP;
-    const int tok = r / w.share, token = j.t0 + t * w.tokens_per_tile + tok;
-    const bool real = tok < w.tokens_per_tile && token < j.q1;
-    const int pos = j.pos0 + t * w.tokens_per_tile + tok;
-    // keys seen: k <= pos, and k > pos - window or k < sinks
-    const int pos_first = j.pos0 + t * w.tokens_per_tile, pos_last = pos_first + w.tokens_per_tile - 1;
+    const int tok = r / w.share;
     const int64_t win = a.window > 0 ? a.window : (int64_t(1) << 40);
-    const int low = static_cast<int>(max(static_cast<int64_t>(-1), pos - win));  // keys above it are recent
-    const int64_t low_last = pos_last - win;
     const int sinks = static_cast<int>(min(a.sinks, static_cast<int64_t>(0x7fffffff)));
     const float scale2 = a.scale * kLog2e;
-    float m = -INFINITY, l = 0.f;  // m in the units of S
     bool ok = true;
-    for (int i = 0; i < n; ++i) {
-      ok = sm100::mbar_wait_warp(s_full(t), i & 1, w.wait_ns);
+    int step = 0, outs = 0;
+    for (int num = 0; ok; ++num) {
+      const int slot = num & 1;
+      ok = sm100::mbar_wait_warp(job_full(slot), (num >> 1) & 1, w.wait_ns);
       if (!ok) break;
-      sm100::tc_fence_after_sync();
-      uint32_t raw[kTile];
-#pragma unroll
-      for (int c = 0; c < kTile; c += 32) tmem_ld_32(s_at + c, raw + c);
-      sm100::tmem_ld_wait();
-      float *s = reinterpret_cast<float *>(raw);
-      const int k0 = key_of_tile(i);
-      const bool plain = k0 + kTile - 1 <= pos_first && (k0 > low_last || k0 + kTile <= sinks) && k0 + kTile <= j.keys;
-      const bool gaps = absent != 0;
-      if (!plain || gaps) {
-#pragma unroll
-        for (int c = 0; c < kTile; ++c) {
-          const int k = k0 + c;
-          if (!(k <= pos && (k > low || k < sinks))) s[c] = -INFINITY;
+      const Job j = jobs[slot];
+      const int n = j.tiles;
+      if (n < 0) break;
+      if (n == 0) {
+        const int total = static_cast<int>(a.tokens);
+        const int end = j.row >= 0 ? min(j.q1, j.t0 + per) : min(total, j.t0 + per);
+        const int count = max(0, end - j.t0) * w.share;
+        for (int i = tid - 128; i < count * a.dim; i += NQ * 128) {
+          const int64_t at =
+              static_cast<int64_t>(j.t0 + i / a.dim / w.share) * a.q_heads + j.head * w.share + i / a.dim % w.share;
+          store1(static_cast<T *>(a.out) + at * a.dim + i % a.dim, 0.f);
+          if (i % a.dim == 0 && a.lse) a.lse[at] = -INFINITY;
         }
-        if (gaps) {
-          const int *table = a.table + static_cast<int64_t>(j.row) * a.width;
-          for (int b = 0; b < kTile / w.granule; ++b) {
-            const int k = k0 + b * w.granule;
-            const int p = k < j.keys ? table[k >> a.page_shift] : 0;
-            if (p < 0 || p >= a.pages) {
-#pragma unroll
-              for (int c = 0; c < kTile; ++c)
-                if (c / w.granule == b) s[c] = -INFINITY;
-            }
-          }
-        }
+        sm100::mbar_arrive(job_empty(slot));
+        continue;
       }
-      float tops[4] = {s[0], s[1], s[2], s[3]};
+      const int token = j.t0 + t * w.tokens_per_tile + tok;
+      const bool real = tok < w.tokens_per_tile && token < j.q1;
+      const int pos = j.pos0 + t * w.tokens_per_tile + tok;
+      // keys seen: k <= pos, and k > pos - window or k < sinks
+      const int pos_first = j.pos0 + t * w.tokens_per_tile, pos_last = pos_first + w.tokens_per_tile - 1;
+      const int low = static_cast<int>(max(static_cast<int64_t>(-1), pos - win));  // keys above it are recent
+      const int64_t low_last = pos_last - win;
+      float m = -INFINITY, l = 0.f;  // m in the units of S
+      for (int i = 0; i < n; ++i) {
+        ok = sm100::mbar_wait_warp(s_full(t), (step + i) & 1, w.wait_ns);
+        if (!ok) break;
+        sm100::tc_fence_after_sync();
+        uint32_t raw[kTile];
+        auto load = [&] {
 #pragma unroll
-      for (int c = 4; c < kTile; c += 8)
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-          tops[x] = fmaxf(fmaxf(tops[x], s[c + x]), c + 4 + x < kTile ? s[c + 4 + x] : s[c + x]);
-      const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-      const float grown = (top - m) * scale2;
-      const bool renew = m == -INFINITY ? top != -INFINITY : grown > 8.f;
-      if (__any_sync(0xffffffffu, renew)) {
-        const float mn = renew ? fmaxf(m, top) : m;
-        const float f = m == mn ? 1.f : ex2((m - mn) * scale2);
-        if (i > 0) {
+          for (int c = 0; c < kTile; c += 32) tmem_ld_32(s_at + c, raw + c);
+          sm100::tmem_ld_wait();
+        };
+        auto store = [&](int half) {  // the weights of 64 keys, over the first quarters of S
+          tmem_st_32(s_at + 32 * half, raw + 64 * half);
+          tmem_st_wait();
+          sm100::tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) sm100::mbar_arrive(half ? p_full(t) : p_half(t));
+        };
+        auto rescale = [&](float mn) {  // to a new reference
+          const float f = m == mn ? 1.f : ex2((m - mn) * scale2);
 #pragma unroll
           for (int c = 0; c < DP; c += 32) {
             uint32_t o[32];
@@ -452,34 +646,81 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
             for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
             tmem_st_32(o_at + c, o);
           }
+          l *= f;
+          m = mn;
+        };
+        load();
+        const int k0 = key_of_tile(j, i);
+        const bool gaps = *const_cast<volatile int *>(&jobs[slot].absent) != 0;
+        const bool plain = k0 + kTile - 1 <= pos_first && (k0 > low_last || k0 + kTile <= sinks) &&
+                           k0 + kTile <= j.keys && !gaps;
+        if (plain && i > 0) {
+          // Most tiles: no mask, and the reference of the tiles before will do, which shows
+          // afterwards.  No weight is above the sum's bound, which float16 holds.  The
+          // product with the first 64 keys' values starts before the others' weights are
+          // made.
+          const float sum = weights<T, kPolyPairs>(raw, scale2, -m * scale2);
+          if (!__any_sync(0xffffffffu, real && !(sum <= kMaxSum && m > -INFINITY))) {
+            store(0);
+            l += sum;
+            float sum2 = weights<T, kPolyPairs>(raw + 64, scale2, -m * scale2);
+            if (__any_sync(0xffffffffu, real && !(sum2 <= kMaxSum))) {
+              // a new reference in the middle: O takes it once the first half is in
+              ok = sm100::mbar_wait_warp(half_done(t), (step + i) & 1, w.wait_ns);
+              if (!ok) break;
+              sm100::tc_fence_after_sync();
+              tmem_ld_32(s_at + 64, raw + 64);
+              tmem_ld_32(s_at + 96, raw + 96);
+              sm100::tmem_ld_wait();
+              const float top = top_of(raw + 64);
+              rescale(top <= m ? m : top);
+              sum2 = weights<T, 0>(raw + 64, scale2, -m * scale2);
+            }
+            l += sum2;
+            store(1);
+            continue;
+          }
+          load();  // S is still in its place
         }
-        l *= f;
-        m = mn;
-      }
-      const float mb = m == -INFINITY ? 0.f : m * scale2;
-      const uint64_t scale_2 = pack2(scale2, scale2), mb_2 = pack2(-mb, -mb);
-      uint64_t sums[2] = {0, 0};
+        float *s = reinterpret_cast<float *>(raw);
+        if (!plain) {
+          // the row's visible keys as bits: places up to hi that are above lo or below sk
+          const int hi = pos - k0, lo = low - k0, sk = sinks - k0;
+          const int *table = a.table + static_cast<int64_t>(j.row) * a.width;
 #pragma unroll
-      for (int c = 0; c < kTile; c += 32) {
+          for (int b = 0; b < kTile; b += 32) {
+            uint32_t see = ones_below(hi + 1 - b) & (~ones_below(lo + 1 - b) | ones_below(sk - b));
+            if (gaps) {
 #pragma unroll
-        for (int x = 0; x < 32; x += 2) {
-          const float2 e = unpack2(fma2(pack2(s[c + x], s[c + x + 1]), scale_2, mb_2));
-          const float p0 = ex2(e.x), p1 = ex2(e.y);
-          sums[(x >> 1) & 1] = add2(sums[(x >> 1) & 1], pack2(p0, p1));
-          split16<T>(p0, p1, raw[(c + x) / 2]);
+              for (int h = 0; h < 32; h += 16) {  // pages hold at least 16 keys
+                const int k = k0 + b + h;
+                const int p = k < j.keys ? table[k >> a.page_shift] : 0;
+                if (p < 0 || p >= a.pages) see &= ~(0xffffu << h);
+              }
+            }
+#pragma unroll
+            for (int c = 0; c < 32; ++c) s[b + c] = (see >> c) & 1 ? s[b + c] : -INFINITY;
+          }
         }
-        tmem_st_16(s_at + c / 2, raw + c / 2);
+        const float top = max3(top_of(raw), top_of(raw + 64), -INFINITY);
+        const bool renew = m == -INFINITY ? top != -INFINITY : !((top - m) * scale2 <= 8.f);  // NaN stays
+        if (i == 0) m = top;
+        else if (__any_sync(0xffffffffu, renew)) rescale(renew ? top : m);
+        const float shift = m == -INFINITY ? 0.f : -m * scale2;
+        l += weights<T, 0>(raw, scale2, shift);
+        store(0);
+        l += weights<T, 0>(raw + 64, scale2, shift);
+        store(1);
       }
-      const float2 sum = unpack2(add2(sums[0], sums[1]));
-      l += sum.x + sum.y;
-      tmem_st_wait();
-      sm100::tc_fence_before_sync();
-      sm100::mbar_arrive(p_full(t));
-    }
-    if (ok && sm100::mbar_wait_warp(o_full(t), 0, w.wait_ns)) {
+      if (!ok) break;
+      step += n;
+      ok = sm100::mbar_wait_warp(o_full(t), outs & 1, w.wait_ns);
+      ++outs;
+      if (!ok) break;
+      sm100::mbar_arrive(job_empty(slot));
       sm100::tc_fence_after_sync();
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      const int64_t at = static_cast<int64_t>(token) * a.q_heads + kvh * w.share + r % w.share;
+      const int64_t at = static_cast<int64_t>(token) * a.q_heads + j.head * w.share + r % w.share;
       T *out = static_cast<T *>(a.out) + at * a.dim;
 #pragma unroll
       for (int c = 0; c < DP; c += 32) {
@@ -498,10 +739,10 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           }
         }
       }
+      sm100::tc_fence_before_sync();  // O is read: the next job's first weights release it
       if (real && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m * scale2 * kLn2) + logf(l);
-    } else {
-      *w.error = 1;
     }
+    if (!ok) *w.error = 1;
   }
   sm100::tc_fence_before_sync();
   __syncthreads();
