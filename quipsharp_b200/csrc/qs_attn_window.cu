@@ -46,11 +46,13 @@ template <int DP, int NQ>
 struct Cfg {
   static constexpr int halves = DP / 64;
   static constexpr int tile_bytes = halves * kHalf;
-  static constexpr int stages = (224 * 1024 - NQ * tile_bytes) / tile_bytes > 8 ? 8 : (224 * 1024 - NQ * tile_bytes) / tile_bytes;
+  static constexpr int out_bytes = NQ * 4 * 32 * 128;  // 32 rows of 64 outputs per softmax warp
+  static constexpr int room = (224 * 1024 - NQ * tile_bytes - out_bytes) / tile_bytes;
+  static constexpr int stages = room > 8 ? 8 : room;
   static constexpr int threads = 128 + NQ * 128;
   static constexpr int tmem_cols = NQ * (kTile + DP) <= 256 ? 256 : 512;
   static constexpr int bars = 3 * stages + 5 * NQ + 8;
-  static constexpr int smem = (NQ + stages) * tile_bytes + bars * 8 + 16 + 1024;
+  static constexpr int smem = (NQ + stages) * tile_bytes + out_bytes + bars * 8 + 16 + 1024;
 };
 
 struct WindowArgs {
@@ -334,7 +336,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   uint8_t *base = dsm + ((1024u - (smem_u32(dsm) & 1023u)) & 1023u);
   const uint32_t q_sm = smem_u32(base), ring = q_sm + NQ * C::tile_bytes;
-  const uint32_t bar0 = ring + S * C::tile_bytes;
+  const uint32_t out_sm = ring + S * C::tile_bytes, bar0 = out_sm + C::out_bytes;
   auto full = [&](int s) { return bar0 + 8u * s; };
   auto empty = [&](int s) { return bar0 + 8u * (S + s); };
   auto landed = [&](int s) { return bar0 + 8u * (2 * S + s); };  // loads of a tile that is then cleared in part
@@ -346,7 +348,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   auto job_full = [&](int s) { return bar0 + 8u * (3 * S + 5 * NQ + s); };
   auto job_empty = [&](int s) { return bar0 + 8u * (3 * S + 5 * NQ + 2 + s); };
   const uint32_t q_full = bar0 + 8u * (3 * S + 5 * NQ + 4), q_empty = q_full + 8, asked = q_full + 16, drain = q_full + 24;
-  uint32_t *holder = reinterpret_cast<uint32_t *>(base + (NQ + S) * C::tile_bytes + C::bars * 8);
+  uint32_t *holder = reinterpret_cast<uint32_t *>(base + (NQ + S) * C::tile_bytes + C::out_bytes + C::bars * 8);
 
   if (tid == 0) {
     for (int s = 0; s < S; ++s) {
@@ -721,23 +723,41 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       sm100::tc_fence_after_sync();
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const int64_t at = static_cast<int64_t>(token) * a.q_heads + j.head * w.share + r % w.share;
-      T *out = static_cast<T *>(a.out) + at * a.dim;
+      // 64 columns at a time through shared memory, so that a warp stores whole lines: four
+      // rows of 128 bytes where its threads' own rows would be 32 lines for 16 bytes each
+      const uint32_t stage = out_sm + (warp - 4) * 4096, mine = stage + lane * 128;
+      const uint32_t reals = __ballot_sync(0xffffffffu, real);
+      const int64_t from = real ? at : 0;
 #pragma unroll
-      for (int c = 0; c < DP; c += 32) {
-        uint32_t o[32];
+      for (int c = 0; c < DP; c += 64) {
+        uint32_t o[64];
         tmem_ld_32(o_at + c, o);
+        tmem_ld_32(o_at + c + 32, o + 32);
         sm100::tmem_ld_wait();
-        if (real) {
 #pragma unroll
-          for (int x = 0; x < 32; x += 8) {
-            if (c + x >= a.dim) continue;
-            uint32_t p[4];
+        for (int x = 0; x < 8; ++x) {
+          uint32_t p[4];
 #pragma unroll
-            for (int y = 0; y < 4; ++y)
-              split16<T>(__uint_as_float(o[x + 2 * y]) * inv, __uint_as_float(o[x + 2 * y + 1]) * inv, p[y]);
-            *reinterpret_cast<uint4 *>(out + c + x) = make_uint4(p[0], p[1], p[2], p[3]);
-          }
+          for (int y = 0; y < 4; ++y)
+            split16<T>(__uint_as_float(o[8 * x + 2 * y]) * inv, __uint_as_float(o[8 * x + 2 * y + 1]) * inv, p[y]);
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(mine + ((x ^ (lane & 7)) << 4)), "r"(p[0]),
+                       "r"(p[1]), "r"(p[2]), "r"(p[3])
+                       : "memory");
         }
+        __syncwarp();
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const int row = 4 * x + (lane >> 3), piece = lane & 7;
+          const int64_t to = __shfl_sync(0xffffffffu, from, row);
+          uint4 v;
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                       : "r"(stage + row * 128 + ((piece ^ (row & 7)) << 4))
+                       : "memory");
+          if (((reals >> row) & 1) && c + piece * 8 < a.dim)
+            *reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + to * a.dim + c + piece * 8) = v;
+        }
+        __syncwarp();
       }
       sm100::tc_fence_before_sync();  // O is read: the next job's first weights release it
       if (real && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m * scale2 * kLn2) + logf(l);
