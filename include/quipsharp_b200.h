@@ -410,8 +410,10 @@ int qs_cache_write(const qs_kv_pool *pool, int64_t rows, int64_t width, const in
 
 /* One token per row, the newest: q (rows, q_heads, dim) with strides in elements
  * (multiples of 8), out (rows, q_heads, dim) and lse (rows, q_heads) contiguous.
- * Rows of length 0 see nothing.  workspace: 256-byte aligned. */
-int64_t qs_attn_decode_workspace_bytes(int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t dim);
+ * Rows of length 0 see nothing.  workspace: 256-byte aligned; none is needed
+ * (0 bytes) where no row's line and window hold many keys. */
+int64_t qs_attn_decode_workspace_bytes(int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t page,
+                                       int64_t width, int64_t window, int64_t sinks);
 int qs_attn_decode(const void *q, int64_t q_row_stride, int64_t q_head_stride, const qs_kv_pool *pool, int64_t rows,
                    int64_t q_heads, int64_t width, const int *table, const int *lengths, float scale, int64_t window,
                    int64_t sinks, void *out, float *lse, void *workspace, int64_t workspace_bytes,
@@ -419,7 +421,8 @@ int qs_attn_decode(const void *q, int64_t q_row_stride, int64_t q_head_stride, c
 /* Many tokens per row, packed: row r's are [cu[r], cu[r+1]) of q (tokens, q_heads,
  * dim) and take its last places, their keys and values already written (lengths
  * count them).  Tokens past cu[rows] give 0. */
-int64_t qs_attn_window_workspace_bytes(int64_t tokens, int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t dim);
+int64_t qs_attn_window_workspace_bytes(int64_t tokens, int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t dim,
+                                       int64_t page, int64_t width, int64_t window, int64_t sinks);
 int qs_attn_window(const void *q, int64_t q_token_stride, int64_t q_head_stride, const qs_kv_pool *pool,
                    int64_t tokens, int64_t rows, int64_t q_heads, int64_t width, const int *table, const int *lengths,
                    const int *cu, float scale, int64_t window, int64_t sinks, void *out, float *lse, void *workspace,

@@ -6,9 +6,10 @@ is missing, every CUDA entry point raises.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import functools
 import os
+import struct
 import threading
 
 import torch
@@ -79,9 +80,9 @@ _SIGS = {
     "qs_cache_fork": (_I, [_P, _L, _L, _P, _P, _P, _P, _P, _P, _P, _P, _L, _P]),
     "qs_cache_compact": (_I, [_P, _L, _L, _P, _P, _P, _P, _P, _P, _P, _L, _P]),
     "qs_cache_extend": (_I, [_L, _L, _L, _L, _P, _P, _P, _P, _P, _P, _P, _P, _L, _P]),
-    "qs_attn_decode_workspace_bytes": (_L, [_L, _L, _L, _L]),
+    "qs_attn_decode_workspace_bytes": (_L, [_L, _L, _L, _L, _L, _L, _L, _L]),
     "qs_attn_decode": (_I, [_P, _L, _L, _P, _L, _L, _L, _P, _P, ctypes.c_float, _L, _L, _P, _P, _P, _L, _P]),
-    "qs_attn_window_workspace_bytes": (_L, [_L, _L, _L, _L, _L]),
+    "qs_attn_window_workspace_bytes": (_L, [_L, _L, _L, _L, _L, _L, _L, _L, _L]),
     "qs_attn_window": (_I, [_P, _L, _L, _P, _L, _L, _L, _L, _P, _P, _P, ctypes.c_float, _L, _L, _P, _P, _P, _L, _P]),
     "qs_beam_workspace_bytes": (_L, [_L, _L, _L, _L]),
     "qs_beam_select": (_I, [_P, _I, _L, _L, _L, _L, _L, _P, _P, _L, _I, _P, _P, _P, _P, _L, _P]),
@@ -189,28 +190,41 @@ def raw_stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
-_NO_GUARD = contextlib.nullcontext()
-
-
-def device_guard(device: torch.device):
-    """Makes `device` current, at no cost where it is already."""
-    return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def is_current(index: int) -> bool:
+    """Whether device `index` is the current one (it must have been used)."""
+    return torch._C._cuda_getDevice() == index
 
 
 def refuse_grad(name: str, *tensors) -> None:
     """The decoding operators have no backward pass: refuse inputs whose
     gradient autograd would silently lose."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} has no backward pass; call it under torch.no_grad() or detach its inputs")
+    for t in tensors:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{name} has no backward pass; call it under torch.no_grad() or detach its inputs")
 
 
 def rows_of_8(t: torch.Tensor) -> torch.Tensor:
     """t as the kernels read it in 16-byte pieces (two-byte elements): the last
     dimension contiguous, other strides multiples of 8, the start aligned; a
     contiguous copy where it is not."""
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1]):
+    *outer, last = t.stride()
+    for s in outer:
+        last |= (s & 7) << 1
+    if last == 1 and not t.data_ptr() & 15:
         return t
     return t.clone(memory_format=torch.contiguous_format)
+
+
+@functools.lru_cache(maxsize=4096)
+def workspace_bytes(name: str, *sizes) -> int:
+    """The library's answer to a *_bytes question (a function of the sizes alone)."""
+    return getattr(lib(), name)(*sizes)
+
+
+# qs_kv_pool as bytes (half the time of filling a ctypes structure)
+_KV_POOL = struct.Struct("@PPi5q8q")
+assert _KV_POOL.size == ctypes.sizeof(KVPool)
+pack_kv_pool = _KV_POOL.pack
 
 
 def require_cuda(*tensors) -> None:

@@ -10,6 +10,7 @@ import torch
 from torch import Tensor
 
 from . import _native as N
+from .kv_cache import _device_of
 
 
 def beam_select(logits: Tensor, scores: Tensor, n: int | None = None, finished: Tensor | None = None,
@@ -25,36 +26,39 @@ def beam_select(logits: Tensor, scores: Tensor, n: int | None = None, finished: 
     is.  Returns (scores float32, parents int32, tokens int32), each (batch, n);
     parents are beam numbers within the search."""
     N.refuse_grad("beam_select", logits, scores)
-    N.require_cuda(logits, scores, finished)
-    if logits.dtype not in N.IO_DTYPES:
+    dev = _device_of(logits, scores, finished)
+    if not N.is_current(dev):
+        with torch.cuda.device(dev):
+            return beam_select(logits, scores, n, finished, pad)
+    dtype = N.IO_DTYPES.get(logits.dtype)
+    if dtype is None:
         raise TypeError(f"beam_select: unsupported logits dtype {logits.dtype}")
     if logits.dim() != 3:
         raise ValueError(f"logits must be (batch, beams, vocab), got {tuple(logits.shape)}")
     batch, beams, vocab = logits.shape
     if n is None:
         n = beams
-    if scores.dtype != torch.float32 or (finished is not None and finished.dtype not in (torch.bool, torch.uint8)):
+    if scores.dtype is not torch.float32 or (finished is not None and finished.dtype not in (torch.bool, torch.uint8)):
         raise TypeError("scores must be float32 and finished bool")
     if scores.shape != (batch, beams) or (finished is not None and finished.shape != (batch, beams)):
         raise ValueError(f"scores and finished must be ({batch}, {beams})")
-    if any(t is not None and t.device != logits.device for t in (scores, finished)):
-        raise ValueError("all tensors must be on one device")
     if not 1 <= n <= vocab:
         raise ValueError(f"n must be between 1 and the vocabulary, got {n} of {vocab}")
-    if logits.stride(2) != 1:
+    strides = logits.stride()
+    if strides[2] != 1:
         logits = logits.contiguous()
+        strides = logits.stride()
     scores = scores.contiguous()
-    finished = None if finished is None else finished.contiguous()
-    dev = logits.device
-    with N.device_guard(dev):
-        nb = N.lib().qs_beam_workspace_bytes(batch, beams, vocab, n)
-        if nb < 0:
-            raise NotImplementedError(f"beam_select takes up to 64 beams and n up to 64, got {beams} and {n}")
-        ws = torch.empty(nb, dtype=torch.uint8, device=dev)
-        out = torch.empty(batch, n, dtype=torch.float32, device=dev)
-        parents, tokens = torch.empty(2, batch, n, dtype=torch.int32, device=dev).unbind(0)
-        N.check(N.lib().qs_beam_select(logits.data_ptr(), N.IO_DTYPES[logits.dtype], logits.stride(0), logits.stride(1),
-                                       batch, beams, vocab, scores.data_ptr(), N.ptr(finished), n, pad, out.data_ptr(),
-                                       parents.data_ptr(), tokens.data_ptr(), ws.data_ptr(), nb,
-                                       N.raw_stream(dev.index)))
-    return out, parents, tokens
+    if finished is not None:
+        finished = finished.contiguous()
+    nb = N.workspace_bytes("qs_beam_workspace_bytes", batch, beams, vocab, n)
+    if nb < 0:
+        raise NotImplementedError(f"beam_select takes up to 64 beams and n up to 64, got {beams} and {n}")
+    ws = scores.new_empty((nb + 3) // 4)
+    out = scores.new_empty((batch, n))
+    picks = scores.new_empty((2, batch, n), dtype=torch.int32)
+    at = picks.data_ptr()
+    N.check(N.lib().qs_beam_select(logits.data_ptr(), dtype, strides[0], strides[1], batch, beams, vocab,
+                                   scores.data_ptr(), None if finished is None else finished.data_ptr(), n, pad,
+                                   out.data_ptr(), at, at + 4 * batch * n, ws.data_ptr(), nb, N.raw_stream(dev)))
+    return out, *picks.unbind(0)

@@ -653,8 +653,12 @@ static bool attn_shape_ok(int64_t rows, int64_t q_heads, int64_t kv_heads, int64
          rows <= (1 << 24) && q_heads <= (1 << 20);
 }
 
-QS_API int64_t qs_attn_decode_workspace_bytes(int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t dim) {
-  return attn_shape_ok(rows, q_heads, kv_heads, dim) ? attn_decode_workspace_bytes(rows, q_heads, kv_heads, dim) : -1;
+QS_API int64_t qs_attn_decode_workspace_bytes(int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t page,
+                                              int64_t width, int64_t window, int64_t sinks) {
+  if (!attn_shape_ok(rows, q_heads, kv_heads, dim) || page < 1 || page > 256 || width < 0 || width > (1 << 24) ||
+      window < 0 || sinks < 0)
+    return -1;
+  return attn_decode_workspace_bytes(rows, q_heads, kv_heads, dim, page, width, window, sinks);
 }
 
 QS_API int qs_attn_decode(const void *q, int64_t q_row_stride, int64_t q_head_stride, const qs_kv_pool *pool, int64_t rows,
@@ -665,16 +669,18 @@ QS_API int qs_attn_decode(const void *q, int64_t q_row_stride, int64_t q_head_st
   const int st = check_attn(&a, q, q_row_stride, q_head_stride, pool, rows, rows, q_heads, width, table, lengths, scale,
                             window, sinks, out, lse, workspace);
   if (st || rows == 0) return st;
-  if (!workspace || workspace_bytes < attn_decode_workspace_bytes(rows, q_heads, pool->heads, pool->dim))
-    return fail(QS_ERR_WORKSPACE, "workspace missing or too small");
+  const int64_t need = attn_decode_workspace_bytes(rows, q_heads, pool->heads, pool->dim, pool->page, width, window, sinks);
+  if (workspace_bytes < need || (need && !workspace)) return fail(QS_ERR_WORKSPACE, "workspace missing or too small");
   if (!aligned(workspace, 256)) return fail(QS_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
   return launch_attn_decode(a, (cudaStream_t)stream);
 }
 
 QS_API int64_t qs_attn_window_workspace_bytes(int64_t tokens, int64_t rows, int64_t q_heads, int64_t kv_heads,
-                                              int64_t dim) {
-  if (tokens < 0 || !attn_shape_ok(rows, q_heads, kv_heads, dim)) return -1;
-  return attn_window_workspace_bytes(tokens, rows, q_heads, kv_heads, dim);
+                                              int64_t dim, int64_t page, int64_t width, int64_t window, int64_t sinks) {
+  if (tokens < 0 || !attn_shape_ok(rows, q_heads, kv_heads, dim) || page < 1 || page > 256 || width < 0 ||
+      width > (1 << 24) || window < 0 || sinks < 0)
+    return -1;
+  return attn_window_workspace_bytes(tokens, rows, q_heads, kv_heads, dim, page, width, window, sinks);
 }
 
 QS_API int qs_attn_window(const void *q, int64_t q_token_stride, int64_t q_head_stride, const qs_kv_pool *pool,
@@ -688,9 +694,9 @@ QS_API int qs_attn_window(const void *q, int64_t q_token_stride, int64_t q_head_
   if (!cu) return fail(QS_ERR_INVALID_ARG, "null pointer");
   if (q_heads / pool->heads > 128 || pool->heads > 65535)
     return fail(QS_ERR_UNSUPPORTED, "up to 128 query heads per key head and 65535 key heads");
-  if (workspace_bytes < attn_window_workspace_bytes(tokens, rows, q_heads, pool->heads, pool->dim) ||
-      (workspace_bytes && !workspace))
-    return fail(QS_ERR_WORKSPACE, "workspace missing or too small");
+  const int64_t need =
+      attn_window_workspace_bytes(tokens, rows, q_heads, pool->heads, pool->dim, pool->page, width, window, sinks);
+  if (workspace_bytes < need || (need && !workspace)) return fail(QS_ERR_WORKSPACE, "workspace missing or too small");
   if (!aligned(workspace, 256)) return fail(QS_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
   a.cu = cu;
   return launch_attn_window(a, (cudaStream_t)stream);

@@ -7,9 +7,13 @@
 // registers, and meets the other warps of its CTA only when a segment ends.
 //
 // Rows differ in length, so the work is cut by keys, not by rows: the groups of all
-// (row, key head) segments form one line that is dealt to the CTAs in equal ranges,
-// whatever the lengths.  A segment that several ranges share leaves partial results
-// (maximum, sum, output in float32), which attn_join_kernel puts together in order.
+// (row, key head) segments form one line that is dealt out in equal ranges, whatever the
+// lengths, a few ranges for each place a CTA can run (SMs reach memory at different rates:
+// with one range for each, the slowest made the others idle for a fifth of the time).  A
+// segment that several ranges share leaves partial results (maximum, sum, output in
+// float32), which attn_join_kernel puts together in order.  Where no row can see more than
+// kWholeGroups groups (short tables, short windows), a CTA takes a segment whole and
+// there is nothing to join.
 //
 // Bound: the keys and values seen, once, at HBM rate.
 #include <cmath>
@@ -20,13 +24,15 @@
 namespace qs {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
+constexpr int kRangesPerCta = 4;  // 64 rows of up to 16000 tokens: 337, 327, 321, 319, 322 us with 1, 2, 3, 4, 6
 constexpr int kStages = 3;
-constexpr int kKeys = 16;       // keys of a group
-constexpr int kRows = 16;       // query heads of a block
-constexpr int kCtasPerSm = 2;
-constexpr int kMinRange = 16;   // groups of a range at least: 4 per warp, or the joins cost more than the split saves
+constexpr int kKeys = 16;         // keys of a group
+constexpr int kRows = 16;         // query heads of a block
+constexpr int kCtasPerSm = 2;     // of four warps
+constexpr int kDealWarps = 4;     // warps of a CTA that is dealt ranges
+constexpr int kRanges = 148 * kCtasPerSm * kRangesPerCta;
+constexpr int kMinRange = 16;     // groups of a range at least: 4 per warp, or the joins cost more than the split saves
+constexpr int kWholeGroups = 80;  // a CTA of four warps takes 20 steps for them
 
 // The groups of 16 keys that a row's newest token sees: the first `sink` groups, then
 // those from `from` on.
@@ -64,11 +70,11 @@ struct Ws {
   float *o;        // [slot][16][DP]
 };
 
-template <typename T, int DP>
+template <typename T, int DP, int W>
 struct Smem {
-  T kv[kWarps][kStages][2][kKeys * DP];
-  float ml[kWarps][kRows][2];
-  int64_t sums[kThreads + 1][2];
+  T kv[W][kStages][2][kKeys * DP];
+  float ml[W][kRows][2];
+  int64_t sums[W * 32 + 1][2];
 };
 
 // One warp's softmax state over 16 query rows (R8: only the first 8 are real).
@@ -165,16 +171,151 @@ struct Warp {
   }
 };
 
-template <typename T, int DP, bool R8>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_decode_kernel(AttnArgs a, Ws ws, int blocks, int share) {
+template <typename T, int DP, bool R8, int W, bool WHOLE>
+__global__ void __launch_bounds__(W * 32, W == 4 || DP == 64 ? 2 : 1)
+attn_decode_kernel(AttnArgs a, Ws ws, int blocks, int share) {
   extern __shared__ __align__(128) uint8_t dsm[];
-  Smem<T, DP> &sm = *reinterpret_cast<Smem<T, DP> *>(dsm);
+  using S = Smem<T, DP, W>;
+  S &sm = *reinterpret_cast<S *>(dsm);
+  constexpr int kThreads = W * 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_wait();
   pdl_launch_dependents();
 
-  // ---- the line of groups: counts per thread's rows, then their prefix
+  const T *kbase = static_cast<const T *>(a.k), *vbase = static_cast<const T *>(a.v);
+  const float scale2 = a.scale * kLog2e;
+  constexpr int CPR = DP / 8;            // 16-byte pieces of a key
+  constexpr int RPI = 32 / CPR;          // keys per warp-wide copy
+  const int piece = lane % CPR, sub = lane / CPR;
+  const uint32_t ring = smem_u32(&sm.kv[warp][0][0][0]);
+
+  // Groups [u0, u1) of one segment; `slot`: where a partial result goes.
+  auto segment = [&](int row, int head, const Seen &seen, int u0, int u1, int64_t slot) {
+    const int kvh = head / blocks, h0 = kvh * share + (head % blocks) * kRows;
+    const int hn = min(kRows, share - (head % blocks) * kRows);
+    const int *table = a.table + static_cast<int64_t>(row) * a.width;
+    Warp<T, DP, R8> w;
+    w.load_q(a, row, h0, hn, lane);
+
+    const int mine = u1 - u0 - warp > 0 ? (u1 - u0 - warp + W - 1) / W : 0;
+    auto group_of = [&](int it) {
+      const int u = u0 + warp + it * W;
+      return u < seen.sink ? u : seen.from + (u - seen.sink);
+    };
+    // lane i: the page of this warp's group 32 * block + i, for the groups being loaded and
+    // for those being computed, which trail them
+    int page_ids = -1, masks_page = -1;
+    auto mask_of = [&](int g, int page) {  // bits of the group's keys that are seen
+      if (page < 0 || page >= a.pages) return 0u;
+      const int k0 = g * kKeys;
+      const uint32_t below = seen.n - k0 >= kKeys ? 0xffffu : (1u << (seen.n - k0)) - 1u;
+      const int lo_k = seen.lo - k0, sink_k = seen.sink_keys - k0;
+      const uint32_t recent = lo_k <= 0 ? 0xffffu : lo_k >= kKeys ? 0u : 0xffffu & ~((1u << lo_k) - 1u);
+      const uint32_t sinks = sink_k <= 0 ? 0u : sink_k >= kKeys ? 0xffffu : (1u << sink_k) - 1u;
+      return below & (recent | sinks);
+    };
+    auto issue = [&](int it) {
+      if (it < mine) {
+        if ((it & 31) == 0) {
+          page_ids = -1;
+          if (it + lane < mine) page_ids = table[(group_of(it + lane) * kKeys) >> a.page_shift];
+        }
+        const int page = __shfl_sync(0xffffffffu, page_ids, it & 31);
+        const int g = group_of(it);
+        const uint32_t mask = mask_of(g, page);
+        const int slot_in_page = (g * kKeys) & ((1 << a.page_shift) - 1);
+        const int64_t pg = mask ? page : 0;
+        const T *kp = kbase + pg * a.ks[0] + kvh * a.ks[1] + slot_in_page * a.ks[2] + piece * 8;
+        const T *vp = vbase + pg * a.vs[0] + kvh * a.vs[1] + slot_in_page * a.vs[2] + piece * 8;
+        const uint32_t st = ring + (it % kStages) * (2 * kKeys * DP * 2);
+        const bool real = piece * 8 < a.dim;
+#pragma unroll
+        for (int i = 0; i < kKeys / RPI; ++i) {
+          const int key = sub + i * RPI;
+          // a key that is not seen is not read: its place is zero, so nothing it holds can enter
+          const bool in = real && ((mask >> key) & 1);
+          const uint32_t dst = st + swizzled<DP>(key, piece);
+          cp_async16(dst, in ? kp + key * a.ks[2] : kbase, in);
+          cp_async16(dst + kKeys * DP * 2, in ? vp + key * a.vs[2] : vbase, in);
+        }
+      }
+      cp_async_commit();
+    };
+
+    w.reset();
+#pragma unroll
+    for (int it = 0; it < kStages - 1; ++it) issue(it);
+    masks_page = page_ids;
+    for (int it = 0; it < mine; ++it) {
+      if (it > 0 && (it & 31) == 0) masks_page = it + lane < mine ? table[(group_of(it + lane) * kKeys) >> a.page_shift] : -1;
+      issue(it + kStages - 1);
+      cp_async_wait<kStages - 1>();
+      __syncwarp();
+      const uint32_t st = ring + (it % kStages) * (2 * kKeys * DP * 2);
+      const uint32_t mask = mask_of(group_of(it), __shfl_sync(0xffffffffu, masks_page, it & 31));
+      w.step(st, st + kKeys * DP * 2, mask, scale2, lane);
+      __syncwarp();
+    }
+    cp_async_wait<0>();
+
+    // the CTA's warps meet: outputs through shared memory (their own rings)
+    float *mine_o = reinterpret_cast<float *>(&sm.kv[warp][0][0][0]);
+    const int g = lane >> 2, t = lane & 3;
+    __syncwarp();
+#pragma unroll
+    for (int h = 0; h < (R8 ? 1 : 2); ++h) {
+      float l = w.l[h];
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+      if (t == 0) sm.ml[warp][g + 8 * h][0] = w.m[h], sm.ml[warp][g + 8 * h][1] = l;
+#pragma unroll
+      for (int j = 0; j < DP / 8; ++j)
+        *reinterpret_cast<float2 *>(mine_o + (g + 8 * h) * DP + 8 * j + 2 * t) =
+            make_float2(w.o[j][2 * h], w.o[j][2 * h + 1]);
+    }
+    __syncthreads();
+    const bool whole = u0 == 0 && u1 == seen.count;
+    for (int i = tid; i < hn * (DP / 2); i += kThreads) {
+      const int r = i / (DP / 2), c2 = i % (DP / 2) * 2;
+      float m = -INFINITY, l = 0.f;
+      float2 o = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int v = 0; v < W; ++v) m = fmaxf(m, sm.ml[v][r][0]);
+#pragma unroll
+      for (int v = 0; v < W; ++v) {
+        const float f = weight(sm.ml[v][r][0], m);
+        const float2 x = *reinterpret_cast<const float2 *>(reinterpret_cast<const float *>(&sm.kv[v][0][0][0]) + r * DP + c2);
+        l += f * sm.ml[v][r][1];
+        o.x += f * x.x;
+        o.y += f * x.y;
+      }
+      if (WHOLE || whole) {
+        const int64_t out = static_cast<int64_t>(row) * a.q_heads + h0 + r;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        uint32_t packed;
+        split16<T>(o.x * inv, o.y * inv, packed);
+        if (c2 < a.dim) *reinterpret_cast<uint32_t *>(static_cast<T *>(a.out) + out * a.dim + c2) = packed;
+        if (c2 == 0 && a.lse) a.lse[out] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+      } else {
+        *reinterpret_cast<float2 *>(ws.o + (slot * kRows + r) * DP + c2) = o;
+        if (c2 == 0) ws.ml[(slot * kRows + r) * 2] = m, ws.ml[(slot * kRows + r) * 2 + 1] = l;
+      }
+    }
+    __syncthreads();
+  };
+
   const int heads = a.kv_heads * blocks;  // segments per row
+  if (WHOLE) {
+    const int row = blockIdx.x / heads;
+    // which part of the row's line is read follows from its length: have all of it in L2
+    for (int c = tid * 32; c < a.width; c += kThreads * 32)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(a.table + static_cast<int64_t>(row) * a.width + c));
+    const Seen seen = seen_of(a.lengths[row], a);
+    segment(row, blockIdx.x % heads, seen, 0, seen.count, 0);
+    return;
+  }
+
+  // ---- the line of groups: counts per thread's rows, then their prefix
   const int per = (a.rows + kThreads - 1) / kThreads;
   const int first_row = min(a.rows, tid * per), last_row = min(a.rows, first_row + per);
   {
@@ -184,28 +325,31 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_decode_kernel(AttnA
       c += n;
       p += padded(n, kMinRange);
     }
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, c, d), y = __shfl_up_sync(0xffffffffu, p, d);
+      if (lane >= d) c += x, p += y;
+    }
     sm.sums[tid + 1][0] = c;
     sm.sums[tid + 1][1] = p;
     if (tid == 0) sm.sums[0][0] = sm.sums[0][1] = 0;
     __syncthreads();
-    for (int d = 1; d < kThreads; d <<= 1) {
-      int64_t x = 0, y = 0;
-      if (tid >= d) x = sm.sums[tid + 1 - d][0], y = sm.sums[tid + 1 - d][1];
-      __syncthreads();
-      sm.sums[tid + 1][0] += x;
-      sm.sums[tid + 1][1] += y;
-      __syncthreads();
-    }
+    int64_t before_c = 0, before_p = 0;
+    for (int v = 0; v < warp; ++v) before_c += sm.sums[v * 32 + 32][0], before_p += sm.sums[v * 32 + 32][1];
+    __syncthreads();
+    sm.sums[tid + 1][0] = c + before_c;
+    sm.sums[tid + 1][1] = p + before_p;
+    __syncthreads();
   }
   // Enough groups for every CTA: one unpadded line in equal ranges.  Else short ranges
   // that begin with their segments, so that most segments need no join.
   Deal d;
   const int64_t groups = sm.sums[kThreads][0] * heads;
-  const bool dense = groups >= static_cast<int64_t>(gridDim.x) * kMinRange;
+  const bool dense = groups >= static_cast<int64_t>(148 * kCtasPerSm) * kMinRange;
   const int col = dense ? 0 : 1;
   d.pad = dense ? 1 : kMinRange;
   d.total = sm.sums[kThreads][col] * heads;
-  d.range = dense ? static_cast<int>((d.total + gridDim.x - 1) / gridDim.x) : kMinRange;
+  d.range = dense ? static_cast<int>(max(static_cast<int64_t>(kMinRange), (d.total + kRanges - 1) / kRanges)) : kMinRange;
   if (blockIdx.x == 0) {  // for the join
     int64_t at = sm.sums[tid][col];
     for (int r = first_row; r < last_row; ++r) {
@@ -219,14 +363,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_decode_kernel(AttnA
     }
   }
 
-  const T *kbase = static_cast<const T *>(a.k), *vbase = static_cast<const T *>(a.v);
-  const float scale2 = a.scale * kLog2e;
-  constexpr int CPR = DP / 8;            // 16-byte pieces of a key
-  constexpr int RPI = 32 / CPR;          // keys per warp-wide copy
-  const int piece = lane % CPR, sub = lane / CPR;
-  const uint32_t ring = smem_u32(&sm.kv[warp][0][0][0]);
-  Warp<T, DP, R8> w;
-
   const int64_t ranges = (d.total + d.range - 1) / d.range;
   for (int64_t range = blockIdx.x; range < ranges; range += gridDim.x) {
     const int64_t r0 = range * d.range, r1 = min(d.total, r0 + d.range);
@@ -239,17 +375,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_decode_kernel(AttnA
     }
     int row = lo * per;
     int64_t at = sm.sums[lo][col] * heads;  // the row's first group
-    while (row < a.rows) {
-      const int c = padded(seen_of(a.lengths[row], a).count, d.pad);
-      if (at + static_cast<int64_t>(c) * heads > r0) break;
-      at += static_cast<int64_t>(c) * heads;
-      ++row;
-    }
     int64_t pos = r0;
     while (pos < r1 && row < a.rows) {
       const Seen seen = seen_of(a.lengths[row], a);
       const int c = padded(seen.count, d.pad);
-      if (c == 0 || at + static_cast<int64_t>(c) * heads <= pos) {
+      if (at + static_cast<int64_t>(c) * heads <= pos) {
         at += static_cast<int64_t>(c) * heads;
         ++row;
         continue;
@@ -259,150 +389,67 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_decode_kernel(AttnA
       const int u0 = static_cast<int>(pos - seg);
       const int u1 = static_cast<int>(min(static_cast<int64_t>(seen.count), r1 - seg));
       pos = min(r1, seg + c);
-      if (u0 >= u1) continue;  // padding only
-      const int kvh = head / blocks, h0 = kvh * share + (head % blocks) * kRows;
-      const int hn = min(kRows, share - (head % blocks) * kRows);
-      const int *table = a.table + static_cast<int64_t>(row) * a.width;
-
-      const int mine = u1 - u0 - warp > 0 ? (u1 - u0 - warp + kWarps - 1) / kWarps : 0;
-      auto group_of = [&](int it) {
-        const int u = u0 + warp + it * kWarps;
-        return u < seen.sink ? u : seen.from + (u - seen.sink);
-      };
-      int page_ids = -1;  // lane i: the page of this warp's group 32 * block + i
-      auto mask_of = [&](int g, int page) {  // bits of the group's keys that are seen
-        if (page < 0 || page >= a.pages) return 0u;
-        const int k0 = g * kKeys;
-        const uint32_t below = seen.n - k0 >= kKeys ? 0xffffu : (1u << (seen.n - k0)) - 1u;
-        const int lo_k = seen.lo - k0, sink_k = seen.sink_keys - k0;
-        const uint32_t recent = lo_k <= 0 ? 0xffffu : lo_k >= kKeys ? 0u : 0xffffu & ~((1u << lo_k) - 1u);
-        const uint32_t sinks = sink_k <= 0 ? 0u : sink_k >= kKeys ? 0xffffu : (1u << sink_k) - 1u;
-        return below & (recent | sinks);
-      };
-      auto issue = [&](int it) {
-        if (it < mine) {
-          if ((it & 31) == 0) {
-            page_ids = -1;
-            if (it + lane < mine) page_ids = table[(group_of(it + lane) * kKeys) >> a.page_shift];
-          }
-          const int page = __shfl_sync(0xffffffffu, page_ids, it & 31);
-          const int g = group_of(it);
-          const uint32_t mask = mask_of(g, page);
-          const int slot = (g * kKeys) & ((1 << a.page_shift) - 1);
-          const int64_t pg = mask ? page : 0;
-          const T *kp = kbase + pg * a.ks[0] + kvh * a.ks[1] + slot * a.ks[2] + piece * 8;
-          const T *vp = vbase + pg * a.vs[0] + kvh * a.vs[1] + slot * a.vs[2] + piece * 8;
-          const uint32_t st = ring + (it % kStages) * (2 * kKeys * DP * 2);
-          const bool real = piece * 8 < a.dim;
-#pragma unroll
-          for (int i = 0; i < kKeys / RPI; ++i) {
-            const int key = sub + i * RPI;
-            // a key that is not seen is not read: its place is zero, so nothing it holds can enter
-            const bool in = real && ((mask >> key) & 1);
-            const uint32_t dst = st + swizzled<DP>(key, piece);
-            cp_async16(dst, in ? kp + key * a.ks[2] : kbase, in);
-            cp_async16(dst + kKeys * DP * 2, in ? vp + key * a.vs[2] : vbase, in);
-          }
-        }
-        cp_async_commit();
-      };
-
-      w.load_q(a, row, h0, hn, lane);
-      w.reset();
-      int masks_page = -1;  // the pages of the groups being computed trail those being loaded
-#pragma unroll
-      for (int it = 0; it < kStages - 1; ++it) issue(it);
-      for (int it = 0; it < mine; ++it) {
-        if ((it & 31) == 0) {
-          masks_page = -1;
-          if (it + lane < mine) masks_page = table[(group_of(it + lane) * kKeys) >> a.page_shift];
-        }
-        issue(it + kStages - 1);
-        cp_async_wait<kStages - 1>();
-        __syncwarp();
-        const uint32_t st = ring + (it % kStages) * (2 * kKeys * DP * 2);
-        const uint32_t mask = mask_of(group_of(it), __shfl_sync(0xffffffffu, masks_page, it & 31));
-        w.step(st, st + kKeys * DP * 2, mask, scale2, lane);
-        __syncwarp();
-      }
-      cp_async_wait<0>();
-
-      // ---- the CTA's warps meet: outputs through shared memory (their own rings)
-      float *mine_o = reinterpret_cast<float *>(&sm.kv[warp][0][0][0]);
-      const int g = lane >> 2, t = lane & 3;
-      __syncwarp();
-#pragma unroll
-      for (int h = 0; h < (R8 ? 1 : 2); ++h) {
-        float l = w.l[h];
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        if (t == 0) sm.ml[warp][g + 8 * h][0] = w.m[h], sm.ml[warp][g + 8 * h][1] = l;
-#pragma unroll
-        for (int j = 0; j < DP / 8; ++j)
-          *reinterpret_cast<float2 *>(mine_o + (g + 8 * h) * DP + 8 * j + 2 * t) =
-              make_float2(w.o[j][2 * h], w.o[j][2 * h + 1]);
-      }
-      __syncthreads();
-      const bool whole = u0 == 0 && u1 == seen.count;
-      const int64_t slot = dense ? 2 * range + (seg > r0 ? 1 : 0) : range;
-      for (int i = tid; i < hn * DP; i += kThreads) {
-        const int r = i / DP, c2 = i % DP;
-        float m = -INFINITY, l = 0.f, o = 0.f;
-#pragma unroll
-        for (int v = 0; v < kWarps; ++v) m = fmaxf(m, sm.ml[v][r][0]);
-#pragma unroll
-        for (int v = 0; v < kWarps; ++v) {
-          const float f = weight(sm.ml[v][r][0], m);
-          l += f * sm.ml[v][r][1];
-          o += f * reinterpret_cast<const float *>(&sm.kv[v][0][0][0])[r * DP + c2];
-        }
-        if (whole) {
-          const int64_t out = static_cast<int64_t>(row) * a.q_heads + h0 + r;
-          if (c2 < a.dim) store1(static_cast<T *>(a.out) + out * a.dim + c2, l == 0.f ? 0.f : o / l);
-          if (c2 == 0 && a.lse) a.lse[out] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
-        } else {
-          ws.o[(slot * kRows + r) * DP + c2] = o;
-          if (c2 == 0) ws.ml[(slot * kRows + r) * 2] = m, ws.ml[(slot * kRows + r) * 2 + 1] = l;
-        }
-      }
-      __syncthreads();
+      if (u0 < u1) segment(row, head, seen, u0, u1, dense ? 2 * range + (seg > r0 ? 1 : 0) : range);
     }
   }
 }
 
-// Joins the partial results of one segment's ranges, in their order; segments that no
-// range covers (rows that see nothing) get zeros.
+// Joins the partial results of one segment's ranges, in their order, a warp for each query
+// row; segments that no range covers (rows that see nothing) get zeros.
 template <typename T, int DP>
 __global__ void __launch_bounds__(128) attn_join_kernel(AttnArgs a, Ws ws, int blocks, int share) {
+  constexpr int PER = DP / 32, U = 4;  // outputs per lane, partial results at a time
   pdl_wait();
   pdl_launch_dependents();
-  const int heads = a.kv_heads * blocks;
-  const int row = blockIdx.x / heads, head = blockIdx.x % heads;
-  const int range = ws.deal[0], pad = ws.deal[1];
+  const int heads = a.kv_heads * blocks, lane = threadIdx.x & 31;
+  const int segment = blockIdx.x / (kRows / 4), r = blockIdx.x % (kRows / 4) * 4 + (threadIdx.x >> 5);
+  const int row = segment / heads, head = segment % heads;
   const int kvh = head / blocks, h0 = kvh * share + (head % blocks) * kRows;
-  const int hn = min(kRows, share - (head % blocks) * kRows);
+  if (r >= min(kRows, share - (head % blocks) * kRows)) return;
+  const int range = ws.deal[0], pad = ws.deal[1];
   const int count = seen_of(a.lengths[row], a).count;
   const int64_t seg = ws.start[row] * heads + static_cast<int64_t>(head) * padded(count, pad);
   const int64_t f = seg / range, e = count ? (seg + count - 1) / range : f;
   if (count && f == e) return;  // one range had it whole
-  for (int i = threadIdx.x; i < hn * DP; i += 128) {
-    const int r = i / DP, c = i % DP;
-    float m = -INFINITY, l = 0.f, o = 0.f;
-    if (count)
-      for (int64_t x = f; x <= e; ++x) {
-        const int64_t slot = pad == 1 ? 2 * x + (x == f && seg > x * range ? 1 : 0) : x;
-        const float m2 = ws.ml[(slot * kRows + r) * 2], l2 = ws.ml[(slot * kRows + r) * 2 + 1];
-        const float o2 = ws.o[(slot * kRows + r) * DP + c];
-        const float mn = fmaxf(m, m2);
-        const float p = weight(m, mn), q = weight(m2, mn);
-        l = l * p + l2 * q;
-        o = o * p + o2 * q;
-        m = mn;
+  const int parts = count ? static_cast<int>(e - f) + 1 : 0;
+  auto slot_of = [&](int i) { return pad == 1 ? 2 * (f + i) + (i == 0 && seg > f * range ? 1 : 0) : f + i; };
+  float m = -INFINITY;
+  for (int i = lane; i < parts; i += 32) m = fmaxf(m, ws.ml[(slot_of(i) * kRows + r) * 2]);
+#pragma unroll
+  for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+  float l = 0.f, o[PER] = {};
+  for (int i0 = 0; i0 < parts; i0 += U) {
+    float2 ml[U];
+    float x[U][PER];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      ml[u] = make_float2(-INFINITY, 0.f);
+      if (i0 + u < parts) {
+        const int64_t at = slot_of(i0 + u) * kRows + r;
+        ml[u] = *reinterpret_cast<const float2 *>(ws.ml + at * 2);
+#pragma unroll
+        for (int c = 0; c < PER; ++c) x[u][c] = ws.o[at * DP + lane * PER + c];
       }
-    const int64_t out = static_cast<int64_t>(row) * a.q_heads + h0 + r;
-    if (c < a.dim) store1(static_cast<T *>(a.out) + out * a.dim + c, l == 0.f ? 0.f : o / l);
-    if (c == 0 && a.lse) a.lse[out] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i0 + u >= parts) break;
+      const float p = weight(ml[u].x, m);
+      l += p * ml[u].y;
+#pragma unroll
+      for (int c = 0; c < PER; ++c) o[c] += p * x[u][c];
+    }
   }
+  const int64_t out = static_cast<int64_t>(row) * a.q_heads + h0 + r;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int c = 0; c < PER; c += 2) {
+    uint32_t packed;
+    split16<T>(o[c] * inv, o[c + 1] * inv, packed);
+    if (lane * PER + c < a.dim)
+      *reinterpret_cast<uint32_t *>(static_cast<T *>(a.out) + out * a.dim + lane * PER + c) = packed;
+  }
+  if (lane == 0 && a.lse) a.lse[out] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 struct Shape {
@@ -415,36 +462,57 @@ Shape shape_of(int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t dim) {
   s.heads = kv_heads * ceil_div(q_heads / kv_heads, kRows);
   // equal ranges leave up to two partial results each; short ranges one, and there are
   // no more of them than the CTAs plus one for each segment's last
-  const int64_t grid = 148 * kCtasPerSm;
-  s.slots = 2 * grid > grid + rows * s.heads ? 2 * grid : grid + rows * s.heads;
+  const int64_t some = 148 * kCtasPerSm + rows * s.heads;
+  s.slots = 2 * kRanges > some ? 2 * kRanges : some;
   s.dp = dim <= 64 ? 64 : 128;
   return s;
 }
 
-template <typename T, int DP, bool R8>
-int run(const AttnArgs &a, const Ws &ws, int blocks, int share, cudaStream_t s) {
-  auto kern = attn_decode_kernel<T, DP, R8>;
-  static const cudaError_t attr =
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(Smem<T, DP>)));
+// Groups that a row can see at most, by its line and the window.
+int64_t most_groups(int64_t page, int64_t width, int64_t window, int64_t sinks) {
+  int64_t keys = width * page;
+  if (window > 0 && window < keys && sinks < keys && window + sinks < keys)
+    keys = window + sinks + 2 * kKeys;  // both ends inside a group
+  return ceil_div(keys, kKeys);
+}
+
+template <typename T, int DP, bool R8, int W, bool WHOLE>
+int run(const AttnArgs &a, const Ws &ws, int blocks, int share, int64_t grid, cudaStream_t s) {
+  auto kern = attn_decode_kernel<T, DP, R8, W, WHOLE>;
+  constexpr int smem = static_cast<int>(sizeof(Smem<T, DP, W>));
+  static const cudaError_t attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (attr != cudaSuccess) return fail(QS_ERR_CUDA, "attention (decode): %s", cudaGetErrorString(attr));
-  const int grid = 148 * kCtasPerSm;
-  int st = launch_pdl("attention (decode)", kern, dim3(grid), dim3(kThreads), sizeof(Smem<T, DP>), s, a, ws, blocks,
-                      share);
+  return launch_pdl("attention (decode)", kern, dim3(static_cast<unsigned>(grid)), dim3(W * 32), smem, s, a, ws, blocks,
+                    share);
+}
+
+template <typename T, int DP, bool R8>
+int run_shape(const AttnArgs &a, const Ws &ws, int blocks, int share, cudaStream_t s) {
+  const int64_t segments = static_cast<int64_t>(a.rows) * a.kv_heads * blocks, most = most_groups(int64_t(1) << a.page_shift, a.width, a.window, a.sinks);
+  if (most <= kWholeGroups) {
+    // eight warps where all segments run at once anyway
+    if (segments <= 148 * (DP == 64 ? 2 : 1)) return run<T, DP, R8, 8, true>(a, ws, blocks, share, segments, s);
+    return run<T, DP, R8, 4, true>(a, ws, blocks, share, segments, s);
+  }
+  const int64_t fewest = ceil_div(most, kMinRange) * segments;  // ranges there can be
+  const int st = run<T, DP, R8, kDealWarps, false>(a, ws, blocks, share, fewest < kRanges ? fewest : kRanges, s);
   if (st) return st;
-  return launch_pdl("attention (join)", attn_join_kernel<T, DP>,
-                    dim3(static_cast<unsigned>(a.rows * a.kv_heads * blocks)), dim3(128), 0, s, a, ws, blocks, share);
+  return launch_pdl("attention (join)", attn_join_kernel<T, DP>, dim3(static_cast<unsigned>(segments * (kRows / 4))),
+                    dim3(128), 0, s, a, ws, blocks, share);
 }
 
 template <typename T>
 int run_type(const AttnArgs &a, const Ws &ws, int blocks, int share, cudaStream_t s) {
   if (a.dim <= 64)
-    return share <= 8 ? run<T, 64, true>(a, ws, blocks, share, s) : run<T, 64, false>(a, ws, blocks, share, s);
-  return share <= 8 ? run<T, 128, true>(a, ws, blocks, share, s) : run<T, 128, false>(a, ws, blocks, share, s);
+    return share <= 8 ? run_shape<T, 64, true>(a, ws, blocks, share, s) : run_shape<T, 64, false>(a, ws, blocks, share, s);
+  return share <= 8 ? run_shape<T, 128, true>(a, ws, blocks, share, s) : run_shape<T, 128, false>(a, ws, blocks, share, s);
 }
 
 }  // namespace
 
-int64_t attn_decode_workspace_bytes(int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t dim) {
+int64_t attn_decode_workspace_bytes(int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t page,
+                                    int64_t width, int64_t window, int64_t sinks) {
+  if (most_groups(page, width, window, sinks) <= kWholeGroups) return 0;
   const Shape s = shape_of(rows, q_heads, kv_heads, dim);
   return round_up((rows + 1) * 8 + 8, 256) + s.slots * kRows * (s.dp + 2) * 4;
 }

@@ -807,7 +807,9 @@ int run(const AttnArgs &a, cudaStream_t s) {
 
 }  // namespace
 
-int64_t attn_window_workspace_bytes(int64_t, int64_t, int64_t, int64_t, int64_t) { return 0; }
+int64_t attn_window_workspace_bytes(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t) {
+  return 0;
+}
 
 int launch_attn_window(const AttnArgs &a, cudaStream_t s) {
   if (a.dim <= 64) return a.dtype == QS_F16 ? run<__half, 64, 2>(a, s) : run<__nv_bfloat16, 64, 2>(a, s);

@@ -160,10 +160,12 @@ struct AttnArgs {
   void *ws;
 };
 // qs_attn_decode.cu
-int64_t attn_decode_workspace_bytes(int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t dim);
+int64_t attn_decode_workspace_bytes(int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t page,
+                                    int64_t width, int64_t window, int64_t sinks);
 int launch_attn_decode(const AttnArgs &a, cudaStream_t s);
 // qs_attn_window.cu
-int64_t attn_window_workspace_bytes(int64_t tokens, int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t dim);
+int64_t attn_window_workspace_bytes(int64_t tokens, int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t dim,
+                                    int64_t page, int64_t width, int64_t window, int64_t sinks);
 int launch_attn_window(const AttnArgs &a, cudaStream_t s);
 
 // qs_beam.cu

@@ -36,57 +36,56 @@ def check_device(device=None) -> None:
 
 
 def _int32(name: str, t: Tensor, *shape) -> Tensor:
-    if t.dtype != torch.int32:
+    if t.dtype is not torch.int32:
         raise TypeError(f"{name} must be int32, got {t.dtype}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _same_device(first: Tensor, *others) -> None:
-    N.require_cuda(first, *others)
+def _device_of(first: Tensor, *others) -> int:
+    """The index of the one CUDA device that holds all the tensors."""
+    index = first.get_device()
+    if index < 0:
+        N.require_cuda(first)
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != index:
+            N.require_cuda(t)
             raise ValueError(f"all tensors must be on one device, got {first.device} and {t.device}")
+    return index
 
 
-def kv_pool(k: Tensor, v: Tensor) -> N.KVPool:
-    """The library's description of pools k, v (layers, pages, heads, page, dim)
-    or, of one layer, (pages, heads, page, dim)."""
-    if k.dtype not in KV_DTYPES or v.dtype != k.dtype:
+def kv_pool(k: Tensor, v: Tensor):
+    """(description for the library, pages, heads, page, dim) of pools k, v
+    (layers, pages, heads, page, dim) or, of one layer, (pages, heads, page, dim)."""
+    dtype = KV_DTYPES.get(k.dtype)
+    if dtype is None or v.dtype is not k.dtype:
         raise TypeError(f"a cache holds float16 or bfloat16 keys and values of one type, got {k.dtype} and {v.dtype}")
-    if k.shape != v.shape or k.dim() not in (4, 5):
+    shape, ks, vs = k.shape, k.stride(), v.stride()
+    if v.shape != shape or len(shape) not in (4, 5):
         raise ValueError("key and value pools must have one shape, ([layers,] pages, heads, page, dim); "
                          f"got {tuple(k.shape)} and {tuple(v.shape)}")
-    if k.stride(-1) != 1 or v.stride(-1) != 1:
+    if ks[-1] != 1 or vs[-1] != 1:
         raise ValueError("the last dimension of a pool must be contiguous")
-    p = N.KVPool()
-    p.k, p.v, p.dtype = k.data_ptr(), v.data_ptr(), KV_DTYPES[k.dtype]
-    if k.dim() == 5:
-        p.layers, p.pages, p.heads, p.page, p.dim = k.shape
-        p.k_stride[:], p.v_stride[:] = k.stride()[:4], v.stride()[:4]
-    else:
-        p.layers = 1
-        p.pages, p.heads, p.page, p.dim = k.shape
-        p.k_stride[:], p.v_stride[:] = (0, *k.stride()[:3]), (0, *v.stride()[:3])
-    return p
+    if len(shape) == 4:
+        shape, ks, vs = (1, *shape), (0, *ks), (0, *vs)
+    return (N.pack_kv_pool(k.data_ptr(), v.data_ptr(), dtype, *shape, *ks[:4], *vs[:4]), *shape[1:])
 
 
-def _workspace(rows: int, pages: int, device) -> tuple[Tensor, int]:
-    n = N.lib().qs_cache_workspace_bytes(rows, pages)
+def _workspace(rows: int, pages: int, like: Tensor) -> tuple[Tensor, int]:
+    n = N.workspace_bytes("qs_cache_workspace_bytes", rows, pages)
     if n < 0:
         raise NotImplementedError(f"a cache has 1 to 2^28 pages and at most 8192 rows, got {pages} pages, {rows} rows")
-    return torch.empty(n, dtype=torch.uint8, device=device), n
+    return like.new_empty(n // 4), n
 
 
 def _state(k: Tensor, v: Tensor, table: Tensor, lengths: Tensor, refcount: Tensor):
-    _same_device(k, v, table, lengths, refcount)
     if table.dim() != 2:
         raise ValueError(f"table must be (rows, width), got {tuple(table.shape)}")
     rows, width = table.shape
-    pool = kv_pool(k, v)
-    return (pool, rows, width, _int32("table", table, rows, width), _int32("lengths", lengths, rows),
-            _int32("refcount", refcount, pool.pages))
+    pool, pages = kv_pool(k, v)[:2]
+    return (pool, pages, rows, width, _int32("table", table, rows, width), _int32("lengths", lengths, rows),
+            _int32("refcount", refcount, pages))
 
 
 def fork_pages(k: Tensor, v: Tensor, table: Tensor, lengths: Tensor, refcount: Tensor,
@@ -99,15 +98,17 @@ def fork_pages(k: Tensor, v: Tensor, table: Tensor, lengths: Tensor, refcount: T
     of all layers copied.  Returns the new (table, lengths, refcount); the pools
     k, v (layers, pages, heads, page, dim) are changed in place.  refcount may
     hold references of the caller's besides the table's: they stay."""
-    pool, rows, width, table, lengths, refcount = _state(k, v, table, lengths, refcount)
-    _same_device(k, parents)
+    dev = _device_of(k, v, table, lengths, refcount, parents)
+    if not N.is_current(dev):
+        with torch.cuda.device(dev):
+            return fork_pages(k, v, table, lengths, refcount, parents)
+    pool, pages, rows, width, table, lengths, refcount = _state(k, v, table, lengths, refcount)
     parents = _int32("parents", parents, rows)
-    with N.device_guard(k.device):
-        ws, nb = _workspace(rows, pool.pages, k.device)
-        t, n, c = torch.empty_like(table), torch.empty_like(lengths), torch.empty_like(refcount)
-        N.check(N.lib().qs_cache_fork(N.ref(pool), rows, width, table.data_ptr(), lengths.data_ptr(), refcount.data_ptr(),
-                                      parents.data_ptr(), t.data_ptr(), n.data_ptr(), c.data_ptr(), ws.data_ptr(), nb,
-                                      N.raw_stream(k.device.index)))
+    ws, nb = _workspace(rows, pages, table)
+    t, n, c = torch.empty_like(table), torch.empty_like(lengths), torch.empty_like(refcount)
+    N.check(N.lib().qs_cache_fork(pool, rows, width, table.data_ptr(), lengths.data_ptr(), refcount.data_ptr(),
+                                  parents.data_ptr(), t.data_ptr(), n.data_ptr(), c.data_ptr(), ws.data_ptr(), nb,
+                                  N.raw_stream(dev)))
     return t, n, c
 
 
@@ -117,14 +118,15 @@ def compact_pages(k: Tensor, v: Tensor, table: Tensor, lengths: Tensor,
     from U on go to the holes below U, both in ascending order.  Returns the new
     (table, refcount, U as an int32 tensor of one); the pools are changed in
     place, and pages from U on are free."""
-    pool, rows, width, table, lengths, refcount = _state(k, v, table, lengths, refcount)
-    with N.device_guard(k.device):
-        ws, nb = _workspace(rows, pool.pages, k.device)
-        t, c = torch.empty_like(table), torch.empty_like(refcount)
-        used = torch.empty(1, dtype=torch.int32, device=k.device)
-        N.check(N.lib().qs_cache_compact(N.ref(pool), rows, width, table.data_ptr(), lengths.data_ptr(), refcount.data_ptr(),
-                                         t.data_ptr(), c.data_ptr(), used.data_ptr(), ws.data_ptr(), nb,
-                                         N.raw_stream(k.device.index)))
+    dev = _device_of(k, v, table, lengths, refcount)
+    if not N.is_current(dev):
+        with torch.cuda.device(dev):
+            return compact_pages(k, v, table, lengths, refcount)
+    pool, pages, rows, width, table, lengths, refcount = _state(k, v, table, lengths, refcount)
+    ws, nb = _workspace(rows, pages, table)
+    t, c, used = torch.empty_like(table), torch.empty_like(refcount), refcount.new_empty(1)
+    N.check(N.lib().qs_cache_compact(pool, rows, width, table.data_ptr(), lengths.data_ptr(), refcount.data_ptr(),
+                                     t.data_ptr(), c.data_ptr(), used.data_ptr(), ws.data_ptr(), nb, N.raw_stream(dev)))
     return t, c, used
 
 
@@ -134,27 +136,28 @@ def extend_pages(table: Tensor, lengths: Tensor, refcount: Tensor, new_tokens: T
     lowest free ones, in row and then column order.  Returns the new (table,
     lengths, refcount).  A row that finds no page, or outgrows its line, has -1
     there: its tokens are left out, and `check_device` raises."""
-    _same_device(table, lengths, refcount, new_tokens)
+    dev = _device_of(table, lengths, refcount, new_tokens)
+    if not N.is_current(dev):
+        with torch.cuda.device(dev):
+            return extend_pages(table, lengths, refcount, new_tokens, page_size)
     if table.dim() != 2 or refcount.dim() != 1:
         raise ValueError("table must be (rows, width) and refcount (pages,), "
                          f"got {tuple(table.shape)} and {tuple(refcount.shape)}")
     rows, width = table.shape
-    pages = refcount.shape[0]
     table, lengths = _int32("table", table, rows, width), _int32("lengths", lengths, rows)
-    refcount, new_tokens = _int32("refcount", refcount, pages), _int32("new_tokens", new_tokens, rows)
-    with N.device_guard(table.device):
-        t, n, c = torch.empty_like(table), torch.empty_like(lengths), torch.empty_like(refcount)
-        _extend(page_size, table, lengths, refcount, new_tokens, t, n, c)
+    refcount, new_tokens = _int32("refcount", refcount, len(refcount)), _int32("new_tokens", new_tokens, rows)
+    t, n, c = torch.empty_like(table), torch.empty_like(lengths), torch.empty_like(refcount)
+    _extend(page_size, table, lengths, refcount, new_tokens, t, n, c, dev)
     return t, n, c
 
 
-def _extend(page_size, table, lengths, refcount, new_tokens, t, n, c) -> None:
+def _extend(page_size, table, lengths, refcount, new_tokens, t, n, c, dev) -> None:
     rows, width = table.shape
-    pages = refcount.shape[0]
-    ws, nb = _workspace(rows, pages, table.device)
+    pages = len(refcount)
+    ws, nb = _workspace(rows, pages, table)
     N.check(N.lib().qs_cache_extend(page_size, pages, rows, width, table.data_ptr(), lengths.data_ptr(),
                                     refcount.data_ptr(), new_tokens.data_ptr(), t.data_ptr(), n.data_ptr(),
-                                    c.data_ptr(), ws.data_ptr(), nb, N.raw_stream(table.device.index)))
+                                    c.data_ptr(), ws.data_ptr(), nb, N.raw_stream(dev)))
 
 
 def write_kv(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor,
@@ -165,24 +168,27 @@ def write_kv(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tens
     cu every row has one.  k and v may be views (the last dimension
     contiguous)."""
     N.refuse_grad("write_kv", k, v)
-    _same_device(k, v, k_pages, v_pages, table, lengths, cu)
+    dev = _device_of(k, v, k_pages, v_pages, table, lengths, cu)
+    if not N.is_current(dev):
+        with torch.cuda.device(dev):
+            return write_kv(k, v, k_pages, v_pages, table, lengths, cu)
     if k_pages.dim() != 4 or table.dim() != 2:
         raise ValueError("write_kv takes one layer's pools (pages, heads, page, dim) and a table (rows, width)")
-    pool = kv_pool(k_pages, v_pages)
+    pool, _, heads, _, dim = kv_pool(k_pages, v_pages)
     rows, width = table.shape
     table, lengths = _int32("table", table, rows, width), _int32("lengths", lengths, rows)
     if cu is not None:
         cu = _int32("cu", cu, rows + 1)
-    if k.dtype != k_pages.dtype or v.dtype != k_pages.dtype:
+    if k.dtype is not k_pages.dtype or v.dtype is not k_pages.dtype:
         raise TypeError(f"keys and values must have the pools' type {k_pages.dtype}, got {k.dtype} and {v.dtype}")
-    if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (pool.heads, pool.dim):
-        raise ValueError(f"keys and values must be (tokens, {pool.heads}, {pool.dim}), "
-                         f"got {tuple(k.shape)} and {tuple(v.shape)}")
+    shape = k.shape
+    if len(shape) != 3 or v.shape != shape or shape[1] != heads or shape[2] != dim:
+        raise ValueError(f"keys and values must be (tokens, {heads}, {dim}), got {tuple(k.shape)} and {tuple(v.shape)}")
     k, v = N.rows_of_8(k), N.rows_of_8(v)
-    with N.device_guard(k.device):
-        N.check(N.lib().qs_cache_write(N.ref(pool), rows, width, table.data_ptr(), lengths.data_ptr(), N.ptr(cu),
-                                       k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                                       k.shape[0], N.raw_stream(k.device.index)))
+    ks, vs = k.stride(), v.stride()
+    N.check(N.lib().qs_cache_write(pool, rows, width, table.data_ptr(), lengths.data_ptr(),
+                                   None if cu is None else cu.data_ptr(), k.data_ptr(), ks[0], ks[1], v.data_ptr(),
+                                   vs[0], vs[1], shape[0], N.raw_stream(dev)))
 
 
 class PagedKVCache:
@@ -218,11 +224,11 @@ class PagedKVCache:
         all rows)."""
         if not isinstance(new_tokens, Tensor):
             new_tokens = torch.full_like(self.lengths, int(new_tokens))
-        _same_device(self.table, new_tokens)
-        new_tokens = _int32("new_tokens", new_tokens, self.lengths.shape[0])
-        with N.device_guard(self.table.device):
+        dev = _device_of(self.table, new_tokens)
+        new_tokens = _int32("new_tokens", new_tokens, len(self.lengths))
+        with torch.cuda.device(dev):
             _extend(self.page_size, self.table, self.lengths, self.refcount, new_tokens, self.table, self.lengths,
-                    self.refcount)
+                    self.refcount, dev)
 
     def write(self, layer: int, k: Tensor, v: Tensor, cu: Tensor | None = None) -> None:
         """New tokens' keys and values of one layer (see write_kv)."""

@@ -61,12 +61,13 @@ def test_cache_arguments():
 
 def test_attention_arguments():
     lib, p, at = N.lib(), pool(), ctypes.c_void_p
-    need = lib.qs_attn_decode_workspace_bytes(3, 4, 2, 64)
-    assert need > 0
-    assert lib.qs_attn_decode_workspace_bytes(3, 5, 2, 64) == -1 and lib.qs_attn_decode_workspace_bytes(3, 4, 2, 136) == -1
+    sizes = lib.qs_attn_decode_workspace_bytes
+    need = sizes(3, 4, 2, 64, 16, 100, 0, 0)
+    assert need > 0 and sizes(3, 4, 2, 64, 16, 10, 0, 0) == sizes(3, 4, 2, 64, 16, 100, 500, 4) == 0  # few keys: no joins
+    assert sizes(3, 5, 2, 64, 16, 100, 0, 0) == sizes(3, 4, 2, 136, 16, 100, 0, 0) == sizes(3, 4, 2, 64, 16, -1, 0, 0) == -1
 
     def decode(q=at(4096), heads=4, scale=0.1, window=0, sinks=0, ws=at(1 << 16), nb=need, pool=p, q_head=64):
-        return lib.qs_attn_decode(q, 256, q_head, N.ref(pool), 3, heads, 1, at(256), at(512), scale, window, sinks, at(8192),
+        return lib.qs_attn_decode(q, 256, q_head, N.ref(pool), 3, heads, 100, at(256), at(512), scale, window, sinks, at(8192),
                                   None, ws, nb, None)
 
     assert decode(q=None) == N.QS_ERR_INVALID_ARG and decode(heads=5) == N.QS_ERR_INVALID_ARG
