@@ -510,12 +510,15 @@ static int check_pool(const qs_kv_pool *p) {
   for (int i = 0; i < 4; ++i)
     if (p->k_stride[i] < 0 || p->v_stride[i] < 0 || p->k_stride[i] % 8 || p->v_stride[i] % 8)
       return fail(QS_ERR_ALIGNMENT, "pool strides must be multiples of 8 elements");
+  if (p->k_stride[3] > (1 << 21) || p->v_stride[3] > (1 << 21) || p->layers * p->heads > (1 << 24))
+    return fail(QS_ERR_UNSUPPORTED, "a token stride above 2^21 elements, or more than 2^24 layers x heads");
   return QS_OK;
 }
 
 static int check_rows(int64_t rows, int64_t width, const int *table, const int *lengths) {
-  if (rows < 0 || width < 0) return fail(QS_ERR_INVALID_ARG, "bad table shape");
-  if (width > (1 << 24)) return fail(QS_ERR_UNSUPPORTED, "more than 2^24 pages in a row");
+  if (rows < 0 || width < 0 || rows > 0x7fffffff) return fail(QS_ERR_INVALID_ARG, "bad table shape");
+  if (width > (1 << 24) || rows * width > 0x7fffffff)
+    return fail(QS_ERR_UNSUPPORTED, "more than 2^24 pages in a row, or 2^31 - 1 in the table");
   if (rows && (!lengths || (width && !table))) return fail(QS_ERR_INVALID_ARG, "null pointer");
   return QS_OK;
 }

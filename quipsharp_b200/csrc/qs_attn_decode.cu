@@ -307,9 +307,6 @@ attn_decode_kernel(AttnArgs a, Ws ws, int blocks, int share) {
   const int heads = a.kv_heads * blocks;  // segments per row
   if (WHOLE) {
     const int row = blockIdx.x / heads;
-    // which part of the row's line is read follows from its length: have all of it in L2
-    for (int c = tid * 32; c < a.width; c += kThreads * 32)
-      asm volatile("prefetch.global.L2 [%0];" ::"l"(a.table + static_cast<int64_t>(row) * a.width + c));
     const Seen seen = seen_of(a.lengths[row], a);
     segment(row, blockIdx.x % heads, seen, 0, seen.count, 0);
     return;

@@ -17,7 +17,7 @@
 namespace qs {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 
 // Raised by the kernels, read and cleared by qs_device_status.
@@ -35,8 +35,13 @@ __device__ __forceinline__ int cluster_size() {
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return static_cast<int>(r);
 }
-// Barrier of every thread of the cluster; global writes before it are seen after it.
+// Barrier of every thread of the cluster; global writes before it are seen after it
+// (within one CTA without the fence, which waits for them to reach L2).
 __device__ __forceinline__ void cluster_barrier() {
+  if (cluster_size() == 1) {
+    __syncthreads();
+    return;
+  }
   __threadfence();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -106,20 +111,25 @@ __device__ __forceinline__ int counts_before(const int *head, int *total) {
 }
 
 // Numbers this CTA's share of the pages with pred true, in page order, from the
-// cluster-wide prefix: emit(page, rank) for each.  All threads call it; the first
-// pass counts, a cluster barrier exchanges the counts, the second pass numbers.
-template <class Pred, class Emit>
+// cluster-wide prefix: emit(page, rank, pred, their number in all) for every page.  All
+// threads call it; a first pass counts and a cluster barrier exchanges the counts (one
+// CTA needs neither, unless emit asks for the number: kNeedAll), the second pass numbers.
+template <bool kNeedAll, class Pred, class Emit>
 __device__ __forceinline__ int number_pages(int pages, int *head, int *tmp, Pred pred, Emit emit) {
   int lo, hi;
   share_of(pages, &lo, &hi);
-  int mine = 0;
-  for (int p = lo + threadIdx.x; p < hi; p += kThreads) mine += pred(p) ? 1 : 0;
-  int total;
-  block_prefix(mine, &total, tmp);
-  if (threadIdx.x == 0) head[8 + cluster_rank()] = total;
-  cluster_barrier();
-  int all;
-  int base = counts_before(head, &all);
+  int all = 0, base = 0;
+  if (cluster_size() > 1 || kNeedAll) {
+    int mine = 0;
+#pragma unroll 4
+    for (int p = lo + threadIdx.x; p < hi; p += kThreads) mine += pred(p) ? 1 : 0;
+    block_prefix(mine, &all, tmp);
+    if (cluster_size() > 1) {
+      if (threadIdx.x == 0) head[8 + cluster_rank()] = all;
+      cluster_barrier();
+      base = counts_before(head, &all);
+    }
+  }
   for (int p0 = lo; p0 < hi; p0 += kThreads) {
     const int p = p0 + threadIdx.x;
     const bool is = p < hi && pred(p);
@@ -128,7 +138,7 @@ __device__ __forceinline__ int number_pages(int pages, int *head, int *tmp, Pred
     if (p < hi) emit(p, r, is, all);
     base += n;
   }
-  return all;
+  return cluster_size() > 1 || kNeedAll ? all : base;
 }
 
 struct Tables {
@@ -147,73 +157,73 @@ __device__ __forceinline__ int pages_of(int64_t n, int shift, int width) {
 // other children get a page of their own, whose filled tokens the second launch
 // copies.  Counts change by references after minus references before, so counts
 // that the caller holds besides the table's stay.
-__global__ void __launch_bounds__(kThreads) fork_kernel(Tables t, const int *parents, Work w) {
+__global__ void __launch_bounds__(kThreads, 1) fork_kernel(Tables t, const int *parents, Work w) {
   extern __shared__ int sm[];
   __shared__ int tmp[32];
-  int *first = sm, *kids = sm + t.rows, *rank = sm + 2 * t.rows;
+  int *first = sm, *kids = sm + t.rows, *rank = sm + 2 * t.rows, *par = sm + 3 * t.rows, *len = sm + 4 * t.rows;
   pdl_wait();
   pdl_launch_dependents();
   const int nthreads = kThreads * cluster_size(), tid = cluster_rank() * kThreads + threadIdx.x;
-  auto parent = [&](int i) {
-    const int p = parents[i];
-    return p >= 0 && p < t.rows ? p : -1;
-  };
-  auto length = [&](int i) { return max(0, t.lengths[i]); };
-  for (int i = threadIdx.x; i < t.rows; i += kThreads) first[i] = t.rows, kids[i] = 0;
-  __syncthreads();
+  const int fill_mask = (1 << t.page_shift) - 1;
+  int lo, hi;
+  share_of(t.pages, &lo, &hi);
   for (int i = threadIdx.x; i < t.rows; i += kThreads) {
-    const int p = parent(i);
-    if (p >= 0) {
-      atomicAdd(&kids[p], 1);
-      atomicMin(&first[p], i);
-    } else if (parents[i] != -1 && cluster_rank() == 0) {
-      flag_error(kCacheErrParent);
-    }
+    const int p = parents[i];
+    first[i] = t.rows;
+    kids[i] = 0;
+    len[i] = max(0, t.lengths[i]);
+    par[i] = p >= 0 && p < t.rows ? p : -1;
+    if (par[i] < 0 && p != -1 && cluster_rank() == 0) flag_error(kCacheErrParent);
   }
+#pragma unroll 4
+  for (int p = lo + threadIdx.x; p < hi; p += kThreads) t.refcount_out[p] = t.refcount[p];
+  __syncthreads();
+  for (int i = threadIdx.x; i < t.rows; i += kThreads)
+    if (par[i] >= 0) {
+      atomicAdd(&kids[par[i]], 1);
+      atomicMin(&first[par[i]], i);
+    }
   __syncthreads();
   // rows that need a page of their own, numbered in row order
   int want = 0;
   for (int i0 = 0; i0 < t.rows; i0 += kThreads) {
     const int i = i0 + threadIdx.x;
     bool dup = false;
-    if (i < t.rows) {
-      const int p = parent(i);
-      if (p >= 0 && first[p] != i) {
-        const int n = length(p);
-        dup = (n & ((1 << t.page_shift) - 1)) != 0 && (n >> t.page_shift) < t.width;
-      }
+    if (i < t.rows && par[i] >= 0 && first[par[i]] != i) {
+      const int n = len[par[i]];
+      dup = (n & fill_mask) != 0 && (n >> t.page_shift) < t.width;
     }
     int n;
     const int r = want + block_prefix(dup ? 1 : 0, &n, tmp);
     if (i < t.rows) rank[i] = dup ? r : -1;
     want += n;
   }
-  int lo, hi;
-  share_of(t.pages, &lo, &hi);
-  for (int p = lo + threadIdx.x; p < hi; p += kThreads) t.refcount_out[p] = t.refcount[p];
   cluster_barrier();
-  const int lane = threadIdx.x & 31;
-  for (int i = tid >> 5; i < t.rows; i += nthreads >> 5) {
-    {  // references of the old row that go or come
-      const int n = length(i), used = pages_of(n, t.page_shift, t.width), delta = kids[i] - 1;
-      const int whole = min(used, n >> t.page_shift);
-      const int *row = t.table + static_cast<int64_t>(i) * t.width;
-      for (int c = lane; c < used; c += 32) {
-        const int d = c < whole ? delta : (kids[i] ? 0 : -1);
-        const int p = row[c];
-        if (d != 0 && p >= 0 && p < t.pages) atomicAdd(t.refcount_out + p, d);
-      }
-    }
-    const int p = parent(i), n = p < 0 ? 0 : length(p), used = pages_of(n, t.page_shift, t.width);
-    const int *row = t.table + static_cast<int64_t>(p) * t.width;
-    int *out = t.table_out + static_cast<int64_t>(i) * t.width;
-    const int keep = used - (rank[i] >= 0 ? 1 : 0);  // the last entry of a copying row follows below
-    for (int c = lane; c < t.width; c += 32)
-      if (c < keep || c >= used) out[c] = c < used ? row[c] : -1;
-    if (lane == 0) t.lengths_out[i] = n;
+  // entry by entry: the references of the old row that go or come, and the new row
+  const int64_t entries = static_cast<int64_t>(t.rows) * t.width;
+#pragma unroll 4
+  for (int64_t e = tid; e < entries; e += nthreads) {
+    const int i = static_cast<int>(static_cast<uint32_t>(e) / static_cast<uint32_t>(t.width));
+    const int c = static_cast<int>(e - static_cast<int64_t>(i) * t.width);
+    const int p = par[i];
+    const int old_used = pages_of(len[i], t.page_shift, t.width), whole = min(old_used, len[i] >> t.page_shift);
+    const int n = p < 0 ? 0 : len[p], used = pages_of(n, t.page_shift, t.width);
+    const int d = c < whole ? kids[i] - 1 : (kids[i] ? 0 : -1);
+    const int was = c < old_used && d != 0 ? t.table[e] : -1;
+    const int is = c < used ? t.table[static_cast<int64_t>(p) * t.width + c] : -1;
+    if (was >= 0 && was < t.pages) atomicAdd(t.refcount_out + was, d);
+    if (rank[i] >= 0 && c == used - 1) w.list[rank[i]].x = is;  // a copying row's last entry follows below
+    else t.table_out[e] = is;
+    if (c == 0) t.lengths_out[i] = n;
   }
+  if (t.width == 0)
+    for (int i = tid; i < t.rows; i += nthreads) t.lengths_out[i] = par[i] < 0 ? 0 : len[par[i]];
   cluster_barrier();
-  const int free_pages = number_pages(
+  if (want == 0) {  // the same in every CTA
+    if (tid == 0) w.head[0] = 0;
+    return;
+  }
+  const int free_pages = number_pages<false>(
       t.pages, w.head, tmp, [&](int p) { return __ldcg(t.refcount_out + p) == 0; },
       [&](int p, int r, bool is, int) {
         if (is && r < want) w.a[r] = p;
@@ -222,12 +232,12 @@ __global__ void __launch_bounds__(kThreads) fork_kernel(Tables t, const int *par
   for (int i = tid; i < t.rows; i += nthreads) {
     const int r = rank[i];
     if (r < 0) continue;
-    const int p = parent(i), n = length(p), last = n >> t.page_shift;
-    const int page = r < free_pages ? __ldcg(w.a + r) : -1;
-    t.table_out[static_cast<int64_t>(i) * t.width + last] = page;
+    const int n = len[par[i]], page = r < free_pages ? __ldcg(w.a + r) : -1;
+    t.table_out[static_cast<int64_t>(i) * t.width + (n >> t.page_shift)] = page;
     if (page >= 0) t.refcount_out[page] = 1;
     else flag_error(kCacheErrPages);
-    w.list[r] = make_int4(t.table[static_cast<int64_t>(p) * t.width + last], page, n & ((1 << t.page_shift) - 1), 0);
+    w.list[r].y = page;
+    w.list[r].z = n & fill_mask;
   }
   if (tid == 0) w.head[0] = want;
 }
@@ -235,7 +245,7 @@ __global__ void __launch_bounds__(kThreads) fork_kernel(Tables t, const int *par
 // ---- compact ---------------------------------------------------------------------
 // With U pages in use, the used pages from U on move to the holes below U, both in
 // ascending order; tables and counts follow.
-__global__ void __launch_bounds__(kThreads) compact_kernel(Tables t, int *used_out, Work w) {
+__global__ void __launch_bounds__(kThreads, 1) compact_kernel(Tables t, int *used_out, Work w) {
   __shared__ int tmp[32];
   pdl_wait();
   pdl_launch_dependents();
@@ -243,7 +253,7 @@ __global__ void __launch_bounds__(kThreads) compact_kernel(Tables t, int *used_o
   if (tid == 0) w.head[1] = 0;
   // rank = used pages before p.  A hole p < U is number p - rank among the holes; a
   // used page p >= U goes by its rank, and those ranks end at U - 1.
-  const int used = number_pages(
+  const int used = number_pages<true>(
       t.pages, w.head, tmp, [&](int p) { return t.refcount[p] > 0; },
       [&](int p, int r, bool is, int all) {
         t.refcount_out[p] = t.refcount[p];
@@ -266,21 +276,21 @@ __global__ void __launch_bounds__(kThreads) compact_kernel(Tables t, int *used_o
     used_out[0] = used;
   }
   cluster_barrier();
-  const int lane = threadIdx.x & 31;
-  for (int i = tid >> 5; i < t.rows; i += nthreads >> 5) {
-    const int n = pages_of(max(0, t.lengths[i]), t.page_shift, t.width);
-    for (int c = lane; c < t.width; c += 32) {
-      const int64_t at = static_cast<int64_t>(i) * t.width + c;
-      const int p = c < n ? t.table[at] : -1;
-      t.table_out[at] = p >= 0 && p < t.pages ? __ldcg(w.map + p) : -1;
-    }
+  const int64_t entries = static_cast<int64_t>(t.rows) * t.width;
+#pragma unroll 4
+  for (int64_t e = tid; e < entries; e += nthreads) {
+    const int i = static_cast<int>(static_cast<uint32_t>(e) / static_cast<uint32_t>(t.width));
+    const int c = static_cast<int>(e - static_cast<int64_t>(i) * t.width);
+    const int p = t.table[e];
+    const bool held = c < pages_of(max(0, t.lengths[i]), t.page_shift, t.width) && p >= 0 && p < t.pages;
+    t.table_out[e] = held ? __ldcg(w.map + p) : -1;
   }
 }
 
 // ---- extend ----------------------------------------------------------------------
 // Row i grows by add[i] tokens; its new pages are the lowest free ones, numbered in
 // row and then column order.
-__global__ void __launch_bounds__(kThreads) extend_kernel(Tables t, const int *add, Work w) {
+__global__ void __launch_bounds__(kThreads, 1) extend_kernel(Tables t, const int *add, Work w) {
   extern __shared__ int sm[];
   __shared__ int tmp[32];
   int *start = sm, *had_s = sm + t.rows, *len_s = sm + 2 * t.rows;
@@ -308,7 +318,7 @@ __global__ void __launch_bounds__(kThreads) extend_kernel(Tables t, const int *a
     if (i < t.rows) start[i] = before;
     want += n;
   }
-  const int free_pages = number_pages(
+  const int free_pages = number_pages<false>(
       t.pages, w.head, tmp, [&](int p) { return t.refcount[p] == 0; },
       [&](int p, int r, bool is, int) {
         const bool take = is && r < want;
@@ -320,18 +330,18 @@ __global__ void __launch_bounds__(kThreads) extend_kernel(Tables t, const int *a
   // the outputs may be the inputs: every input value was read before the last barrier,
   // except the table entries that stay where they are
   for (int p = tid; p < t.pages; p += nthreads) t.refcount_out[p] = __ldcg(w.b + p);
-  const int lane = threadIdx.x & 31;
-  for (int i = tid >> 5; i < t.rows; i += nthreads >> 5) {
-    const int had = had_s[i], has = pages_of(len_s[i], t.page_shift, t.width);
-    for (int c = lane; c < t.width; c += 32) {
-      const int64_t at = static_cast<int64_t>(i) * t.width + c;
-      int p = -1;
-      if (c < had) p = t.table[at];
-      else if (c < has && start[i] + c - had < free_pages) p = __ldcg(w.a + start[i] + c - had);
-      t.table_out[at] = p;
-    }
-    if (lane == 0) t.lengths_out[i] = len_s[i];
+  const int64_t entries = static_cast<int64_t>(t.rows) * t.width;
+#pragma unroll 4
+  for (int64_t e = tid; e < entries; e += nthreads) {
+    const int i = static_cast<int>(static_cast<uint32_t>(e) / static_cast<uint32_t>(t.width));
+    const int c = static_cast<int>(e - static_cast<int64_t>(i) * t.width);
+    const int had = had_s[i], has = pages_of(len_s[i], t.page_shift, t.width), r = start[i] + c - had;
+    int p = -1;
+    if (c < had) p = t.table[e];
+    else if (c < has && r < free_pages) p = __ldcg(w.a + r);
+    t.table_out[e] = p;
   }
+  for (int i = tid; i < t.rows; i += nthreads) t.lengths_out[i] = len_s[i];
 }
 
 // ---- moving page contents ------------------------------------------------------------
@@ -353,42 +363,52 @@ Pool make_pool(const qs_kv_pool &p) {
   return q;
 }
 
-// A warp takes one (copy, layer, K or V, head): `tokens` rows of `chunks` 16-byte pieces.
+// A warp takes 4 KB (256 pieces of 16 bytes) of one (copy, layer, K or V, head) at a time:
+// `tokens` rows of `chunks` pieces.  The list is kept in shared memory, so that the parts
+// that lie beyond a part-filled page's tokens cost next to nothing.
 constexpr int kCopyUnroll = 8;
-__global__ void __launch_bounds__(256) copy_pages_kernel(Pool p, const int *head, const int4 *list) {
+constexpr int kCopyList = 1024;
+__global__ void __launch_bounds__(256) copy_pages_kernel(Pool p, int page, const int *head, const int4 *list) {
+  __shared__ int4 near[kCopyList];
   pdl_wait();
   pdl_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  const int64_t units = static_cast<int64_t>(head[0]) * p.layers * 2 * p.heads;
+  const int lane = threadIdx.x & 31, count = head[0];
+  for (int i = threadIdx.x; i < min(count, kCopyList); i += blockDim.x) near[i] = list[i];
+  __syncthreads();
+  const uint32_t parts = (page * p.chunks + 32 * kCopyUnroll - 1) / (32 * kCopyUnroll);
+  const uint32_t each = static_cast<uint32_t>(p.layers) * 2 * p.heads * parts;  // warps' shares per copy
+  const int64_t units = static_cast<int64_t>(count) * each;
   const int64_t step = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
   for (int64_t u = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5); u < units; u += step) {
-    const int h = static_cast<int>(u % p.heads);
-    int64_t r = u / p.heads;
+    const int at = static_cast<int>(u / each);
+    uint32_t r = static_cast<uint32_t>(u - static_cast<int64_t>(at) * each);
+    const int4 e = at < kCopyList ? near[at] : list[at];
+    const uint32_t part = r % parts;
+    const int n = e.z * p.chunks, i0 = static_cast<int>(part) * 32 * kCopyUnroll + lane;
+    if (i0 - lane >= n || e.x < 0 || e.x >= p.pages || e.y < 0 || e.y >= p.pages) continue;
+    r /= parts;
+    const uint32_t h = r % p.heads;
+    r /= p.heads;
     const bool is_v = r & 1;
-    r >>= 1;
-    const int layer = static_cast<int>(r % p.layers);
-    const int4 e = list[r / p.layers];
-    if (e.x < 0 || e.x >= p.pages || e.y < 0 || e.y >= p.pages) continue;
     const int64_t *st = is_v ? p.vs : p.ks;
-    char *base = (is_v ? p.v : p.k) + layer * st[0] + h * st[2];
+    char *base = (is_v ? p.v : p.k) + (r >> 1) * st[0] + h * st[2];
     const char *src = base + e.x * st[1];
     char *dst = base + e.y * st[1];
-    const int n = e.z * p.chunks;
-    for (int i0 = lane; i0 < n; i0 += 32 * kCopyUnroll) {
-      uint4 x[kCopyUnroll];
-      int64_t off[kCopyUnroll];
+    const int token = static_cast<int>(st[3]);
+    uint4 x[kCopyUnroll];
+    int off[kCopyUnroll];
 #pragma unroll
-      for (int j = 0; j < kCopyUnroll; ++j) {
-        const int i = i0 + 32 * j;
-        if (i < n) {
-          off[j] = (i / p.chunks) * st[3] + (i % p.chunks) * 16;
-          x[j] = *reinterpret_cast<const uint4 *>(src + off[j]);
-        }
+    for (int j = 0; j < kCopyUnroll; ++j) {
+      const int i = i0 + 32 * j;
+      if (i < n) {
+        const int row = i / p.chunks;
+        off[j] = row * token + (i - row * p.chunks) * 16;
+        x[j] = *reinterpret_cast<const uint4 *>(src + off[j]);
       }
-#pragma unroll
-      for (int j = 0; j < kCopyUnroll; ++j)
-        if (i0 + 32 * j < n) *reinterpret_cast<uint4 *>(dst + off[j]) = x[j];
     }
+#pragma unroll
+    for (int j = 0; j < kCopyUnroll; ++j)
+      if (i0 + 32 * j < n) *reinterpret_cast<uint4 *>(dst + off[j]) = x[j];
   }
 }
 
@@ -411,13 +431,16 @@ __global__ void __launch_bounds__(256) write_kernel(WriteArgs a) {
   if (tok >= a.tokens) return;
   int row = tok, back = 1;  // back: tokens from this one to the row's end
   if (a.cu) {
-    int lo = 0, hi = a.rows;  // first row whose end is past tok
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (a.cu[mid + 1] > tok) hi = mid;
-      else lo = mid + 1;
+    // the first row whose end is past tok, 32 probes at a time
+    int lo = 0, n = a.rows;
+    while (n > 0) {
+      const int step = (n + 31) >> 5, at = lo + lane * step + step - 1;
+      const int c = __popc(__ballot_sync(0xffffffffu, at < lo + n && a.cu[at + 1] <= tok));
+      const int end = lo + n;
+      lo += c * step;
+      n = min(step - 1, end - lo);
     }
-    row = lo;
+    row = min(lo, a.rows);
     if (row < a.rows) back = a.cu[row + 1] - tok;
   }
   if (row >= a.rows) return;
@@ -449,6 +472,7 @@ int launch_cluster(const char *what, void (*kern)(KArgs...), int ctas, size_t sm
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
+  if (ctas == 1) return launch_pdl(what, kern, dim3(1), dim3(kThreads), smem, s, args...);
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -470,7 +494,7 @@ int log2_of(int64_t v) {
 
 int launch_copy(const qs_kv_pool &pool, const Work &w, cudaStream_t s) {
   return launch_pdl("copy_pages", copy_pages_kernel, dim3(device_sms() * 8), dim3(256), 0, s, make_pool(pool),
-                    static_cast<const int *>(w.head), static_cast<const int4 *>(w.list));
+                    static_cast<int>(pool.page), static_cast<const int *>(w.head), static_cast<const int4 *>(w.list));
 }
 
 }  // namespace
@@ -507,7 +531,7 @@ int launch_cache_fork(const qs_kv_pool &pool, int rows, int width, const int *ta
                  table_out, lengths_out, refcount_out};
   const Work w = split_work(ws, rows, pool.pages);
   const int st = launch_cluster("cache fork", fork_kernel, cluster_for(rows, width, pool.pages),
-                                static_cast<size_t>(rows) * 12, s, t, parents, w);
+                                static_cast<size_t>(rows) * 20, s, t, parents, w);
   return st ? st : launch_copy(pool, w, s);
 }
 
