@@ -21,6 +21,10 @@
 // group begin while the one before is still being summed; with a CTA per group instead,
 // 14 to 17 us of each went into starting, the first loads and the last stores.
 //
+// Where the tiles are fewer than the SMs (few tokens over many keys), each is split along
+// the keys: a block takes a share of its key tiles and leaves its sum, maximum and output
+// in float32, and window_join_kernel puts the shares together.
+//
 // Warps: 0 loads, 1 issues the products (2 and 3 only fill their warpgroup), then four
 // per query tile for the softmax, to which the first four leave most of the registers.
 #include <cuda.h>
@@ -58,6 +62,9 @@ struct Cfg {
 struct WindowArgs {
   AttnArgs a;
   int share, tokens_per_tile, granule;  // granule: keys of a load box
+  int splits;                           // shares of a tile's keys
+  float *part_o;                        // [split][token, head][DP] where splits > 1
+  float2 *part_ml;                      // [split][token, head]: reference (log2), sum
   uint64_t wait_ns;
   int *error;
 };
@@ -220,7 +227,9 @@ struct Job {
   int pos0;         // its place in the row
   int keys;         // keys that any of the tokens sees end before this
   int sink_tiles;   // key tiles from 0
-  int from, tiles;  // first key after them, tiles in all (0: tokens to clear, -1: no more jobs)
+  int from;         // first key after them
+  int first, tiles; // this share's first tile, its tiles (0: tokens to clear, -1: no more jobs)
+  int split;        // which share
   int absent;       // a page among the keys is missing
 };
 
@@ -252,29 +261,33 @@ __device__ __forceinline__ void ask_next_block(uint32_t answer, uint32_t bar) {
                : "memory");
 }
 // The block taken over, or false where none was left.
-__device__ __forceinline__ bool next_block(uint32_t answer, int &x, int &y) {
-  uint32_t taken, bx, by;
+__device__ __forceinline__ bool next_block(uint32_t answer, int &x, int &y, int &z) {
+  uint32_t taken, bx, by, bz;
   asm volatile(
-      "{\n\t.reg .b128 a;\n\t.reg .pred p;\n\t.reg .b32 z;\n\tld.shared.b128 a, [%3];\n\t"
+      "{\n\t.reg .b128 a;\n\t.reg .pred p;\n\tld.shared.b128 a, [%4];\n\t"
       "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\tselp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
-      "mov.u32 %2, 0;\n\t@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, %2, z, _}, a;\n\t}"
-      : "=r"(taken), "=r"(bx), "=r"(by)
+      "mov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, %2, %3, _}, a;\n\t}"
+      : "=r"(taken), "=r"(bx), "=r"(by), "=r"(bz)
       : "r"(answer)
       : "memory");
   sm100::fence_proxy_async_smem();  // read before the next answer is written
   x = static_cast<int>(bx);
   y = static_cast<int>(by);
+  z = static_cast<int>(bz);
   return taken != 0;
 }
 
-// Block (x, y) of the grid as a job (a whole warp): the rows' tiles in row order, a row's
-// last tile (the most keys) first.
-__device__ __forceinline__ Job job_of(const WindowArgs &w, int x, int y, int per, int lane) {
+// Block (x, y, z) of the grid as a job (a whole warp): the rows' tiles in row order, a row's
+// last tile (the most keys) first; y the key head, z the share of the keys.
+__device__ __forceinline__ Job job_of(const WindowArgs &w, int x, int y, int z, int per, int lane) {
   const AttnArgs &a = w.a;
   const int total_tokens = static_cast<int>(a.tokens);
   Job j;
   j.row = -1;
   j.head = y;
+  j.split = z;
+  j.first = 0;
   j.q0 = j.q1 = j.t0 = 0;
   int end = 0, want = x;
   for (int r0 = 0; r0 < a.rows && j.row < 0; r0 += 32) {
@@ -315,7 +328,9 @@ __device__ __forceinline__ Job job_of(const WindowArgs &w, int x, int y, int per
     const int sinks = static_cast<int>(min(static_cast<int64_t>(min(lo, j.keys)), a.sinks));
     j.sink_tiles = (sinks + kTile - 1) / kTile;
     j.from = max(lo / w.granule * w.granule, j.sink_tiles * kTile);
-    j.tiles = j.sink_tiles + max(0, (j.keys - j.from + kTile - 1) / kTile);
+    const int all = j.sink_tiles + max(0, (j.keys - j.from + kTile - 1) / kTile);
+    j.first = static_cast<int>(static_cast<int64_t>(all) * z / w.splits);
+    j.tiles = static_cast<int>(static_cast<int64_t>(all) * (z + 1) / w.splits) - j.first;
   } else {  // a block beyond the tiles clears its share of the tokens that belong to no row
     j.t0 = end + want * per;
     j.tiles = 0;
@@ -385,6 +400,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   const uint32_t tmem = *holder;
   const int per = NQ * w.tokens_per_tile;
   auto key_of_tile = [&](const Job &j, int i) {
+    i += j.first;
     return i < j.sink_tiles ? i * kTile : j.from + (i - j.sink_tiles) * kTile;
   };
 
@@ -397,10 +413,10 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       int issued = 0, q_loads = 0, asks = 0, answers = 0;
       uint32_t landed_phase = 0;
       bool ok = true;
-      int bx = blockIdx.x, by = blockIdx.y;
+      int bx = blockIdx.x, by = blockIdx.y, bz = blockIdx.z;
       for (int num = 0; ok; ++num) {
         const int slot = num & 1;
-        const Job j = job_of(w, bx, by, per, lane);
+        const Job j = job_of(w, bx, by, bz, per, lane);
         if (num >= 2) ok = sm100::mbar_wait_warp(job_empty(slot), ((num >> 1) - 1) & 1, w.wait_ns);
         if (!ok) break;
         if (lane == 0) {
@@ -478,7 +494,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         if (!ok) break;
         ok = sm100::mbar_wait_warp(asked, num & 1, w.wait_ns);
         if (ok) ++answers;
-        if (!ok || !next_block(answer, bx, by)) {
+        if (!ok || !next_block(answer, bx, by, bz)) {
           // no block is left: the job after this one says so
           const int last = (num + 1) & 1;
           if (ok && num >= 1) ok = sm100::mbar_wait_warp(job_empty(last), (((num + 1) >> 1) - 1) & 1, w.wait_ns);
@@ -606,6 +622,10 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         for (int i = tid - 128; i < count * a.dim; i += NQ * 128) {
           const int64_t at =
               static_cast<int64_t>(j.t0 + i / a.dim / w.share) * a.q_heads + j.head * w.share + i / a.dim % w.share;
+          if (w.splits > 1) {  // an empty share
+            if (i % a.dim == 0) w.part_ml[j.split * a.tokens * a.q_heads + at] = make_float2(-INFINITY, 0.f);
+            continue;
+          }
           store1(static_cast<T *>(a.out) + at * a.dim + i % a.dim, 0.f);
           if (i % a.dim == 0 && a.lse) a.lse[at] = -INFINITY;
         }
@@ -723,27 +743,18 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       sm100::tc_fence_after_sync();
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const int64_t at = static_cast<int64_t>(token) * a.q_heads + j.head * w.share + r % w.share;
-      // 64 columns at a time through shared memory, so that a warp stores whole lines: four
-      // rows of 128 bytes where its threads' own rows would be 32 lines for 16 bytes each
+      // 32 words of each row at a time through shared memory, so that a warp stores whole
+      // lines: four rows of 128 bytes where its threads' own rows would be 32 lines for 16
+      // bytes each
       const uint32_t stage = out_sm + (warp - 4) * 4096, mine = stage + lane * 128;
       const uint32_t reals = __ballot_sync(0xffffffffu, real);
       const int64_t from = real ? at : 0;
+      auto send = [&](const uint32_t *words, char *rows, int64_t row_bytes, int bytes) {
 #pragma unroll
-      for (int c = 0; c < DP; c += 64) {
-        uint32_t o[64];
-        tmem_ld_32(o_at + c, o);
-        tmem_ld_32(o_at + c + 32, o + 32);
-        sm100::tmem_ld_wait();
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          uint32_t p[4];
-#pragma unroll
-          for (int y = 0; y < 4; ++y)
-            split16<T>(__uint_as_float(o[8 * x + 2 * y]) * inv, __uint_as_float(o[8 * x + 2 * y + 1]) * inv, p[y]);
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(mine + ((x ^ (lane & 7)) << 4)), "r"(p[0]),
-                       "r"(p[1]), "r"(p[2]), "r"(p[3])
+        for (int x = 0; x < 8; ++x)
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(mine + ((x ^ (lane & 7)) << 4)), "r"(words[4 * x]),
+                       "r"(words[4 * x + 1]), "r"(words[4 * x + 2]), "r"(words[4 * x + 3])
                        : "memory");
-        }
         __syncwarp();
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
@@ -754,10 +765,33 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
                        : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                        : "r"(stage + row * 128 + ((piece ^ (row & 7)) << 4))
                        : "memory");
-          if (((reals >> row) & 1) && c + piece * 8 < a.dim)
-            *reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + to * a.dim + c + piece * 8) = v;
+          if (((reals >> row) & 1) && piece * 16 < bytes) *reinterpret_cast<uint4 *>(rows + to * row_bytes + piece * 16) = v;
         }
         __syncwarp();
+      };
+      if (w.splits > 1) {
+        const int64_t base = j.split * a.tokens * a.q_heads;
+#pragma unroll
+        for (int c = 0; c < DP; c += 32) {
+          uint32_t o[32];
+          tmem_ld_32(o_at + c, o);
+          sm100::tmem_ld_wait();
+          send(o, reinterpret_cast<char *>(w.part_o + base * DP + c), DP * 4, 128);
+        }
+        if (real) w.part_ml[base + at] = make_float2(m == -INFINITY ? -INFINITY : m * scale2, l);
+        sm100::tc_fence_before_sync();
+        continue;
+      }
+#pragma unroll
+      for (int c = 0; c < DP; c += 64) {
+        uint32_t o[64];
+        tmem_ld_32(o_at + c, o);
+        tmem_ld_32(o_at + c + 32, o + 32);
+        sm100::tmem_ld_wait();
+#pragma unroll
+        for (int x = 0; x < 32; ++x)
+          split16<T>(__uint_as_float(o[2 * x]) * inv, __uint_as_float(o[2 * x + 1]) * inv, o[x]);
+        send(o, reinterpret_cast<char *>(static_cast<T *>(a.out) + c), a.dim * 2, (a.dim - c) * 2);
       }
       sm100::tc_fence_before_sync();  // O is read: the next job's first weights release it
       if (real && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m * scale2 * kLn2) + logf(l);
@@ -768,6 +802,64 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   __syncthreads();
   sm100::tc_fence_after_sync();
   if (warp == 1) sm100::tmem_dealloc(tmem, C::tmem_cols);
+}
+
+// Joins a row's shares, a warp for each token and query head.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) window_join_kernel(WindowArgs w) {
+  constexpr int PER = DP / 32, U = 4;  // outputs per lane, shares at a time
+  pdl_wait();
+  pdl_launch_dependents();
+  const AttnArgs &a = w.a;
+  const int lane = threadIdx.x & 31;
+  const int64_t rows = a.tokens * a.q_heads, at = blockIdx.x * int64_t(8) + (threadIdx.x >> 5);
+  if (at >= rows) return;
+  float m = -INFINITY;
+  for (int i = lane; i < w.splits; i += 32) m = fmaxf(m, w.part_ml[i * rows + at].x);
+#pragma unroll
+  for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+  float l = 0.f, o[PER] = {};
+  for (int i0 = 0; i0 < w.splits; i0 += U) {
+    float2 ml[U];
+    float x[U][PER];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i0 + u >= w.splits) break;
+      ml[u] = w.part_ml[(i0 + u) * rows + at];
+#pragma unroll
+      for (int c = 0; c < PER; ++c) x[u][c] = w.part_o[((i0 + u) * rows + at) * DP + lane * PER + c];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i0 + u >= w.splits) break;
+      if (ml[u].y == 0.f) continue;  // an empty share has no output
+      const float p = weight(ml[u].x, m);
+      l += p * ml[u].y;
+#pragma unroll
+      for (int c = 0; c < PER; ++c) o[c] += p * x[u][c];
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int c = 0; c < PER; c += 2) {
+    uint32_t packed;
+    split16<T>(o[c] * inv, o[c + 1] * inv, packed);
+    if (lane * PER + c < a.dim) *reinterpret_cast<uint32_t *>(static_cast<T *>(a.out) + at * a.dim + lane * PER + c) = packed;
+  }
+  if (lane == 0 && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+// Shares of a tile's keys: as many as there are SMs for, of at least two key tiles each.
+int splits_for(int64_t tokens, int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t page, int64_t width,
+               int64_t window, int64_t sinks) {
+  const int64_t share = q_heads / kv_heads;
+  if (share > kTile) return 1;
+  const int64_t per = 2 * (kTile / share), blocks = (ceil_div(tokens, per) + (rows < tokens ? rows : tokens)) * kv_heads;
+  int64_t keys = width * page;
+  if (window > 0 && window < keys && sinks < keys && window + sinks + per < keys) keys = window + sinks + per;
+  int64_t n = ceil_div(ceil_div(keys, kTile), 2);
+  if (n > 148 / (blocks > 0 ? blocks : 1)) n = 148 / (blocks > 0 ? blocks : 1);
+  return static_cast<int>(n < 1 ? 1 : n);
 }
 
 template <typename T, int DP, int NQ>
@@ -801,14 +893,23 @@ int run(const AttnArgs &a, cudaStream_t s) {
   static const cudaError_t attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem);
   if (attr != cudaSuccess) return fail(QS_ERR_CUDA, "attention (window): %s", cudaGetErrorString(attr));
   const int64_t per = static_cast<int64_t>(NQ) * w.tokens_per_tile;
-  const dim3 grid(static_cast<unsigned>(ceil_div(a.tokens, per) + a.rows), a.kv_heads);
-  return launch_pdl("attention (window)", kern, grid, dim3(C::threads), C::smem, s, qmap, kmap, vmap, w);
+  const int64_t rows = a.tokens * a.q_heads;
+  w.splits = splits_for(a.tokens, a.rows, a.q_heads, a.kv_heads, page, a.width, a.window, a.sinks);
+  w.part_o = static_cast<float *>(a.ws);
+  w.part_ml = reinterpret_cast<float2 *>(w.part_o + w.splits * rows * DP);
+  const dim3 grid(static_cast<unsigned>(ceil_div(a.tokens, per) + a.rows), a.kv_heads, w.splits);
+  const int st = launch_pdl("attention (window)", kern, grid, dim3(C::threads), C::smem, s, qmap, kmap, vmap, w);
+  if (st || w.splits == 1) return st;
+  return launch_pdl("attention (window, join)", window_join_kernel<T, DP>, dim3(static_cast<unsigned>(ceil_div(rows, 8))),
+                    dim3(256), 0, s, w);
 }
 
 }  // namespace
 
-int64_t attn_window_workspace_bytes(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t) {
-  return 0;
+int64_t attn_window_workspace_bytes(int64_t tokens, int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t dim,
+                                    int64_t page, int64_t width, int64_t window, int64_t sinks) {
+  const int64_t splits = splits_for(tokens, rows, q_heads, kv_heads, page, width, window, sinks);
+  return splits == 1 ? 0 : splits * tokens * q_heads * ((dim <= 64 ? 64 : 128) + 2) * 4;
 }
 
 int launch_attn_window(const AttnArgs &a, cudaStream_t s) {

@@ -234,6 +234,9 @@ WINDOW = [
     ([9, 1, 4], [700, 30, 250], 16, 4, 16, 64, 256, 4),
     ([2, 3, 1] * 40, [10, 50, 300] * 40, 8, 2, 16, 64, 64, 2),  # more rows than a warp
     ([1500], [0], 8, 8, 64, 128, 0, 0),
+    ([8], [15000], 8, 1, 64, 128, 0, 0),                   # few tokens over many keys: shares of the keys, joined
+    ([5, 0, 70, 1], [9000, 50, 40, 0], 8, 2, 32, 64, 0, 0),   # shares that are empty for the short rows
+    ([3, 2], [15000, 2000], 6, 2, 16, 96, 5000, 300),
 ]
 
 
