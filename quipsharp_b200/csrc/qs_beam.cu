@@ -8,9 +8,9 @@
 // largest logit.  The n-th largest of those thread maxima is a bound that at least
 // n logits of the chunk reach and few others do, so only the few threads whose
 // maximum reaches it look at their logits again.  beam_merge: one CTA per search
-// joins the chunks' sorted lists into the beams', and the beams' into the result;
-// a candidate's place in the merged list is the sum of its places in each list
-// (binary searches), so nothing is sorted and nothing depends on arrival order.
+// joins the chunks' lists into the beams', and the beams' into the result; a candidate's
+// place is the number of those ahead of it, so nothing is sorted and nothing depends on
+// the order of arrival.
 //
 // Bound: the logits' bytes, once.
 #include <cmath>
@@ -465,10 +465,11 @@ __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;
 __global__ void __launch_bounds__(kT) beam_merge_kernel(MergeArgs a) {
   extern __shared__ uint32_t sm[];
   uint2 *in = reinterpret_cast<uint2 *>(sm);                // chunks' lists of some beams
-  uint32_t *key = sm + 2 * kLists;                          // [beams][n]: score keys, falling
+  uint16_t *left = reinterpret_cast<uint16_t *>(sm + 2 * kLists);  // entries of each beam that matter
+  uint32_t *key = sm + 2 * kLists + kLists / 2;             // [beams][n]: score keys, falling
   int *tok = reinterpret_cast<int *>(key + a.beams * a.n);  // [beams][n]
   int *place = tok + a.beams * a.n;                         // [beams][n]: places in the joint list
-  Beam *beams = reinterpret_cast<Beam *>(sm + 2 * kLists + round4(3 * a.beams * a.n));
+  Beam *beams = reinterpret_cast<Beam *>(key + round4(3 * a.beams * a.n));
   pdl_wait();
   pdl_launch_dependents();
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
@@ -494,16 +495,41 @@ __global__ void __launch_bounds__(kT) beam_merge_kernel(MergeArgs a) {
       for (int i = tid; i < kn * per; i += kT) copy8(&in[i], &lists[static_cast<int64_t>(k0) * per + i]);
     copies_done();
     __syncthreads();
-    for (int i = tid; i < kn * per; i += kT) {
-      const int k = i / per, c = (i % per) / a.n, j = i % a.n;
-      const uint2 x = in[i];
-      if (x.x == 0u) continue;
-      int r = j;
-      for (int o = 0; o < a.chunks && r < a.n; ++o)
-        if (o != c) r += entries_before(&in[k * per + o * a.n].x, 2, a.n, x.x, o < c);
-      if (r >= a.n) continue;
-      key[(k0 + k) * a.n + r] = x.x;
-      tok[(k0 + k) * a.n + r] = static_cast<int>(x.y);
+    // a warp for each beam: the upper half of its n-th largest key, bit by bit; the entries
+    // that reach it; their places by counting those ahead
+    for (int k = tid >> 5; k < kn; k += kT / 32) {
+      const uint2 *mine = in + k * per;
+      uint16_t *some = left + k * per;
+      uint32_t bound = 0;
+#pragma unroll 1
+      for (int bit = 15; bit >= 0 && per > 48; --bit) {  // fewer are counted through as they are
+        const uint32_t t = bound | (1u << bit);
+        int c = 0;
+#pragma unroll 4
+        for (int i = lane; i < per; i += 32) c += (mine[i].x >> 16) >= t ? 1 : 0;
+        if (__reduce_add_sync(0xffffffffu, c) >= a.n) bound = t;
+      }
+      bound <<= 16;
+      int count = 0;
+      for (int i0 = 0; i0 < per; i0 += 32) {
+        const int i = i0 + lane;
+        const uint32_t key_i = i < per ? mine[i].x : 0u;
+        const uint32_t who = __ballot_sync(0xffffffffu, key_i != 0u && key_i >= bound);
+        if ((who >> lane) & 1) some[count + __popc(who & ((1u << lane) - 1u))] = static_cast<uint16_t>(i);
+        count += __popc(who);
+      }
+      __syncwarp();
+      for (int s = lane; s < count; s += 32) {
+        const uint2 x = mine[some[s]];
+        int r = 0;
+        for (int o = 0; o < count && r < a.n; ++o) {
+          const uint2 y = mine[some[o]];
+          r += before(y.x, static_cast<int>(y.y), x.x, static_cast<int>(x.y)) ? 1 : 0;
+        }
+        if (r >= a.n) continue;
+        key[(k0 + k) * a.n + r] = x.x;
+        tok[(k0 + k) * a.n + r] = static_cast<int>(x.y);
+      }
     }
     __syncthreads();
   }
@@ -585,9 +611,9 @@ int launch_beam_select(const void *logits, int dtype, int64_t batch_stride, int6
   if (st) return st;
   const MergeArgs m{static_cast<int>(beams), n, chunks, pad, stats, cand, scores, finished, scores_out, parents_out,
                     tokens_out};
-  const size_t smem = static_cast<size_t>(kLists) * 8 + round4(static_cast<int>(3 * beams * n)) * 4 + beams * sizeof(Beam);
+  const size_t smem = static_cast<size_t>(kLists) * 10 + round4(static_cast<int>(3 * beams * n)) * 4 + beams * sizeof(Beam);
   static const cudaError_t attr = cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                       kLists * 8 + kBeamMaxBeams * kBeamMaxN * 12 + kBeamMaxBeams * (int)sizeof(Beam));
+                                                       kLists * 10 + kBeamMaxBeams * kBeamMaxN * 12 + kBeamMaxBeams * (int)sizeof(Beam));
   if (attr != cudaSuccess) return fail(QS_ERR_CUDA, "beam merge: %s", cudaGetErrorString(attr));
   return launch_pdl("beam merge", beam_merge_kernel, dim3(static_cast<unsigned>(batch)), dim3(kT), smem, s, m);
 }
