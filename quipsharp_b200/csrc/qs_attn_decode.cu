@@ -32,6 +32,7 @@ constexpr int kCtasPerSm = 2;     // of four warps
 constexpr int kDealWarps = 4;     // warps of a CTA that is dealt ranges
 constexpr int kRanges = 148 * kCtasPerSm * kRangesPerCta;
 constexpr int kMinRange = 16;     // groups of a range at least: 4 per warp, or the joins cost more than the split saves
+constexpr int kLongRange = 128;   // the start of a shorter range is not paid for by the evener shares
 constexpr int kWholeGroups = 80;  // a CTA of four warps takes 20 steps for them
 
 // The groups of 16 keys that a row's newest token sees: the first `sink` groups, then
@@ -75,6 +76,7 @@ struct Smem {
   T kv[W][kStages][2][kKeys * DP];
   float ml[W][kRows][2];
   int64_t sums[W * 32 + 1][2];
+  int lengths[W * 32];  // of the first rows
 };
 
 // One warp's softmax state over 16 query rows (R8: only the first 8 are real).
@@ -318,7 +320,8 @@ attn_decode_kernel(AttnArgs a, Ws ws, int blocks, int share) {
   {
     int64_t c = 0, p = 0;
     for (int r = first_row; r < last_row; ++r) {
-      const int n = seen_of(a.lengths[r], a).count;
+      const int length = a.lengths[r], n = seen_of(length, a).count;
+      if (r == tid) sm.lengths[tid] = length;  // a row per thread: they are all here
       c += n;
       p += padded(n, kMinRange);
     }
@@ -346,7 +349,9 @@ attn_decode_kernel(AttnArgs a, Ws ws, int blocks, int share) {
   const int col = dense ? 0 : 1;
   d.pad = dense ? 1 : kMinRange;
   d.total = sm.sums[kThreads][col] * heads;
-  d.range = dense ? static_cast<int>(max(static_cast<int64_t>(kMinRange), (d.total + kRanges - 1) / kRanges)) : kMinRange;
+  const int64_t one_each = (d.total + 148 * kCtasPerSm - 1) / (148 * kCtasPerSm);
+  d.range = dense ? static_cast<int>(max(min(one_each, static_cast<int64_t>(kLongRange)), (d.total + kRanges - 1) / kRanges))
+                  : kMinRange;
   if (blockIdx.x == 0) {  // for the join
     int64_t at = sm.sums[tid][col];
     for (int r = first_row; r < last_row; ++r) {
@@ -374,7 +379,7 @@ attn_decode_kernel(AttnArgs a, Ws ws, int blocks, int share) {
     int64_t at = sm.sums[lo][col] * heads;  // the row's first group
     int64_t pos = r0;
     while (pos < r1 && row < a.rows) {
-      const Seen seen = seen_of(a.lengths[row], a);
+      const Seen seen = seen_of(per == 1 ? sm.lengths[row] : a.lengths[row], a);
       const int c = padded(seen.count, d.pad);
       if (at + static_cast<int64_t>(c) * heads <= pos) {
         at += static_cast<int64_t>(c) * heads;
@@ -391,21 +396,24 @@ attn_decode_kernel(AttnArgs a, Ws ws, int blocks, int share) {
   }
 }
 
-// Joins the partial results of one segment's ranges, in their order, a warp for each query
-// row; segments that no range covers (rows that see nothing) get zeros.
-template <typename T, int DP>
+// Joins the partial results of one segment's ranges, in their order; segments that no range
+// covers (rows that see nothing) get zeros.  A warp for each query row, or, where the rows
+// are few and their parts may be many, four (WPR) that take every fourth part each.
+template <typename T, int DP, int WPR>
 __global__ void __launch_bounds__(128) attn_join_kernel(AttnArgs a, Ws ws, int blocks, int share) {
-  constexpr int PER = DP / 32, U = 4;  // outputs per lane, partial results at a time
+  constexpr int PER = DP / 32, U = 4, ROWS = 4 / WPR;  // outputs per lane, parts at a time, rows of a CTA
+  __shared__ float sums[WPR > 1 ? 4 : 1][DP + 1];
   pdl_wait();
   pdl_launch_dependents();
-  const int heads = a.kv_heads * blocks, lane = threadIdx.x & 31;
-  const int segment = blockIdx.x / (kRows / 4), r = blockIdx.x % (kRows / 4) * 4 + (threadIdx.x >> 5);
+  const int heads = a.kv_heads * blocks, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int segment = blockIdx.x / (kRows / ROWS), r = blockIdx.x % (kRows / ROWS) * ROWS + warp / WPR;
   const int row = segment / heads, head = segment % heads;
   const int kvh = head / blocks, h0 = kvh * share + (head % blocks) * kRows;
-  if (r >= min(kRows, share - (head % blocks) * kRows)) return;
   const int range = ws.deal[0], pad = ws.deal[1];
+  const int64_t start = ws.start[row];
   const int count = seen_of(a.lengths[row], a).count;
-  const int64_t seg = ws.start[row] * heads + static_cast<int64_t>(head) * padded(count, pad);
+  if (r >= min(kRows, share - (head % blocks) * kRows)) return;  // with several warps a row, the whole CTA
+  const int64_t seg = start * heads + static_cast<int64_t>(head) * padded(count, pad);
   const int64_t f = seg / range, e = count ? (seg + count - 1) / range : f;
   if (count && f == e) return;  // one range had it whole
   const int parts = count ? static_cast<int>(e - f) + 1 : 0;
@@ -415,14 +423,14 @@ __global__ void __launch_bounds__(128) attn_join_kernel(AttnArgs a, Ws ws, int b
 #pragma unroll
   for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
   float l = 0.f, o[PER] = {};
-  for (int i0 = 0; i0 < parts; i0 += U) {
+  for (int i0 = warp % WPR; i0 < parts; i0 += U * WPR) {
     float2 ml[U];
     float x[U][PER];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      ml[u] = make_float2(-INFINITY, 0.f);
-      if (i0 + u < parts) {
-        const int64_t at = slot_of(i0 + u) * kRows + r;
+      const int i = i0 + u * WPR;
+      if (i < parts) {
+        const int64_t at = slot_of(i) * kRows + r;
         ml[u] = *reinterpret_cast<const float2 *>(ws.ml + at * 2);
 #pragma unroll
         for (int c = 0; c < PER; ++c) x[u][c] = ws.o[at * DP + lane * PER + c];
@@ -430,11 +438,24 @@ __global__ void __launch_bounds__(128) attn_join_kernel(AttnArgs a, Ws ws, int b
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (i0 + u >= parts) break;
+      if (i0 + u * WPR >= parts) break;
       const float p = weight(ml[u].x, m);
       l += p * ml[u].y;
 #pragma unroll
       for (int c = 0; c < PER; ++c) o[c] += p * x[u][c];
+    }
+  }
+  if (WPR > 1) {
+#pragma unroll
+    for (int c = 0; c < PER; ++c) sums[warp][lane * PER + c] = o[c];
+    if (lane == 0) sums[warp][DP] = l;
+    __syncthreads();
+    if (warp) return;
+#pragma unroll
+    for (int v = 1; v < 4; ++v) {
+      l += sums[v][DP];
+#pragma unroll
+      for (int c = 0; c < PER; ++c) o[c] += sums[v][lane * PER + c];
     }
   }
   const int64_t out = static_cast<int64_t>(row) * a.q_heads + h0 + r;
@@ -494,7 +515,10 @@ int run_shape(const AttnArgs &a, const Ws &ws, int blocks, int share, cudaStream
   const int64_t fewest = ceil_div(most, kMinRange) * segments;  // ranges there can be
   const int st = run<T, DP, R8, kDealWarps, false>(a, ws, blocks, share, fewest < kRanges ? fewest : kRanges, s);
   if (st) return st;
-  return launch_pdl("attention (join)", attn_join_kernel<T, DP>, dim3(static_cast<unsigned>(segments * (kRows / 4))),
+  if (segments <= 148)
+    return launch_pdl("attention (join)", attn_join_kernel<T, DP, 4>, dim3(static_cast<unsigned>(segments * kRows)),
+                      dim3(128), 0, s, a, ws, blocks, share);
+  return launch_pdl("attention (join)", attn_join_kernel<T, DP, 1>, dim3(static_cast<unsigned>(segments * (kRows / 4))),
                     dim3(128), 0, s, a, ws, blocks, share);
 }
 
