@@ -37,10 +37,6 @@
 namespace qs {
 namespace {
 
-#ifndef VPOLY
-#define VPOLY 0
-#endif
-constexpr int kPolyPairs = VPOLY;
 constexpr int kTile = 128;            // query rows of a tile, keys of a tile
 constexpr float kMaxSum = 32768.f;
 constexpr int kHalf = kTile * 128;    // bytes of 128 rows of 64 values
@@ -93,58 +89,21 @@ __device__ __forceinline__ void tmem_st_32(uint32_t addr, const uint32_t *v) {
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-__device__ __forceinline__ float min_nan(float a, float b) {
-  float d;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-
-// 2^t for two t on the multiply-add pipe (16 special-function lanes per SM would
-// bound the kernel if they took every exponential): t is split into the nearest integer,
-// left in the low bits of t + 1.5 * 2^23 and added to the result's exponent, and a rest f
-// in [-1/2, 1/2], whose 2^f is a polynomial of degree 4 fitted to the least relative error
-// (2.7e-6, and 4e-8 on average: a float16 weight's rounding is a hundred times that).
-// t is taken as at least -125 and at most 120; NaN gives a huge number.
-__device__ __forceinline__ float2 exp2_poly(uint64_t t) {
-  float2 x = unpack2(t);
-  x.x = min_nan(max_nan(x.x, -125.f), 120.f);
-  x.y = min_nan(max_nan(x.y, -125.f), 120.f);
-  t = pack2(x.x, x.y);
-  const uint64_t magic = pack2(12582912.f, 12582912.f), minus = pack2(-12582912.f, -12582912.f);
-  const uint64_t r = add2(t, magic);
-  const uint64_t f = fma2(add2(r, minus), pack2(-1.f, -1.f), t);
-  uint64_t p = fma2(pack2(9.570101276e-3f, 9.570101276e-3f), f, pack2(5.591785908e-2f, 5.591785908e-2f));
-  p = fma2(p, f, pack2(2.402474433e-1f, 2.402474433e-1f));
-  p = fma2(p, f, pack2(6.931217909e-1f, 6.931217909e-1f));
-  p = fma2(p, f, pack2(9.999992847e-1f, 9.999992847e-1f));
-  const float2 q = unpack2(p), n = unpack2(r);
-  return make_float2(__uint_as_float(__float_as_uint(q.x) + (__float_as_uint(n.x) << 23)),
-                     __uint_as_float(__float_as_uint(q.y) + (__float_as_uint(n.y) << 23)));
-}
-
 // 64 scores of a row (float32 in raw) to weights 2^(s scale2 + shift), as 16-bit values in
-// raw's first half; returns their sum before that rounding.  POLY of every 16 pairs go
-// through exp2_poly.
-template <typename T, int POLY>
+// raw's first half; returns their sum before that rounding.  The special-function unit
+// takes 8 cycles for a warp's exponential and bounds it: 533 cycles a warp with two warps
+// on a scheduler.  A quarter of them as polynomials on the multiply-add pipe (26 cycles a
+// pair against 16) took as long.
+template <typename T>
 __device__ __forceinline__ float weights(uint32_t *raw, float scale2, float shift) {
   const uint64_t scale_2 = pack2(scale2, scale2), shift_2 = pack2(shift, shift);
   uint64_t sums[2] = {0, 0};
 #pragma unroll
   for (int j = 0; j < 32; ++j) {
     const uint64_t e2 = fma2(pack2(__uint_as_float(raw[2 * j]), __uint_as_float(raw[2 * j + 1])), scale_2, shift_2);
-    float2 e;
-    if (j % 16 * POLY / 16 != (j % 16 + 1) * POLY / 16) {
-      e = exp2_poly(e2);
-    } else {
-      e = unpack2(e2);
-      e.x = ex2(e.x);
-      e.y = ex2(e.y);
-    }
+    float2 e = unpack2(e2);
+    e.x = ex2(e.x);
+    e.y = ex2(e.y);
     sums[j & 1] = add2(sums[j & 1], pack2(e.x, e.y));
     split16<T>(e.x, e.y, raw[j]);
   }
@@ -475,6 +434,8 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
             ++issued;
             if (clear) {
               ok = sm100::mbar_wait_warp(bar, (landed_phase >> s) & 1, w.wait_ns);
+              // given up, but the copies must not outlive the CTA
+              if (!ok && !sm100::mbar_wait_warp(bar, (landed_phase >> s) & 1, kDrainNs)) *w.error = 1;
               landed_phase ^= 1u << s;
               for (int r = lane; r < kTile; r += 32) {
                 const int p = __shfl_sync(0xffffffffu, page, r / w.granule);
@@ -681,11 +642,11 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           // afterwards.  No weight is above the sum's bound, which float16 holds.  The
           // product with the first 64 keys' values starts before the others' weights are
           // made.
-          const float sum = weights<T, kPolyPairs>(raw, scale2, -m * scale2);
+          const float sum = weights<T>(raw, scale2, -m * scale2);
           if (!__any_sync(0xffffffffu, real && !(sum <= kMaxSum && m > -INFINITY))) {
             store(0);
             l += sum;
-            float sum2 = weights<T, kPolyPairs>(raw + 64, scale2, -m * scale2);
+            float sum2 = weights<T>(raw + 64, scale2, -m * scale2);
             if (__any_sync(0xffffffffu, real && !(sum2 <= kMaxSum))) {
               // a new reference in the middle: O takes it once the first half is in
               ok = sm100::mbar_wait_warp(half_done(t), (step + i) & 1, w.wait_ns);
@@ -696,7 +657,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
               sm100::tmem_ld_wait();
               const float top = top_of(raw + 64);
               rescale(top <= m ? m : top);
-              sum2 = weights<T, 0>(raw + 64, scale2, -m * scale2);
+              sum2 = weights<T>(raw + 64, scale2, -m * scale2);
             }
             l += sum2;
             store(1);
@@ -729,9 +690,9 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         if (i == 0) m = top;
         else if (__any_sync(0xffffffffu, renew)) rescale(renew ? top : m);
         const float shift = m == -INFINITY ? 0.f : -m * scale2;
-        l += weights<T, 0>(raw, scale2, shift);
+        l += weights<T>(raw, scale2, shift);
         store(0);
-        l += weights<T, 0>(raw + 64, scale2, shift);
+        l += weights<T>(raw + 64, scale2, shift);
         store(1);
       }
       if (!ok) break;
@@ -897,7 +858,8 @@ int run(const AttnArgs &a, cudaStream_t s) {
   w.splits = splits_for(a.tokens, a.rows, a.q_heads, a.kv_heads, page, a.width, a.window, a.sinks);
   w.part_o = static_cast<float *>(a.ws);
   w.part_ml = reinterpret_cast<float2 *>(w.part_o + w.splits * rows * DP);
-  const dim3 grid(static_cast<unsigned>(ceil_div(a.tokens, per) + a.rows), a.kv_heads, w.splits);
+  const int64_t most_rows = a.rows < a.tokens ? a.rows : a.tokens;  // that have a token
+  const dim3 grid(static_cast<unsigned>(ceil_div(a.tokens, per) + most_rows), a.kv_heads, w.splits);
   const int st = launch_pdl("attention (window)", kern, grid, dim3(C::threads), C::smem, s, qmap, kmap, vmap, w);
   if (st || w.splits == 1) return st;
   return launch_pdl("attention (window, join)", window_join_kernel<T, DP>, dim3(static_cast<unsigned>(ceil_div(rows, 8))),
