@@ -156,11 +156,14 @@ __device__ __forceinline__ int pages_of(int64_t n, int shift, int width) {
 // pages are shared; a part-filled last page stays with the first child, and the
 // other children get a page of their own, whose filled tokens the second launch
 // copies.  Counts change by references after minus references before, so counts
-// that the caller holds besides the table's stay.
+// that the caller holds besides the table's stay.  NEAR (one CTA, counts that fit its
+// shared memory): the counts are changed and searched there, which saves two trips to L2.
+template <bool NEAR>
 __global__ void __launch_bounds__(kThreads, 1) fork_kernel(Tables t, const int *parents, Work w) {
   extern __shared__ int sm[];
   __shared__ int tmp[32];
   int *first = sm, *kids = sm + t.rows, *rank = sm + 2 * t.rows, *par = sm + 3 * t.rows, *len = sm + 4 * t.rows;
+  int *fresh = NEAR ? sm + 5 * t.rows : w.a, *count = NEAR ? sm + 6 * t.rows : t.refcount_out;
   pdl_wait();
   pdl_launch_dependents();
   const int nthreads = kThreads * cluster_size(), tid = cluster_rank() * kThreads + threadIdx.x;
@@ -176,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1) fork_kernel(Tables t, const int *
     if (par[i] < 0 && p != -1 && cluster_rank() == 0) flag_error(kCacheErrParent);
   }
 #pragma unroll 4
-  for (int p = lo + threadIdx.x; p < hi; p += kThreads) t.refcount_out[p] = t.refcount[p];
+  for (int p = lo + threadIdx.x; p < hi; p += kThreads) count[p] = t.refcount[p];
   __syncthreads();
   for (int i = threadIdx.x; i < t.rows; i += kThreads)
     if (par[i] >= 0) {
@@ -211,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 1) fork_kernel(Tables t, const int *
     const int d = c < whole ? kids[i] - 1 : (kids[i] ? 0 : -1);
     const int was = c < old_used && d != 0 ? t.table[e] : -1;
     const int is = c < used ? t.table[static_cast<int64_t>(p) * t.width + c] : -1;
-    if (was >= 0 && was < t.pages) atomicAdd(t.refcount_out + was, d);
+    if (was >= 0 && was < t.pages) atomicAdd(count + was, d);
     if (rank[i] >= 0 && c == used - 1) w.list[rank[i]].x = is;  // a copying row's last entry follows below
     else t.table_out[e] = is;
     if (c == 0) t.lengths_out[i] = n;
@@ -219,23 +222,28 @@ __global__ void __launch_bounds__(kThreads, 1) fork_kernel(Tables t, const int *
   if (t.width == 0)
     for (int i = tid; i < t.rows; i += nthreads) t.lengths_out[i] = par[i] < 0 ? 0 : len[par[i]];
   cluster_barrier();
+  auto count_of = [&](int p) { return NEAR ? count[p] : __ldcg(count + p); };
   if (want == 0) {  // the same in every CTA
+    if (NEAR)
+      for (int p = tid; p < t.pages; p += nthreads) t.refcount_out[p] = count[p];
     if (tid == 0) w.head[0] = 0;
     return;
   }
   const int free_pages = number_pages<false>(
-      t.pages, w.head, tmp, [&](int p) { return __ldcg(t.refcount_out + p) == 0; },
+      t.pages, w.head, tmp, [&](int p) { return count_of(p) == 0; },
       [&](int p, int r, bool is, int) {
-        if (is && r < want) w.a[r] = p;
+        const bool take = is && r < want;
+        if (take) fresh[r] = p;
+        if (NEAR) t.refcount_out[p] = take ? 1 : count[p];
       });
   cluster_barrier();
   for (int i = tid; i < t.rows; i += nthreads) {
     const int r = rank[i];
     if (r < 0) continue;
-    const int n = len[par[i]], page = r < free_pages ? __ldcg(w.a + r) : -1;
+    const int n = len[par[i]], page = r < free_pages ? (NEAR ? fresh[r] : __ldcg(fresh + r)) : -1;
     t.table_out[static_cast<int64_t>(i) * t.width + (n >> t.page_shift)] = page;
-    if (page >= 0) t.refcount_out[page] = 1;
-    else flag_error(kCacheErrPages);
+    if (page < 0) flag_error(kCacheErrPages);
+    else if (!NEAR) t.refcount_out[page] = 1;
     w.list[r].y = page;
     w.list[r].z = n & fill_mask;
   }
@@ -289,14 +297,20 @@ __global__ void __launch_bounds__(kThreads, 1) compact_kernel(Tables t, int *use
 
 // ---- extend ----------------------------------------------------------------------
 // Row i grows by add[i] tokens; its new pages are the lowest free ones, numbered in
-// row and then column order.
+// row and then column order.  NEAR: as for fork.
+template <bool NEAR>
 __global__ void __launch_bounds__(kThreads, 1) extend_kernel(Tables t, const int *add, Work w) {
   extern __shared__ int sm[];
   __shared__ int tmp[32];
   int *start = sm, *had_s = sm + t.rows, *len_s = sm + 2 * t.rows;
+  int *fresh = NEAR ? sm + 3 * t.rows : w.a, *count = NEAR ? fresh + t.pages : w.b;
   pdl_wait();
   pdl_launch_dependents();
   const int nthreads = kThreads * cluster_size(), tid = cluster_rank() * kThreads + threadIdx.x;
+  if (NEAR) {
+#pragma unroll 4
+    for (int p = threadIdx.x; p < t.pages; p += kThreads) count[p] = t.refcount[p];
+  }
   int want = 0;
   for (int i0 = 0; i0 < t.rows; i0 += kThreads) {
     const int i = i0 + threadIdx.x;
@@ -318,18 +332,19 @@ __global__ void __launch_bounds__(kThreads, 1) extend_kernel(Tables t, const int
     if (i < t.rows) start[i] = before;
     want += n;
   }
-  const int free_pages = number_pages<false>(
-      t.pages, w.head, tmp, [&](int p) { return t.refcount[p] == 0; },
+  const int free_pages = number_pages<false>(  // NEAR: a thread's own entries of count
+      t.pages, w.head, tmp, [&](int p) { return (NEAR ? count[p] : t.refcount[p]) == 0; },
       [&](int p, int r, bool is, int) {
         const bool take = is && r < want;
-        if (take) w.a[r] = p;
-        w.b[p] = take ? 1 : t.refcount[p];
+        const int had = NEAR ? count[p] : t.refcount[p];
+        if (take) fresh[r] = p;
+        count[p] = take ? 1 : had;
       });
   if (tid == 0 && want > free_pages) flag_error(kCacheErrPages);
   cluster_barrier();
   // the outputs may be the inputs: every input value was read before the last barrier,
   // except the table entries that stay where they are
-  for (int p = tid; p < t.pages; p += nthreads) t.refcount_out[p] = __ldcg(w.b + p);
+  for (int p = tid; p < t.pages; p += nthreads) t.refcount_out[p] = NEAR ? count[p] : __ldcg(count + p);
   const int64_t entries = static_cast<int64_t>(t.rows) * t.width;
 #pragma unroll 4
   for (int64_t e = tid; e < entries; e += nthreads) {
@@ -338,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 1) extend_kernel(Tables t, const int
     const int had = had_s[i], has = pages_of(len_s[i], t.page_shift, t.width), r = start[i] + c - had;
     int p = -1;
     if (c < had) p = t.table[e];
-    else if (c < has && r < free_pages) p = __ldcg(w.a + r);
+    else if (c < has && r < free_pages) p = NEAR ? fresh[r] : __ldcg(fresh + r);
     t.table_out[e] = p;
   }
   for (int i = tid; i < t.rows; i += nthreads) t.lengths_out[i] = len_s[i];
@@ -459,6 +474,8 @@ __global__ void __launch_bounds__(256) write_kernel(WriteArgs a) {
   }
 }
 
+constexpr size_t kNearBytes = 160 * 1024;
+
 // One CTA while a scan of the counts and the tables is short; a cluster of eight
 // shares longer ones.
 int cluster_for(int64_t rows, int64_t width, int64_t pages) { return rows * width + pages <= 32768 ? 1 : 8; }
@@ -530,8 +547,11 @@ int launch_cache_fork(const qs_kv_pool &pool, int rows, int width, const int *ta
   const Tables t{rows, width, static_cast<int>(pool.pages), log2_of(pool.page), table, lengths, refcount,
                  table_out, lengths_out, refcount_out};
   const Work w = split_work(ws, rows, pool.pages);
-  const int st = launch_cluster("cache fork", fork_kernel, cluster_for(rows, width, pool.pages),
-                                static_cast<size_t>(rows) * 20, s, t, parents, w);
+  const int ctas = cluster_for(rows, width, pool.pages);
+  const size_t near = static_cast<size_t>(rows) * 24 + pool.pages * 4;
+  const int st = ctas == 1 && near <= kNearBytes
+                     ? launch_cluster("cache fork", fork_kernel<true>, ctas, near, s, t, parents, w)
+                     : launch_cluster("cache fork", fork_kernel<false>, ctas, static_cast<size_t>(rows) * 20, s, t, parents, w);
   return st ? st : launch_copy(pool, w, s);
 }
 
@@ -551,8 +571,11 @@ int launch_cache_extend(int64_t page, int64_t pages, int rows, int width, const 
                         void *ws, cudaStream_t s) {
   const Tables t{rows, width, static_cast<int>(pages), log2_of(page), table, lengths, refcount,
                  table_out, lengths_out, refcount_out};
-  return launch_cluster("cache extend", extend_kernel, cluster_for(rows, width, pages), static_cast<size_t>(rows) * 12,
-                        s, t, add, split_work(ws, rows, pages));
+  const Work w = split_work(ws, rows, pages);
+  const int ctas = cluster_for(rows, width, pages);
+  const size_t near = static_cast<size_t>(rows) * 12 + pages * 8;
+  if (ctas == 1 && near <= kNearBytes) return launch_cluster("cache extend", extend_kernel<true>, ctas, near, s, t, add, w);
+  return launch_cluster("cache extend", extend_kernel<false>, ctas, static_cast<size_t>(rows) * 12, s, t, add, w);
 }
 
 int launch_cache_write(const qs_kv_pool &pool, int rows, int width, const int *table, const int *lengths,

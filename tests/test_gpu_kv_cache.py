@@ -80,6 +80,7 @@ def same(got, want, what):
     (24, 8, 32, 300, 500, 3, 80, 3, torch.bfloat16),
     (600, 5, 16, 6000, 150, 1, 16, 1, torch.float16),      # more rows than threads of a block
     (40, 4, 16, 40000, 900, 1, 8, 1, torch.float16),       # more pages than one block scans: the cluster
+    (8192, 2, 16, 16000, 15, 1, 8, 1, torch.bfloat16),     # one block whose counts do not fit shared memory
 ])
 @pytest.mark.parametrize("kind", ["random", "identity", "all_of_one", "free_all"])
 def test_fork(rows, share, page, pages, max_len, heads, dim, layers, dtype, kind):
@@ -169,7 +170,8 @@ def test_compact_of_an_empty_and_of_a_full_pool():
 
 
 @pytest.mark.parametrize("rows,page,pages,max_len,max_new,heads,dim", [
-    (16, 16, 1400, 700, 512, 8, 128), (1, 256, 2, 0, 300, 1, 8), (700, 16, 40000, 60, 1, 2, 72), (3, 64, 50, 200, 0, 1, 64)])
+    (16, 16, 1400, 700, 512, 8, 128), (1, 256, 2, 0, 300, 1, 8), (700, 16, 40000, 60, 1, 2, 72), (3, 64, 50, 200, 0, 1, 64),
+    (9, 16, 25000, 300, 70, 1, 16)])
 def test_extend_and_write(rows, page, pages, max_len, max_new, heads, dim):
     rs = np.random.RandomState(rows)
     width = -(-(max_len + max_new) // page) + 1
