@@ -248,11 +248,12 @@ __device__ __forceinline__ Job job_of(const WindowArgs &w, int x, int y, int z, 
   j.split = z;
   j.first = 0;
   j.q0 = j.q1 = j.t0 = 0;
-  int end = 0, want = x;
+  int end = 0, want = x, length = 0;
   for (int r0 = 0; r0 < a.rows && j.row < 0; r0 += 32) {
     const int r = r0 + lane;
-    int q0 = 0, q1 = 0, n = 0;
+    int q0 = 0, q1 = 0, n = 0, len = 0;
     if (r < a.rows) {
+      len = a.lengths[r];
       q0 = clampi(a.cu[r], 0, total_tokens);
       q1 = clampi(a.cu[r + 1], q0, total_tokens);
       n = (q1 - q0 + per - 1) / per;
@@ -270,6 +271,7 @@ __device__ __forceinline__ Job job_of(const WindowArgs &w, int x, int y, int z, 
       j.row = r0 + src;
       j.q0 = __shfl_sync(0xffffffffu, q0, src);
       j.q1 = __shfl_sync(0xffffffffu, q1, src);
+      length = max(0, __shfl_sync(0xffffffffu, len, src));
       const int local = __shfl_sync(0xffffffffu, want - (sum - n), src), all = __shfl_sync(0xffffffffu, n, src);
       j.t0 = j.q0 + (all - 1 - local) * per;
     } else {
@@ -277,7 +279,6 @@ __device__ __forceinline__ Job job_of(const WindowArgs &w, int x, int y, int z, 
     }
   }
   if (j.row >= 0) {
-    const int length = max(0, a.lengths[j.row]);
     const int cap = static_cast<int>(min(static_cast<int64_t>(a.width) << a.page_shift, static_cast<int64_t>(0x7ffffff0)));
     const int back = length - (j.q1 - j.q0);
     j.pos0 = back + (j.t0 - j.q0);
@@ -382,10 +383,15 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           jobs[slot] = j;
           jobs[slot].absent = 0;
           sm100::mbar_arrive(job_full(slot));
-          ask_next_block(answer, asked);
         }
-        ++asks;
         __syncwarp();
+        // The next block is asked for with the last tile's loads: early enough for its own
+        // loads to follow, and no earlier, or this CTA keeps it from one that is idle.
+        auto ask = [&] {
+          if (lane == 0) ask_next_block(answer, asked);
+          ++asks;
+          __syncwarp();
+        };
         const int n = j.tiles;
         if (n > 0) {
           if (q_loads > 0) ok = sm100::mbar_wait_warp(q_empty, (q_loads - 1) & 1, w.wait_ns);
@@ -407,7 +413,9 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           return p >= 0 && p < a.pages ? p : -1;
         };
         int next_page = page_at(0);
+        if (n == 0) ask();
         for (int i = 0; i < n && ok; ++i) {
+          if (i + 1 == n) ask();
           const int page = next_page;
           next_page = page_at(i + 1);
           const int k0 = key_of_tile(j, i), k = k0 + lane * w.granule;
@@ -810,16 +818,22 @@ __global__ void __launch_bounds__(256) window_join_kernel(WindowArgs w) {
   if (lane == 0 && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
+// Query tiles of a block: one where the rows' tokens fill no more than one on average (a
+// second would mostly be empty: 16 rows of 8 tokens over 16000 keys), else two.
+int query_tiles(int64_t tokens, int64_t rows, int64_t share) { return tokens <= rows * (kTile / share) ? 1 : 2; }
+
 // Shares of a tile's keys: as many as there are SMs for, of at least two key tiles each.
 int splits_for(int64_t tokens, int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t page, int64_t width,
                int64_t window, int64_t sinks) {
   const int64_t share = q_heads / kv_heads;
-  if (share > kTile) return 1;
-  const int64_t per = 2 * (kTile / share), blocks = (ceil_div(tokens, per) + (rows < tokens ? rows : tokens)) * kv_heads;
+  if (share > kTile || tokens < 1 || rows < 1) return 1;
+  const int64_t per = query_tiles(tokens, rows, share) * (kTile / share);
+  int64_t blocks = ceil_div(tokens, per);  // there are at least so many, or as many as rows with tokens
+  if (blocks < (rows < tokens ? rows : tokens)) blocks = rows < tokens ? rows : tokens;
   int64_t keys = width * page;
   if (window > 0 && window < keys && sinks < keys && window + sinks + per < keys) keys = window + sinks + per;
   int64_t n = ceil_div(ceil_div(keys, kTile), 2);
-  if (n > 148 / (blocks > 0 ? blocks : 1)) n = 148 / (blocks > 0 ? blocks : 1);
+  if (n > 148 / (blocks * kv_heads)) n = 148 / (blocks * kv_heads);
   return static_cast<int>(n < 1 ? 1 : n);
 }
 
@@ -874,9 +888,15 @@ int64_t attn_window_workspace_bytes(int64_t tokens, int64_t rows, int64_t q_head
   return splits == 1 ? 0 : splits * tokens * q_heads * ((dim <= 64 ? 64 : 128) + 2) * 4;
 }
 
+template <typename T>
+int run_type(const AttnArgs &a, cudaStream_t s) {
+  const bool one = query_tiles(a.tokens, a.rows, a.q_heads / a.kv_heads) == 1;
+  if (a.dim <= 64) return one ? run<T, 64, 1>(a, s) : run<T, 64, 2>(a, s);
+  return one ? run<T, 128, 1>(a, s) : run<T, 128, 2>(a, s);
+}
+
 int launch_attn_window(const AttnArgs &a, cudaStream_t s) {
-  if (a.dim <= 64) return a.dtype == QS_F16 ? run<__half, 64, 2>(a, s) : run<__nv_bfloat16, 64, 2>(a, s);
-  return a.dtype == QS_F16 ? run<__half, 128, 2>(a, s) : run<__nv_bfloat16, 128, 2>(a, s);
+  return a.dtype == QS_F16 ? run_type<__half>(a, s) : run_type<__nv_bfloat16>(a, s);
 }
 
 }  // namespace qs
