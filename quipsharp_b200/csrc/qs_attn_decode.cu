@@ -27,6 +27,7 @@ namespace {
 constexpr int kRangesPerCta = 4;  // 64 rows of up to 16000 tokens: 337, 327, 321, 319, 322 us with 1, 2, 3, 4, 6
 constexpr int kStages = 3;
 constexpr int kKeys = 16;         // keys of a group
+constexpr float kBias = 12.f;     // no weight is above 2^12
 constexpr int kRows = 16;         // query heads of a block
 constexpr int kCtasPerSm = 2;     // of four warps
 constexpr int kDealWarps = 4;     // warps of a CTA that is dealt ranges
@@ -147,13 +148,14 @@ struct Warp {
     }
     // The weights enter the second product as the sum of two 16-bit values (what the
     // first leaves of 24 bits, the second takes), so they lose nothing that the output's
-    // rounding would show; the extra products are hidden behind the loads.
+    // rounding would show; the extra products are hidden behind the loads.  They are
+    // 2^kBias times what the softmax has, which keeps small ones in float16's range.
     uint32_t ph[4] = {}, pl[4] = {};
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int h = 0; h < (R8 ? 1 : 2); ++h) {
-        const float base = m[h] == -INFINITY ? 0.f : m[h];
+        const float base = m[h] == -INFINITY ? 0.f : m[h] - kBias;
         const float x = ex2(s[j][2 * h] - base), y = ex2(s[j][2 * h + 1] - base);
         l[h] += x + y;
         const float2 back = split16<T>(x, y, ph[2 * j + h]);
@@ -297,7 +299,7 @@ attn_decode_kernel(AttnArgs a, Ws ws, int blocks, int share) {
         uint32_t packed;
         split16<T>(o.x * inv, o.y * inv, packed);
         if (c2 < a.dim) *reinterpret_cast<uint32_t *>(static_cast<T *>(a.out) + out * a.dim + c2) = packed;
-        if (c2 == 0 && a.lse) a.lse[out] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+        if (c2 == 0 && a.lse) a.lse[out] = l == 0.f ? -INFINITY : (m - kBias + log2f(l)) * kLn2;
       } else {
         *reinterpret_cast<float2 *>(ws.o + (slot * kRows + r) * DP + c2) = o;
         if (c2 == 0) ws.ml[(slot * kRows + r) * 2] = m, ws.ml[(slot * kRows + r) * 2 + 1] = l;
@@ -467,7 +469,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(AttnArgs a, Ws ws, int b
     if (lane * PER + c < a.dim)
       *reinterpret_cast<uint32_t *>(static_cast<T *>(a.out) + out * a.dim + lane * PER + c) = packed;
   }
-  if (lane == 0 && a.lse) a.lse[out] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+  if (lane == 0 && a.lse) a.lse[out] = l == 0.f ? -INFINITY : (m - kBias + log2f(l)) * kLn2;
 }
 
 struct Shape {

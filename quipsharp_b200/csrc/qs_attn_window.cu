@@ -11,15 +11,16 @@
 // P V on the tensor core with P read from TMEM.  With two query tiles the tensor core
 // works on one while the other's softmax runs.
 //
-// The maximum that the weights refer to is renewed, and O rescaled, only when it has
-// grown by more than 2^8: until then weights up to 2^8 are exact in the float32 sum
-// and lose nothing in the 16-bit ones, and most tiles rescale nothing.
+// The weights are 2^(s - reference), the reference kBias below a maximum of the scores so
+// far.  Most tiles keep it: whether it still will do shows in the weights' sum, and only
+// then is a maximum taken and O rescaled.  Float16 weights have to stay below 65504, and
+// the bias keeps those down to 2^-20 of the largest in float16's normal range (a first
+// token that takes nearly all the weight and has next to no value is common).
 //
 // One CTA per SM stays and takes one group of tiles after another: the grid has a block
 // for each, and a running CTA cancels the next one that has not started and does its work
 // (so the longest are begun first and none waits for a fixed share).  The loads of a
-// group begin while the one before is still being summed; with a CTA per group instead,
-// 14 to 17 us of each went into starting, the first loads and the last stores.
+// group begin while the one before is still being summed.
 //
 // Where the tiles are fewer than the SMs (few tokens over many keys), each is split along
 // the keys: a block takes a share of its key tiles and leaves its sum, maximum and output
@@ -38,7 +39,12 @@ namespace qs {
 namespace {
 
 constexpr int kTile = 128;            // query rows of a tile, keys of a tile
-constexpr float kMaxSum = 32768.f;
+constexpr float kBias = 6.f;
+// Of 64 weights with the reference kept.  None of them may overflow float16; a first tile
+// with few keys seen leaves a low reference, from which this has room for 2^3 with scores
+// of ordinary spread (bias 8: 2^1, and chunks under a window took 93 us for 84).
+template <typename T>
+constexpr float kMaxSum = std::is_same<T, __half>::value ? 60000.f : 1e30f;
 constexpr int kHalf = kTile * 128;    // bytes of 128 rows of 64 values
 constexpr uint64_t kDrainNs = kDefaultWaitNs;
 
@@ -203,8 +209,8 @@ __device__ __forceinline__ int clampi(int v, int lo, int hi) { return min(max(v,
 
 // True in one thread of a warp that is here as a whole.  The compiler knows that it is
 // one: what the product instructions take from uniform registers stays there, where a
-// test of the lane number has every operand moved by way of a loop (155 cycles for each
-// product of 64, measured).
+// test of the lane number has every operand moved there first (chunks under a window took
+// 122 us that way, 98 this way).
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
@@ -650,12 +656,13 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           // afterwards.  No weight is above the sum's bound, which float16 holds.  The
           // product with the first 64 keys' values starts before the others' weights are
           // made.
-          const float sum = weights<T>(raw, scale2, -m * scale2);
-          if (!__any_sync(0xffffffffu, real && !(sum <= kMaxSum && m > -INFINITY))) {
+          const float shift = kBias - m * scale2;
+          const float sum = weights<T>(raw, scale2, shift);
+          if (!__any_sync(0xffffffffu, real && !(sum <= kMaxSum<T> && m > -INFINITY))) {
             store(0);
             l += sum;
-            float sum2 = weights<T>(raw + 64, scale2, -m * scale2);
-            if (__any_sync(0xffffffffu, real && !(sum2 <= kMaxSum))) {
+            float sum2 = weights<T>(raw + 64, scale2, shift);
+            if (__any_sync(0xffffffffu, real && !(sum2 <= kMaxSum<T>))) {
               // a new reference in the middle: O takes it once the first half is in
               ok = sm100::mbar_wait_warp(half_done(t), (step + i) & 1, w.wait_ns);
               if (!ok) break;
@@ -665,7 +672,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
               sm100::tmem_ld_wait();
               const float top = top_of(raw + 64);
               rescale(top <= m ? m : top);
-              sum2 = weights<T>(raw + 64, scale2, -m * scale2);
+              sum2 = weights<T>(raw + 64, scale2, kBias - m * scale2);
             }
             l += sum2;
             store(1);
@@ -694,10 +701,10 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           }
         }
         const float top = max3(top_of(raw), top_of(raw + 64), -INFINITY);
-        const bool renew = m == -INFINITY ? top != -INFINITY : !((top - m) * scale2 <= 8.f);  // NaN stays
+        const bool renew = m == -INFINITY ? top != -INFINITY : !((top - m) * scale2 <= 7.f);  // NaN stays; 2^(7 + kBias) fits float16
         if (i == 0) m = top;
         else if (__any_sync(0xffffffffu, renew)) rescale(renew ? top : m);
-        const float shift = m == -INFINITY ? 0.f : -m * scale2;
+        const float shift = m == -INFINITY ? 0.f : kBias - m * scale2;
         l += weights<T>(raw, scale2, shift);
         store(0);
         l += weights<T>(raw + 64, scale2, shift);
@@ -747,7 +754,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           sm100::tmem_ld_wait();
           send(o, reinterpret_cast<char *>(w.part_o + base * DP + c), DP * 4, 128);
         }
-        if (real) w.part_ml[base + at] = make_float2(m == -INFINITY ? -INFINITY : m * scale2, l);
+        if (real) w.part_ml[base + at] = make_float2(m == -INFINITY ? -INFINITY : m * scale2 - kBias, l);
         sm100::tc_fence_before_sync();
         continue;
       }
@@ -763,7 +770,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         send(o, reinterpret_cast<char *>(static_cast<T *>(a.out) + c), a.dim * 2, (a.dim - c) * 2);
       }
       sm100::tc_fence_before_sync();  // O is read: the next job's first weights release it
-      if (real && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m * scale2 * kLn2) + logf(l);
+      if (real && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : (m * scale2 - kBias) * kLn2) + logf(l);
     }
     if (!ok) *w.error = 1;
   }

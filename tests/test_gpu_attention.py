@@ -200,6 +200,30 @@ def test_scale_and_large_scores():
         check(at.window_attention(q, k, v, table, n, cu, scale=scale, return_lse=True), want, torch.float16, True)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_a_first_token_that_takes_the_weight_and_has_no_value(dtype):
+    """The others' weights, 2^-20 of the first one's, decide the output: none may fall out of
+    float16's normal range, so the roundings are those of the other tests without an
+    absolute part."""
+    rs = np.random.RandomState(10)
+    n = 600
+    k, v, table, lengths = make(rs, [n], 1, 16, 64, dtype)
+    q = torch.randn(3, 4, 64, device=DEV).to(dtype)
+    q[:, :, 0] = 4.0
+    k[:, :, :, 0] = 0
+    v *= 200
+    first = int(table[0, 0])
+    k[first, 0, 0], v[first, 0, 0] = 0, 0
+    k[first, 0, 0, 0] = 28.0  # a score of 4 * 28 / 8 = 14 above the others' mean
+    cu = torch.tensor([0, 3], dtype=torch.int32, device=DEV)
+    for got, new, u in ((at.window_attention(q, k, v, table, lengths, cu), 3, 2 * U[dtype]),
+                        (at.decode_attention(q[2:], k, v, table, lengths), 1, U[dtype])):
+        o, _, a = exact(q[3 - new:], k, v, table, lengths, [new], 0, 0)
+        assert float(a.max()) < 1.0
+        err = (got.double() - o).abs()
+        assert bool((err <= u * (o.abs() + a) + 1e-4 * a + 2.0 ** -25).all()), float((err / a).max())
+
+
 def test_pools_past_32_bit_offsets():
     """A pool of more than 2^32 bytes, with the row's pages at its end."""
     pages = (1 << 31) // (2 * 64 * 64) + 40
