@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import importlib.util
 import os
 import struct
 import threading
@@ -152,6 +153,26 @@ def lib():
                     fn.argtypes = args
                 _lib = h
     return _lib
+
+
+_fast = None
+
+
+def fast():
+    """The extension module with the decoding operators' direct calls (csrc/qs_fast.cpp)."""
+    global _fast
+    if _fast is None:
+        lib()
+        path = os.path.join(os.path.dirname(_LIB_PATH), "_fast.so")
+        try:
+            spec = importlib.util.spec_from_file_location("_fast", path)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+        except ImportError as e:
+            raise NativeLibraryMissing(f"{path} is missing or was built for another torch ({e}); "
+                                       "run `python -m quipsharp_b200.build_native -f`") from e
+        _fast = module
+    return _fast
 
 
 def library_path() -> str:

@@ -57,6 +57,9 @@ def decode_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor,
     cache.  Rows of length 0 give 0.  Returns (rows, q_heads, dim), with
     return_lse also log sum exp of the scaled scores, float32 (rows, q_heads)
     (-inf where a row sees nothing).  Keys that are not seen are not read."""
+    got = N.fast().attend(q, k_pages, v_pages, table, lengths, None, window, sinks, scale, return_lse)
+    if got is not None:
+        return got
     dev = _device_of(q, k_pages, v_pages, table, lengths)
     if not N.is_current(dev):
         with torch.cuda.device(dev):
@@ -92,6 +95,9 @@ def window_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor,
     Up to 128 query heads share a key head.  Values that are infinite or NaN are
     only kept from tokens that do not see them where no token of the same tile
     does (places past a row's length never enter)."""
+    got = N.fast().attend(q, k_pages, v_pages, table, lengths, cu, window, sinks, scale, return_lse)
+    if got is not None:
+        return got
     dev = _device_of(q, k_pages, v_pages, table, lengths, cu)
     if not N.is_current(dev):
         with torch.cuda.device(dev):

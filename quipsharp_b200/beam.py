@@ -25,6 +25,9 @@ def beam_select(logits: Tensor, scores: Tensor, n: int | None = None, finished: 
     beams) bool: an ended beam has one continuation, `pad`, with its score as it
     is.  Returns (scores float32, parents int32, tokens int32), each (batch, n);
     parents are beam numbers within the search."""
+    got = N.fast().beam_select(logits, scores, n, finished, pad)
+    if got is not None:
+        return got
     N.refuse_grad("beam_select", logits, scores)
     dev = _device_of(logits, scores, finished)
     if not N.is_current(dev):

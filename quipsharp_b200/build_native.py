@@ -2,7 +2,8 @@
 
     python -m quipsharp_b200.build_native [-v]
 
-Writes quipsharp_b200/_lib/libquipsharp_b200.so.  The codebook tables and the
+Writes quipsharp_b200/_lib/libquipsharp_b200.so and the Python extension
+quipsharp_b200/_lib/_fast.so (host code only).  The codebook tables and the
 odd-prime DFT constants are generated into quipsharp_b200/_build/qs_tables_gen.inc
 from quipsharp_b200/codebooks/tables.py before compiling, so the device code
 carries exactly the tables the Python codebook objects expose.
@@ -161,7 +162,35 @@ def build(verbose: bool = False, force: bool = False) -> str:
         if res.returncode != 0:
             sys.stderr.write(res.stdout + res.stderr)
             raise RuntimeError("link failed")
+    build_fast(verbose, force)
     return lib
+
+
+def build_fast(verbose: bool, force: bool) -> str:
+    """The Python extension with the decoding operators' direct calls, linked to the library."""
+    import sysconfig
+
+    import torch
+    src, out = os.path.join(CSRC, "qs_fast.cpp"), os.path.join(LIBDIR, "_fast.so")
+    newest = max(os.path.getmtime(src), os.path.getmtime(os.path.join(REPO, "include", "quipsharp_b200.h")))
+    if not force and os.path.exists(out) and os.path.getmtime(out) >= newest:
+        return out
+    inc = os.path.join(os.path.dirname(torch.__file__), "include")
+    cuda = os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")
+    cmd = [os.environ.get("CXX") or shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC",
+           "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", sysconfig.get_paths()["include"], "-I", inc,
+           "-I", os.path.join(inc, "torch", "csrc", "api", "include"), "-I", cuda,
+           src, "-o", out, "-L", LIBDIR, f"-l:{LIBNAME}", "-Wl,-rpath,$ORIGIN",
+           # torch's own libraries are loaded by the time this is
+           "-L", os.path.join(os.path.dirname(inc), "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError(f"g++ failed on {src}")
+    return out
 
 
 if __name__ == "__main__":

@@ -98,6 +98,9 @@ def fork_pages(k: Tensor, v: Tensor, table: Tensor, lengths: Tensor, refcount: T
     of all layers copied.  Returns the new (table, lengths, refcount); the pools
     k, v (layers, pages, heads, page, dim) are changed in place.  refcount may
     hold references of the caller's besides the table's: they stay."""
+    got = N.fast().fork_pages(k, v, table, lengths, refcount, parents)
+    if got is not None:
+        return got
     dev = _device_of(k, v, table, lengths, refcount, parents)
     if not N.is_current(dev):
         with torch.cuda.device(dev):
@@ -118,6 +121,9 @@ def compact_pages(k: Tensor, v: Tensor, table: Tensor, lengths: Tensor,
     from U on go to the holes below U, both in ascending order.  Returns the new
     (table, refcount, U as an int32 tensor of one); the pools are changed in
     place, and pages from U on are free."""
+    got = N.fast().compact_pages(k, v, table, lengths, refcount)
+    if got is not None:
+        return got
     dev = _device_of(k, v, table, lengths, refcount)
     if not N.is_current(dev):
         with torch.cuda.device(dev):
@@ -136,6 +142,9 @@ def extend_pages(table: Tensor, lengths: Tensor, refcount: Tensor, new_tokens: T
     lowest free ones, in row and then column order.  Returns the new (table,
     lengths, refcount).  A row that finds no page, or outgrows its line, has -1
     there: its tokens are left out, and `check_device` raises."""
+    got = N.fast().extend_pages(table, lengths, refcount, new_tokens, page_size)
+    if got is not None:
+        return got
     dev = _device_of(table, lengths, refcount, new_tokens)
     if not N.is_current(dev):
         with torch.cuda.device(dev):
@@ -167,6 +176,8 @@ def write_kv(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tens
     cu[r+1]) and take its last places, which `lengths` already counts; without
     cu every row has one.  k and v may be views (the last dimension
     contiguous)."""
+    if N.fast().write_kv(k, v, k_pages, v_pages, table, lengths, cu):
+        return
     N.refuse_grad("write_kv", k, v)
     dev = _device_of(k, v, k_pages, v_pages, table, lengths, cu)
     if not N.is_current(dev):

@@ -327,3 +327,37 @@ def test_empty_calls():
     empty = torch.zeros(2, 0, dtype=torch.int32, device=DEV)  # lines without a page
     out = at.decode_attention(torch.ones(2, 4, 64, device=DEV).half(), k, k, empty, n)
     assert not out.any()
+
+
+def test_arguments_that_need_a_copy_or_a_refusal():
+    """What the direct call does not take goes the longer way and gives the same, or its error."""
+    rs = np.random.RandomState(11)
+    k, v, table, n = make(rs, [77, 300, 16], 4, 32, 64, torch.float16)
+    q = torch.randn(3, 8, 64, device=DEV).half()
+    cu = torch.arange(4, device=DEV, dtype=torch.int32)
+    decode = at.decode_attention(q, k, v, table, n)
+    window = at.window_attention(q, k, v, table, n, cu)
+    wide = torch.stack((table, table), -1)[..., 0]
+    twice = torch.stack((n, n), -1)[:, 0]
+    unaligned = torch.empty(3 * 8 * 64 + 1, device=DEV, dtype=torch.float16)[1:].view(3, 8, 64).copy_(q)
+    assert not wide.is_contiguous() and not twice.is_contiguous() and unaligned.data_ptr() % 16
+    for args in ((q, k, v, wide, n), (q, k, v, table, twice), (unaligned, k, v, table, n)):
+        assert torch.equal(at.decode_attention(*args), decode)
+        assert torch.equal(at.window_attention(*args, cu), window)
+    assert torch.equal(at.decode_attention(q, k, v, table, n, window=np.int64(1000), scale=np.float64(0.125)), decode)
+    grad = q.clone().requires_grad_()
+    for error, call in (
+            (TypeError, lambda: at.decode_attention(q.bfloat16(), k, v, table, n)),
+            (TypeError, lambda: at.decode_attention(q, k, v, table.long(), n)),
+            (TypeError, lambda: at.window_attention(q, k, v, table, n, cu.long())),
+            (ValueError, lambda: at.decode_attention(q[:2], k, v, table, n)),
+            (ValueError, lambda: at.decode_attention(q, k, v, table, n, window=0)),
+            (ValueError, lambda: at.window_attention(q, k, v, table, n, cu[:3])),
+            (RuntimeError, lambda: at.decode_attention(grad, k, v, table, n)),
+            (RuntimeError, lambda: at.decode_attention(q, k, v, table.cpu(), n)),
+            (RuntimeError, lambda: at.decode_attention(q, k, v, table, n, scale=-1.0)),
+            (NotImplementedError, lambda: at.decode_attention(q, k[:, :, :24], v[:, :, :24], table, n))):
+        with pytest.raises(error):
+            call()
+    with torch.no_grad():
+        assert torch.equal(at.decode_attention(grad, k, v, table, n), decode)

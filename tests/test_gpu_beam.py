@@ -145,3 +145,16 @@ def test_empty_batch_and_other_stream():
     side.synchronize()
     for a, b in zip(got, beam_select(x, s, 4)):
         assert torch.equal(a, b)
+
+
+def test_refusals():
+    x, s = torch.zeros(2, 3, 50, device=DEV), torch.zeros(2, 3, device=DEV)
+    for error, call in (
+            (ValueError, lambda: beam_select(x, s, 51)), (ValueError, lambda: beam_select(x, s, 0)),
+            (ValueError, lambda: beam_select(x[0], s)), (ValueError, lambda: beam_select(x, s[:1])),
+            (TypeError, lambda: beam_select(x.double(), s)), (TypeError, lambda: beam_select(x, s.half())),
+            (TypeError, lambda: beam_select(x, s, finished=s)), (RuntimeError, lambda: beam_select(x, s.cpu())),
+            (NotImplementedError, lambda: beam_select(torch.zeros(1, 65, 50, device=DEV), torch.zeros(1, 65, device=DEV), 4)),
+            (RuntimeError, lambda: beam_select(x.clone().requires_grad_(), s))):
+        with pytest.raises(error):
+            call()

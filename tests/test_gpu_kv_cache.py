@@ -245,3 +245,31 @@ def test_cache_object_steps_in_a_graph():
     assert torch.equal(got, new[3])
     cache.free([0, 1, 2, 3])
     assert int(cache.refcount.sum()) == 0 and cache.lengths.tolist() == [0] * 4
+
+
+def test_arguments_that_need_a_copy_or_a_refusal():
+    rs = np.random.RandomState(3)
+    page, pages = 16, 40
+    state = make_state(rs, 4, page, pages, 6, 80)
+    table, lengths, refcount = on(*state)
+    parents = torch.tensor([1, 1, 3, -1], dtype=torch.int32, device=DEV)
+    k, v = (x.to(DEV) for x in pools(rs, 2, pages, 2, page, 24, torch.float16))
+    want = kc.fork_pages(k, v, table, lengths, refcount, parents)
+    spread = torch.stack((parents, parents), -1)[:, 0]
+    for a, b in zip(kc.fork_pages(k, v, table, lengths, refcount, spread), want):
+        assert torch.equal(a, b)
+    new = torch.tensor([3, 0, 20, 1], dtype=torch.int32, device=DEV)
+    want = kc.extend_pages(table, lengths, refcount, new, page)
+    for a, b in zip(kc.extend_pages(table, lengths, refcount, new, np.int64(page)), want):
+        assert torch.equal(a, b)
+    for error, call in (
+            (TypeError, lambda: kc.fork_pages(k, v, table, lengths, refcount, parents.long())),
+            (TypeError, lambda: kc.fork_pages(k.float(), v.float(), table, lengths, refcount, parents)),
+            (ValueError, lambda: kc.fork_pages(k, v[:, :9], table, lengths, refcount, parents)),
+            (ValueError, lambda: kc.fork_pages(k, v, table, lengths, refcount[:9], parents)),
+            (ValueError, lambda: kc.compact_pages(k, v, table, lengths[:3], refcount)),
+            (NotImplementedError, lambda: kc.extend_pages(table, lengths, refcount, new, 24)),
+            (ValueError, lambda: kc.write_kv(k[0, 0], v[0, 0], k[0], v[0], table, lengths)),
+            (RuntimeError, lambda: kc.fork_pages(k, v, table, lengths, refcount, parents.cpu()))):
+        with pytest.raises(error):
+            call()
