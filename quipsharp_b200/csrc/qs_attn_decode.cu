@@ -124,7 +124,8 @@ struct Warp {
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int i = 0; i < (R8 ? 2 : 4); ++i) {
-        s[j][i] = (mask >> (8 * j + 2 * t + (i & 1))) & 1 ? s[j][i] * scale2 : -INFINITY;
+        s[j][i] *= scale2;
+        if (mask != 0xffffu && !((mask >> (8 * j + 2 * t + (i & 1))) & 1)) s[j][i] = -INFINITY;
         top_s[i >> 1] = fmaxf(top_s[i >> 1], s[j][i]);
       }
     bool grew = false;
@@ -212,12 +213,19 @@ attn_decode_kernel(AttnArgs a, Ws ws, int blocks, int share) {
     auto mask_of = [&](int g, int page) {  // bits of the group's keys that are seen
       if (page < 0 || page >= a.pages) return 0u;
       const int k0 = g * kKeys;
+      if (k0 >= seen.lo && k0 + kKeys <= seen.n) return 0xffffu;  // most groups
       const uint32_t below = seen.n - k0 >= kKeys ? 0xffffu : (1u << (seen.n - k0)) - 1u;
       const int lo_k = seen.lo - k0, sink_k = seen.sink_keys - k0;
       const uint32_t recent = lo_k <= 0 ? 0xffffu : lo_k >= kKeys ? 0u : 0xffffu & ~((1u << lo_k) - 1u);
       const uint32_t sinks = sink_k <= 0 ? 0u : sink_k >= kKeys ? 0xffffu : (1u << sink_k) - 1u;
       return below & (recent | sinks);
     };
+    // this lane's piece of a group's first key, and the step to its next one
+    const bool real = piece * 8 < a.dim;
+    const T *kp0 = kbase + kvh * a.ks[1] + sub * a.ks[2] + (real ? piece * 8 : 0);
+    const T *vp0 = vbase + kvh * a.vs[1] + sub * a.vs[2] + (real ? piece * 8 : 0);
+    const int64_t kstep = RPI * a.ks[2], vstep = RPI * a.vs[2];
+    const int page_mask = (1 << a.page_shift) - 1;
     auto issue = [&](int it) {
       if (it < mine) {
         if ((it & 31) == 0) {
@@ -227,20 +235,19 @@ attn_decode_kernel(AttnArgs a, Ws ws, int blocks, int share) {
         const int page = __shfl_sync(0xffffffffu, page_ids, it & 31);
         const int g = group_of(it);
         const uint32_t mask = mask_of(g, page);
-        const int slot_in_page = (g * kKeys) & ((1 << a.page_shift) - 1);
         const int64_t pg = mask ? page : 0;
-        const T *kp = kbase + pg * a.ks[0] + kvh * a.ks[1] + slot_in_page * a.ks[2] + piece * 8;
-        const T *vp = vbase + pg * a.vs[0] + kvh * a.vs[1] + slot_in_page * a.vs[2] + piece * 8;
+        const int slot_in_page = (g * kKeys) & page_mask;
+        const T *kp = kp0 + pg * a.ks[0] + slot_in_page * a.ks[2];
+        const T *vp = vp0 + pg * a.vs[0] + slot_in_page * a.vs[2];
         const uint32_t st = ring + (it % kStages) * (2 * kKeys * DP * 2);
-        const bool real = piece * 8 < a.dim;
+        // a key that is not seen is not read: its place is zero, so nothing it holds can enter
 #pragma unroll
         for (int i = 0; i < kKeys / RPI; ++i) {
           const int key = sub + i * RPI;
-          // a key that is not seen is not read: its place is zero, so nothing it holds can enter
-          const bool in = real && ((mask >> key) & 1);
+          const bool in = real && (mask == 0xffffu || ((mask >> key) & 1));
           const uint32_t dst = st + swizzled<DP>(key, piece);
-          cp_async16(dst, in ? kp + key * a.ks[2] : kbase, in);
-          cp_async16(dst + kKeys * DP * 2, in ? vp + key * a.vs[2] : vbase, in);
+          cp_async16(dst, kp + i * kstep, in);
+          cp_async16(dst + kKeys * DP * 2, vp + i * vstep, in);
         }
       }
       cp_async_commit();
