@@ -26,6 +26,13 @@
 // the keys: a block takes a share of its key tiles and leaves its sum, maximum and output
 // in float32, and window_join_kernel puts the shares together.
 //
+// Bound: the exponentials.  A key tile of one query tile takes 128 x 128 of them, 1024
+// cycles of an SM's sixteen a cycle, next to 1024 of the two products (dim 128) and the
+// rest of the softmax's issue.  Measured: a prompt of 8192 tokens, 64 query heads over 8
+// of 128, bfloat16: 970 us (1.13 PFLOP/s); four chunks of 300 to 2000 tokens under a window
+// of 1024: 83 us (0.7 PFLOP/s of visible pairs: edge tiles are computed whole); up to 9
+// tokens of 3 rows: 10 us, latency alone.
+//
 // Warps: 0 loads, 1 issues the products (2 and 3 only fill their warpgroup), then four
 // per query tile for the softmax, to which the first four leave most of the registers.
 #include <cuda.h>
