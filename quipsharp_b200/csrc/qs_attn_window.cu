@@ -29,9 +29,16 @@
 // Bound: the exponentials.  A key tile of one query tile takes 128 x 128 of them, 1024
 // cycles of an SM's sixteen a cycle, next to 1024 of the two products (dim 128) and the
 // rest of the softmax's issue.  Measured: a prompt of 8192 tokens, 64 query heads over 8
-// of 128, bfloat16: 970 us (1.13 PFLOP/s); four chunks of 300 to 2000 tokens under a window
-// of 1024: 83 us (0.7 PFLOP/s of visible pairs: edge tiles are computed whole); up to 9
+// of 128, bfloat16: 960 us (1.15 PFLOP/s); four chunks of 300 to 2000 tokens under a window
+// of 1024: 81 us (0.73 PFLOP/s of visible pairs; ten tiles a job, four of them with masks); up to 9
 // tokens of 3 rows: 10 us, latency alone.
+//
+// A tile of which 64 keys hold all that its tokens see (a window's edge, the diagonal, first
+// tokens that stay) is computed for those 64 alone.  The loading warp, which has the time,
+// works out what each query tile sees of a key tile and leaves it as a word for the others;
+// the product instructions are the same for both kinds, with other addresses (a branch
+// around two bodies of them, or one that leaves out tiles that nothing sees, cost the
+// issuing warp more than the smaller tiles save: chunks 89 us).
 //
 // Warps: 0 loads, 1 issues the products (2 and 3 only fill their warpgroup), then four
 // per query tile for the softmax, to which the first four leave most of the registers.
@@ -202,7 +209,6 @@ struct Job {
   int from;         // first key after them
   int first, tiles; // this share's first tile, its tiles (0: tokens to clear, -1: no more jobs)
   int split;        // which share
-  int absent;       // a page among the keys is missing
 };
 
 // Registers per thread: 168 at launch (65536 / 384, in eights); the sum over the
@@ -311,6 +317,31 @@ __device__ __forceinline__ Job job_of(const WindowArgs &w, int x, int y, int z, 
   return j;
 }
 
+// What a query tile's tokens see of a key tile, as the loading warp tells it to the others:
+// where 64 keys from a multiple of 32 on hold all that any of them sees (a window's or the
+// diagonal's edge, first tokens that stay), the products and the softmax take only those.
+constexpr uint32_t kPlain = 1, kNarrow = 2;  // every token sees every key; 64 keys are enough
+constexpr int kFrom = 2;                     // two bits: where those begin, in 32s
+constexpr int kGaps = 8;                     // eight bits: 16s of keys whose page is missing
+__device__ __forceinline__ int narrow_from(uint32_t s) { return static_cast<int>((s >> kFrom) & 3) * 32; }
+
+__device__ __forceinline__ uint32_t span_of(const WindowArgs &w, const Job &j, int t, int k0, uint32_t gaps) {
+  const int ahead = t * w.tokens_per_tile, tokens = min(j.q1 - j.t0 - ahead, w.tokens_per_tile);
+  const int first = j.pos0 + ahead;
+  const int64_t window = w.a.window > 0 ? w.a.window : int64_t(1) << 40, sinks = w.a.sinks;
+  int lo = first + 1 > window ? static_cast<int>(first + 1 - window) - k0 : 0;
+  int hi = min(min(first + tokens, j.keys) - k0, kTile);
+  const bool plain = k0 + kTile <= min(first + 1, j.keys) && gaps == 0 &&
+                     (k0 + kTile <= sinks || k0 > first + w.tokens_per_tile - 1 - window);
+  if (plain) return kPlain;
+  if (lo > 0 && sinks > k0) {
+    if (lo >= hi) hi = static_cast<int>(min(static_cast<int64_t>(hi), sinks - k0));
+    lo = 0;
+  }
+  lo = clampi(lo, 0, kTile - 64) / 32;
+  return gaps << kGaps | (tokens <= 0 || hi <= lo * 32 + 64 ? kNarrow | lo << kFrom : 0u);
+}
+
 template <typename T, int DP, int NQ>
 __global__ void __launch_bounds__(Cfg<DP, NQ>::threads, 1)
 attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
@@ -319,6 +350,9 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   constexpr int S = C::stages;
   extern __shared__ uint8_t dsm[];
   __shared__ Job jobs[2];  // the current one and the next
+  constexpr int kSpans = 16;
+  static_assert(kSpans >= S / 2 + 3, "loads run ahead by half the ring");
+  __shared__ uint32_t spans[kSpans][NQ];  // of the last key tiles
   __shared__ __align__(16) uint8_t answer_s[16];
   const AttnArgs &a = w.a;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -383,7 +417,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       // ---- jobs, and loads: Q, then K and V tiles through one ring.  Lane b takes box b.
       const int boxes = kTile / w.granule, mask = (1 << a.page_shift) - 1;
       const uint32_t answer = smem_u32(answer_s);
-      int issued = 0, q_loads = 0, asks = 0, answers = 0;
+      int issued = 0, tiles = 0, q_loads = 0, asks = 0, answers = 0;
       uint32_t landed_phase = 0;
       bool ok = true;
       int bx = blockIdx.x, by = blockIdx.y, bz = blockIdx.z;
@@ -394,7 +428,6 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         if (!ok) break;
         if (lane == 0) {
           jobs[slot] = j;
-          jobs[slot].absent = 0;
           sm100::mbar_arrive(job_full(slot));
         }
         __syncwarp();
@@ -434,8 +467,12 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           const int k0 = key_of_tile(j, i), k = k0 + lane * w.granule;
           const uint32_t have = __ballot_sync(0xffffffffu, page >= 0);
           const int bytes = __popc(have) * w.granule * 128 * C::halves;
-          if (__any_sync(0xffffffffu, page < 0 && lane < boxes && k < j.keys) && lane == 0)
-            *const_cast<volatile int *>(&jobs[slot].absent) = 1;  // before the tile's loads: its scores come after
+          uint32_t gaps = __ballot_sync(0xffffffffu, page < 0 && lane < boxes && k < j.keys);  // boxes, then 16s
+          gaps = __ballot_sync(0xffffffffu, lane < kTile / 16 && (gaps >> (lane * 16 / w.granule)) & 1u);
+          if (lane < NQ)  // before the tile's loads: what reads it comes after them
+            *const_cast<volatile uint32_t *>(&spans[tiles % kSpans][lane]) = span_of(w, j, lane, k0, gaps);
+          ++tiles;
+          __syncwarp();
           // values of absent pages and past the last key must be zero: their weights are,
           // but zero times what stale memory may hold need not be
           const bool partial = __popc(have) != boxes || k0 + kTile > j.keys;
@@ -497,16 +534,23 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       }
     } else if (warp == 1) {
       // ---- products: the warp waits, one thread issues
-      constexpr uint32_t id_s = idesc_of<T>(kTile, false), id_o = idesc_of<T>(DP, true);
+      constexpr uint32_t id_s = idesc_of<T>(kTile, false), id_n = idesc_of<T>(kTile / 2, false), id_o = idesc_of<T>(DP, true);
       auto stage_of = [&](int x) { return ring + (x % S) * C::tile_bytes; };
       auto wait_tile = [&](int x) { return sm100::mbar_wait_warp(full(x % S), (x / S) & 1, w.wait_ns); };
-      auto scores = [&](int t, int x) {  // S of query tile t over the keys in ring place x
+      auto span_at = [&](int t, int i) {  // of key tile i, counted through the jobs
+        const uint32_t span = *const_cast<volatile uint32_t *>(&spans[i % kSpans][t]);
+        return __reduce_or_sync(0xffffffffu, span);  // a uniform register: see elect_one
+      };
+      auto scores = [&](int t, int x, int i) {  // S of query tile t over the keys of tile i, in ring place x
+        const uint32_t span = span_at(t, i);
         const uint64_t qd = sm100::sw128_kmajor_desc(q_sm + t * C::tile_bytes), kd = sm100::sw128_kmajor_desc(stage_of(x));
+        const bool narrow = span & kNarrow;
+        const uint32_t id = narrow ? id_n : id_s, from = narrow ? narrow_from(span) : 0;
         if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < DP / 16; ++k) {
             const uint32_t off = ((k / 4) * kHalf + (k % 4) * 32) >> 4;
-            sm100::umma_f16(tmem + t * kTile, qd + off, kd + off, id_s, k != 0);
+            sm100::umma_f16(tmem + t * kTile + from, qd + off, kd + (from * 128 >> 4) + off, id, k != 0);
           }
           sm100::umma_commit(s_full(t));
         }
@@ -531,7 +575,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         ++q_loads;
         if (!ok) break;
         sm100::tc_fence_after_sync();
-        for (int t = 0; t < NQ; ++t) scores(t, place);
+        for (int t = 0; t < NQ; ++t) scores(t, place, step);
         commit(empty(place % S));
         if (n == 1) commit(q_empty);
         for (int i = 0; i < n && ok; ++i) {
@@ -540,13 +584,16 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           for (int t = 0; t < NQ && ok; ++t) {
             const uint64_t vb = sw128_mnmajor_desc(stage_of(v));
             const uint32_t od = tmem + NQ * kTile + t * DP, pa = tmem + t * kTile;
+            const uint32_t span = span_at(t, step + i);
+            const bool narrow = span & kNarrow;
+            const uint32_t from = narrow ? narrow_from(span) / 16 : 0;
             ok = sm100::mbar_wait_warp(p_half(t), (step + i) & 1, w.wait_ns);
             if (!ok) break;
             sm100::tc_fence_after_sync();
             if (elect_one()) {
 #pragma unroll
               for (int k = 0; k < kTile / 32; ++k)
-                umma_ts(od, pa + k * 8, vb + k * (16 * 128 >> 4), id_o, k != 0 || i != 0);
+                umma_ts(od, pa + (from + k) * 8, vb + (from + k) * (16 * 128 >> 4), id_o, k != 0 || i != 0);
               sm100::umma_commit(half_done(t));
             }
             __syncwarp();
@@ -554,8 +601,10 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
             if (!ok) break;
             sm100::tc_fence_after_sync();
             if (elect_one()) {
+              if (!narrow) {
 #pragma unroll
-              for (int k = kTile / 32; k < kTile / 16; ++k) umma_ts(od, pa + k * 8, vb + k * (16 * 128 >> 4), id_o, 1);
+                for (int k = kTile / 32; k < kTile / 16; ++k) umma_ts(od, pa + k * 8, vb + k * (16 * 128 >> 4), id_o, 1);
+              }
               if (i + 1 == n) sm100::umma_commit(o_full(t));
             }
             __syncwarp();
@@ -563,7 +612,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
               if (t == 0) ok = wait_tile(k_next);
               if (!ok) break;
               sm100::tc_fence_after_sync();
-              scores(t, k_next);
+              scores(t, k_next, step + i + 1);
             }
           }
           if (!ok) break;
@@ -618,9 +667,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       const bool real = tok < w.tokens_per_tile && token < j.q1;
       const int pos = j.pos0 + t * w.tokens_per_tile + tok;
       // keys seen: k <= pos, and k > pos - window or k < sinks
-      const int pos_first = j.pos0 + t * w.tokens_per_tile, pos_last = pos_first + w.tokens_per_tile - 1;
       const int low = static_cast<int>(max(static_cast<int64_t>(-1), pos - win));  // keys above it are recent
-      const int64_t low_last = pos_last - win;
       float m = -INFINITY, l = 0.f;  // m in the units of S
       for (int i = 0; i < n; ++i) {
         ok = sm100::mbar_wait_warp(s_full(t), (step + i) & 1, w.wait_ns);
@@ -632,12 +679,15 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           for (int c = 0; c < kTile; c += 32) tmem_ld_32(s_at + c, raw + c);
           sm100::tmem_ld_wait();
         };
-        auto store = [&](int half) {  // the weights of 64 keys, over the first quarters of S
-          tmem_st_32(s_at + 32 * half, raw + 64 * half);
+        auto tell = [&](uint32_t bar) {  // that weights are stored
           tmem_st_wait();
           sm100::tc_fence_before_sync();
           __syncwarp();
-          if (lane == 0) sm100::mbar_arrive(half ? p_full(t) : p_half(t));
+          if (lane == 0) sm100::mbar_arrive(bar);
+        };
+        auto store = [&](int half) {  // the weights of 64 keys, over the first quarters of S
+          tmem_st_32(s_at + 32 * half, raw + 64 * half);
+          tell(half ? p_full(t) : p_half(t));
         };
         auto rescale = [&](float mn) {  // to a new reference
           const float f = m == mn ? 1.f : ex2((m - mn) * scale2);
@@ -653,11 +703,10 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           l *= f;
           m = mn;
         };
-        load();
+        const uint32_t span = *const_cast<volatile uint32_t *>(&spans[(step + i) % kSpans][t]);
+        load();  // what no token sees of it holds anything, and is not looked at
         const int k0 = key_of_tile(j, i);
-        const bool gaps = *const_cast<volatile int *>(&jobs[slot].absent) != 0;
-        const bool plain = k0 + kTile - 1 <= pos_first && (k0 > low_last || k0 + kTile <= sinks) &&
-                           k0 + kTile <= j.keys && !gaps;
+        const bool plain = span & kPlain, narrow = span & kNarrow;
         if (plain && i > 0) {
           // Most tiles: no mask, and the reference of the tiles before will do, which shows
           // afterwards.  No weight is above the sum's bound, which float16 holds.  The
@@ -688,34 +737,46 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           load();  // S is still in its place
         }
         float *s = reinterpret_cast<float *>(raw);
-        if (!plain) {
-          // the row's visible keys as bits: places up to hi that are above lo or below sk
+        // of 32 keys from b on, what the row does not see becomes -inf: as bits, the places up
+        // to hi that are above lo or below sk
+        auto mask = [&](float *s, int b) {
           const int hi = pos - k0, lo = low - k0, sk = sinks - k0;
-          const int *table = a.table + static_cast<int64_t>(j.row) * a.width;
+          uint32_t see = ones_below(hi + 1 - b) & (~ones_below(lo + 1 - b) | ones_below(sk - b));
+          const uint32_t gone = span >> (kGaps + b / 16);
+          see &= ~((gone & 1u ? 0xffffu : 0u) | (gone & 2u ? 0xffff0000u : 0u));
 #pragma unroll
-          for (int b = 0; b < kTile; b += 32) {
-            uint32_t see = ones_below(hi + 1 - b) & (~ones_below(lo + 1 - b) | ones_below(sk - b));
-            if (gaps) {
-#pragma unroll
-              for (int h = 0; h < 32; h += 16) {  // pages hold at least 16 keys
-                const int k = k0 + b + h;
-                const int p = k < j.keys ? table[k >> a.page_shift] : 0;
-                if (p < 0 || p >= a.pages) see &= ~(0xffffu << h);
-              }
-            }
-#pragma unroll
-            for (int c = 0; c < 32; ++c) s[b + c] = (see >> c) & 1 ? s[b + c] : -INFINITY;
-          }
+          for (int c = 0; c < 32; ++c) s[c] = (see >> c) & 1 ? s[c] : -INFINITY;
+        };
+        const int from = narrow ? narrow_from(span) : 0;
+        if (narrow) {
+          tmem_ld_32(s_at + from, raw);
+          tmem_ld_32(s_at + from + 32, raw + 32);
+          sm100::tmem_ld_wait();
         }
-        const float top = max3(top_of(raw), top_of(raw + 64), -INFINITY);
+        if (!plain) {
+          mask(s, from);
+          mask(s + 32, from + 32);
+        }
+        float top = top_of(raw);
+        if (!narrow) {
+          if (!plain) {
+            mask(s + 64, 64);
+            mask(s + 96, 96);
+          }
+          top = max3(top, top_of(raw + 64), top);
+        }
         const bool renew = m == -INFINITY ? top != -INFINITY : !((top - m) * scale2 <= 7.f);  // NaN stays; 2^(7 + kBias) fits float16
         if (i == 0) m = top;
         else if (__any_sync(0xffffffffu, renew)) rescale(renew ? top : m);
         const float shift = m == -INFINITY ? 0.f : kBias - m * scale2;
         l += weights<T>(raw, scale2, shift);
-        store(0);
-        l += weights<T>(raw + 64, scale2, shift);
-        store(1);
+        tmem_st_32(s_at + from / 2, raw);
+        tell(p_half(t));
+        if (!narrow) {
+          l += weights<T>(raw + 64, scale2, shift);
+          tmem_st_32(s_at + 32, raw + 64);
+        }
+        tell(p_full(t));
       }
       if (!ok) break;
       step += n;

@@ -42,8 +42,9 @@ def make(rs, lengths, kv_heads, page, dim, dtype, width=None, spare=3, junk=0.0)
     return k, v, torch.from_numpy(table).to(DEV), torch.from_numpy(lengths).to(DEV)
 
 
-def exact(q, k, v, table, lengths, new, window, sinks, scale=None):
-    """(out, lse, A) in 64 bits: row r's last new[r] tokens, packed."""
+def exact(q, k, v, table, lengths, new, window, sinks, scale=None, hidden=()):
+    """(out, lse, A) in 64 bits: row r's last new[r] tokens, packed; nobody sees the keys of
+    the columns `hidden`."""
     page, dim = k.shape[2], k.shape[3]
     share = q.shape[1] // k.shape[1]
     scale = dim ** -0.5 if scale is None else scale
@@ -60,6 +61,8 @@ def exact(q, k, v, table, lengths, new, window, sinks, scale=None):
         see = key <= pos
         if window:
             see &= (key > pos - window) | (key < sinks)
+        for c in hidden:
+            see &= key // page != c
         s = torch.einsum("thd,nhd->htn", qq, kk) * scale
         s = s.masked_fill(~see, -math.inf)
         lse = torch.logsumexp(s, -1)
@@ -275,6 +278,26 @@ def test_window(new, past, q_heads, kv_heads, page, dim, window, sinks, dtype):
     check(got, exact(q, k, v, table, n, new, window, sinks), dtype, weights=True)
     assert torch.equal(at.window_attention(q, k, v, table, n, cu, window=window or None, sinks=sinks), got[0])
     assert N.lib().qs_device_status(N.stream_of(q)) == N.QS_OK
+
+
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 32), (128, 128)])
+@pytest.mark.parametrize("hidden", [(), (3, 4)])
+def test_edges_at_every_place_of_a_key_tile(dim, page, hidden):
+    """Windows, sinks and starts that put the edges of what a query tile sees before, at and
+    after each 32 keys of a tile, with pages missing too."""
+    rs = np.random.RandomState(dim + page)
+    new, past = [150, 33, 1], [130, 421, 255]
+    k, v, table, n = make(rs, [a + b for a, b in zip(new, past)], 2, page, dim, torch.float16)
+    q = torch.randn(sum(new), 16, dim, device=DEV).half()
+    cu = torch.tensor(np.concatenate([[0], np.cumsum(new)]).astype(np.int32), device=DEV)
+    lines = table.clone()
+    for c in hidden:
+        if c < table.shape[1]:
+            table[:, c] = -1
+    for window in (1, 2, 31, 32, 33, 63, 64, 65, 95, 97, 127, 128, 129, 161, 200, 300):
+        for sinks in (0, 1, 33, 65, 100, 129):
+            got = at.window_attention(q, k, v, table, n, cu, window=window, sinks=sinks, return_lse=True)
+            check(got, exact(q, k, v, lines, n, new, window, sinks, hidden=hidden), torch.float16, weights=True)
 
 
 def test_window_tokens_of_no_row_are_zero():
