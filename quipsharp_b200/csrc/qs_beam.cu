@@ -5,14 +5,17 @@
 // continuations are its n largest logits, and the log-sum, which is not known until
 // the row ends, is not needed to find them.  beam_scan: each CTA takes a chunk of
 // one row; its threads keep a running maximum and sum of exponentials, and their
-// largest logit.  The n-th largest of those thread maxima is a bound that at least
+// largest logit.  A bound on the n-th largest of those thread maxima is one that at least
 // n logits of the chunk reach and few others do, so only the few threads whose
 // maximum reaches it look at their logits again.  beam_merge: one CTA per search
 // joins the chunks' lists into the beams', and the beams' into the result; a candidate's
 // place is the number of those ahead of it, so nothing is sorted and nothing depends on
 // the order of arrival.
 //
-// Bound: the logits' bytes, once.
+// Bound: the logits' bytes, once, for many rows; dependent steps for few.  Measured: 32
+// searches of 8 beams over 128000 bfloat16 logits, n = 16: 28 us (2.3 TB/s; 8 of them after
+// the stream's end); 4 beams over 32000 float32 logits, n = 4: 7.9 us.
+#include <algorithm>
 #include <cmath>
 
 #include "qs_common.cuh"
@@ -28,9 +31,11 @@ constexpr int kStep = 4;       // 16-byte pieces that a scanning thread takes at
 constexpr int kRing = 2;       // steps of its ring in shared memory
 constexpr int kCap = 1024;     // candidates of a chunk kept in shared memory
 constexpr int kItems = 512;    // pieces that are looked at again
+constexpr int kQuick = 16;     // n up to which the scan's bound comes from 32 maxima
 constexpr int kMinChunk = 2048;
 constexpr int kScanCtas = 8;   // scanning CTAs per SM
 constexpr int kLists = 4096;   // candidates merged at a time
+constexpr int kDirect = 32;    // candidates of a beam that are counted through as they are
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <typename T> struct Vec;  // a 16-byte piece of a row
@@ -220,6 +225,22 @@ __device__ __forceinline__ bool before(uint32_t k1, int t1, uint32_t k2, int t2)
   return k1 > k2 || (k1 == k2 && t1 < t2);
 }
 
+// How many of a list's entries come before x; at least n where they are no fewer (the list
+// is then left early, eight entries at a time, so that their loads do not wait).
+__device__ __forceinline__ int place_of(const uint2 *list, int count, uint2 x, int n) {
+  int r = 0, k = 0;
+  for (; k + 8 <= count && r < n; k += 8) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint2 y = list[k + i];
+      r += before(y.x, static_cast<int>(y.y), x.x, static_cast<int>(x.y)) ? 1 : 0;
+    }
+  }
+  for (; k < count && r < n; ++k)
+    r += before(list[k].x, static_cast<int>(list[k].y), x.x, static_cast<int>(x.y)) ? 1 : 0;
+  return r;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kS, kScanCtas) beam_scan_kernel(ScanArgs a) {
   constexpr int NV = Vec<T>::n, U = kStep, W = kS / 32;
@@ -318,22 +339,36 @@ __global__ void __launch_bounds__(kS, kScanCtas) beam_scan_kernel(ScanArgs a) {
   if (lane == 0) part[warp] = make_float2(sum.b, sum.l);
   __syncthreads();
   if (warp == 0) {
-    // a bound that at least n thread maxima, and so n logits, reach: the upper half of the
-    // n-th largest key, bit by bit, by one warp (every thread counting the maxima ahead of
-    // its own took 3 us more at 1024 CTAs: the others' instructions wait)
-    uint32_t k[W];
+    // A bound that at least n thread maxima, and so n logits, reach, by one warp (every
+    // thread counting the maxima ahead of its own took 3 us more at 1024 CTAs: the others'
+    // instructions wait).  For small n the n-th largest of 32 maxima of four threads each:
+    // about n + n^2 / 64 threads reach it, and it takes 200 cycles for the 2000 of the other.
+    // That one is the upper half of the n-th largest key, bit by bit.
+    uint32_t k[W], bound = 0;
 #pragma unroll
-    for (int i = 0; i < W; ++i) k[i] = tops[i * 32 + lane] >> 16;
-    uint32_t bound = 0;
+    for (int i = 0; i < W; ++i) k[i] = tops[i * 32 + lane];
+    if (a.n <= kQuick) {
+      uint32_t top4 = k[0];
+#pragma unroll
+      for (int i = 1; i < W; ++i) top4 = max(top4, k[i]);
+      int r = 0;
+#pragma unroll
+      for (int o = 0; o < 32; ++o) {
+        const uint32_t y = __shfl_sync(0xffffffffu, top4, o);
+        r += y > top4 || (y == top4 && o < lane) ? 1 : 0;
+      }
+      bound = __shfl_sync(0xffffffffu, top4, __ffs(__ballot_sync(0xffffffffu, r == a.n - 1)) - 1);
+    } else {
 #pragma unroll 1
-    for (int bit = 15; bit >= 0; --bit) {
-      const uint32_t t = bound | (1u << bit);
-      int c = 0;
+      for (int bit = 31; bit >= 16; --bit) {
+        const uint32_t t = bound | (1u << bit);
+        int c = 0;
 #pragma unroll
-      for (int i = 0; i < W; ++i) c += k[i] >= t ? 1 : 0;
-      if (__reduce_add_sync(0xffffffffu, c) >= a.n) bound = t;
+        for (int i = 0; i < W; ++i) c += k[i] >= t ? 1 : 0;
+        if (__reduce_add_sync(0xffffffffu, c) >= a.n) bound = t;
+      }
     }
-    if (lane == 0) bound_s = bound << 16;
+    if (lane == 0) bound_s = bound;
   } else if (tid == 32) {
     float b = part[0].x, l = part[0].y;
     for (int w = 1; w < W; ++w) join(b, l, part[w].x, part[w].y);
@@ -355,31 +390,25 @@ __global__ void __launch_bounds__(kS, kScanCtas) beam_scan_kernel(ScanArgs a) {
   };
   // the threads that reach it: usually only the step with the thread's largest logit, else
   // all its pieces, go to a list that all threads then share
-  for (uint32_t who = __ballot_sync(0xffffffffu, any && key >= bound); who; who &= who - 1) {
-    const int src = __ffs(who) - 1;
-    const bool one = __shfl_sync(0xffffffffu, next < least && top_at >= 0, src);
-    const int first = lo + (tid - lane) + src, step = __shfl_sync(0xffffffffu, top_at, src);
-    const int start = one ? step : first, stop = one ? min(hi, step + U * kS) : hi;
-    const int need = (stop - start + kS - 1) / kS;
-    int at = 0;
-    if (lane == 0) at = atomicAdd(&item_count, need);
-    at = __shfl_sync(0xffffffffu, at, 0);
-    for (int i = lane; i < need; i += 32) {
+  if (any && key >= bound) {
+    const bool one = next < least && top_at >= 0;
+    const int start = one ? top_at : lo + tid, stop = one ? min(hi, top_at + U * kS) : hi;
+    const int need = (stop - start + kS - 1) / kS, at = atomicAdd(&item_count, need);
+    for (int i = 0; i < need; ++i) {
       if (at + i < kItems) items[at + i] = start + i * kS;
       else look(start + i * kS);
     }
   }
   __syncthreads();
   for (int i = tid; i < min(item_count, kItems); i += kS)
-    if (items[i] >= 0) look(items[i]);
+    look(items[i]);
   __syncthreads();
   uint2 *out = a.cand + (static_cast<int64_t>(row) * a.chunks + chunk) * a.n;
   const int have = count;
   if (have <= kCap) {
     for (int i = tid; i < have; i += kS) {
       const uint2 c = cand[i];
-      int r = 0;
-      for (int k = 0; k < have && r < a.n; ++k) r += before(cand[k].x, cand[k].y, c.x, c.y) ? 1 : 0;
+      const int r = place_of(cand, have, c, a.n);
       if (r < a.n) out[r] = c;
     }
     for (int i = have + tid; i < a.n; i += kS) out[i] = make_uint2(0u, 0u);  // a chunk of fewer than n logits
@@ -418,6 +447,7 @@ __global__ void __launch_bounds__(kS, kScanCtas) beam_scan_kernel(ScanArgs a) {
 
 struct MergeArgs {
   int beams, n, chunks, pad;
+  int group, room;  // beams at a time; their entries, to a multiple of 4
   const float2 *stats;
   const uint2 *cand;
   const float *scores;
@@ -425,27 +455,6 @@ struct MergeArgs {
   float *scores_out;
   int *parents_out, *tokens_out;
 };
-
-// Entries of a list of n falling keys that come before key k: those >= k where the
-// list goes first among equals (x >= k is x > k - 1: no key of an entry is 0), those > k
-// where it goes later.  Short lists are counted through (their loads do not wait for one
-// another), longer ones halved.
-__device__ __forceinline__ int entries_before(const uint32_t *list, int stride, int n, uint32_t k, bool first) {
-  const uint32_t above = first ? k - 1u : k;
-  int lo = 0;
-  if (n <= 16) {
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) lo += list[i * stride] > above ? 1 : 0;
-    return lo;
-  }
-  int hi = n;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (list[mid * stride] > above) lo = mid + 1;
-    else hi = mid;
-  }
-  return lo;
-}
 
 __host__ __device__ constexpr int round4(int v) { return (v + 3) / 4 * 4; }
 
@@ -463,76 +472,114 @@ __device__ __forceinline__ void copy8(void *dst, const void *src) {
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 __global__ void __launch_bounds__(kT) beam_merge_kernel(MergeArgs a) {
-  extern __shared__ uint32_t sm[];
+  extern __shared__ __align__(16) uint32_t sm[];
   uint2 *in = reinterpret_cast<uint2 *>(sm);                // chunks' lists of some beams
-  uint16_t *left = reinterpret_cast<uint16_t *>(sm + 2 * kLists);  // entries of each beam that matter
-  uint32_t *key = sm + 2 * kLists + kLists / 2;             // [beams][n]: score keys, falling
-  int *tok = reinterpret_cast<int *>(key + a.beams * a.n);  // [beams][n]
-  int *place = tok + a.beams * a.n;                         // [beams][n]: places in the joint list
-  Beam *beams = reinterpret_cast<Beam *>(key + round4(3 * a.beams * a.n));
+  uint2 *left = in + a.room;                                // entries of each beam that matter
+  const int total = a.beams * a.n, total4 = round4(total);
+  uint32_t *key = sm + (a.chunks * a.n <= kDirect ? 2 : 4) * a.room;  // [beams][n]: score keys; zeros to a multiple of 4
+  int *tok = reinterpret_cast<int *>(key + total4);         // [beams][n]
+  Beam *beams = reinterpret_cast<Beam *>(tok + total4);
   pdl_wait();
   pdl_launch_dependents();
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
-  const int per = a.chunks * a.n, group = min(a.beams, kLists / per);  // beams at a time
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = a.chunks * a.n, group = a.group;
   const uint2 *lists = a.cand + static_cast<int64_t>(b) * a.beams * per;
-  for (int i = tid; i < group * per; i += kT) copy8(&in[i], &lists[i]);
-  for (int k = tid >> 5; k < a.beams; k += kT / 32) {
-    const int64_t row = static_cast<int64_t>(b) * a.beams + k;
-    const float score = a.scores[row];
-    const int ended = a.finished ? a.finished[row] : 0;
-    float sb = -INFINITY, sl = 0.f;
-    for (int c = lane; c < a.chunks; c += 32) {
-      const float2 s = a.stats[row * a.chunks + c];
-      join(sb, sl, s.x, s.y);
+  for (int i = total + tid; i < total4; i += kT) key[i] = 0u;
+  // The beams' sums: by the warps that have no list while the others are at theirs, where
+  // there are such, else afterwards.
+  auto sums = [&] {
+    for (int k = warp ^ (kT / 64); k < a.beams; k += kT / 32) {
+      const int64_t row = static_cast<int64_t>(b) * a.beams + k;
+      const float score = a.scores[row];
+      const int ended = a.finished ? a.finished[row] : 0;
+      float sb = -INFINITY, sl = 0.f;
+      for (int c = lane; c < a.chunks; c += 32) {
+        const float2 s = a.stats[row * a.chunks + c];
+        join(sb, sl, s.x, s.y);
+      }
+      for (int d = 1; d < a.chunks && d < 32; d <<= 1)
+        join(sb, sl, __shfl_xor_sync(0xffffffffu, sb, d), __shfl_xor_sync(0xffffffffu, sl, d));
+      if (lane == 0) beams[k] = Beam{log(static_cast<double>(sl)), sb, score, ended};
     }
-    for (int d = 1; d < a.chunks && d < 32; d <<= 1)
-      join(sb, sl, __shfl_xor_sync(0xffffffffu, sb, d), __shfl_xor_sync(0xffffffffu, sl, d));
-    if (lane == 0) beams[k] = Beam{log(static_cast<double>(sl)), sb, score, ended};
-  }
-  for (int k0 = 0; k0 < a.beams; k0 += group) {
+  };
+  const bool apart = a.beams <= kT / 64 && group == a.beams;
+  const int listing = apart ? kT / 2 : kT;
+  auto listed = [&] { asm volatile("bar.sync 1, %0;" ::"r"(listing) : "memory"); };
+  if (apart && warp >= kT / 64) sums();
+  for (int k0 = 0; k0 < a.beams && tid < listing; k0 += group) {
     const int kn = min(group, a.beams - k0);
-    if (k0)
-      for (int i = tid; i < kn * per; i += kT) copy8(&in[i], &lists[static_cast<int64_t>(k0) * per + i]);
+    for (int i = tid; i < kn * per; i += listing) copy8(&in[i], &lists[static_cast<int64_t>(k0) * per + i]);
     copies_done();
-    __syncthreads();
-    // a warp for each beam: the upper half of its n-th largest key, bit by bit; the entries
-    // that reach it; their places by counting those ahead
-    for (int k = tid >> 5; k < kn; k += kT / 32) {
+    listed();
+    // A warp for each beam.  Its n best are no lower than a bound that n entries reach: the
+    // n-th largest of the chunks' first ones where there are n chunks, else of their first m,
+    // of which there are n and a half of n or more.  Each chunk's list falls, so a lane walks
+    // it down to the bound; places come from counting those ahead.
+    for (int k = warp; k < kn; k += listing / 32) {
       const uint2 *mine = in + k * per;
-      uint16_t *some = left + k * per;
-      uint32_t bound = 0;
-#pragma unroll 1
-      for (int bit = 15; bit >= 0 && per > 48; --bit) {  // fewer are counted through as they are
-        const uint32_t t = bound | (1u << bit);
-        int c = 0;
-#pragma unroll 4
-        for (int i = lane; i < per; i += 32) c += (mine[i].x >> 16) >= t ? 1 : 0;
-        if (__reduce_add_sync(0xffffffffu, c) >= a.n) bound = t;
-      }
-      bound <<= 16;
-      int count = 0;
-      for (int i0 = 0; i0 < per; i0 += 32) {
-        const int i = i0 + lane;
-        const uint32_t key_i = i < per ? mine[i].x : 0u;
-        const uint32_t who = __ballot_sync(0xffffffffu, key_i != 0u && key_i >= bound);
-        if ((who >> lane) & 1) some[count + __popc(who & ((1u << lane) - 1u))] = static_cast<uint16_t>(i);
-        count += __popc(who);
-      }
-      __syncwarp();
-      for (int s = lane; s < count; s += 32) {
-        const uint2 x = mine[some[s]];
-        int r = 0;
-        for (int o = 0; o < count && r < a.n; ++o) {
-          const uint2 y = mine[some[o]];
-          r += before(y.x, static_cast<int>(y.y), x.x, static_cast<int>(x.y)) ? 1 : 0;
+      uint2 *some = left + k * per;
+      int count = per;
+      if (per <= kDirect) {
+        some = in + k * per;
+      } else {
+        uint32_t bound = 0;  // the same key may be there more than once
+        if (a.chunks >= a.n) {
+          for (int c = lane; c < a.chunks; c += 32) {
+            const uint32_t x = mine[c * a.n].x;
+            int r = 0;
+#pragma unroll 8
+            for (int d = 0; d < a.chunks; ++d) {
+              const uint32_t y = mine[d * a.n].x;
+              r += y > x || (y == x && d < c) ? 1 : 0;
+            }
+            if (r == a.n - 1) bound = x;
+          }
+        } else {
+          const int m = min(a.n, (a.n + a.n / 2 + a.chunks - 1) / a.chunks);
+          for (int i = lane; i < a.chunks * m; i += 32) {
+            const uint32_t x = mine[i / m * a.n + i % m].x;
+            int r = 0;
+            for (int c = 0, d = 0; c < a.chunks; ++c)
+#pragma unroll 2
+              for (int j = 0; j < m; ++j, ++d) {
+                const uint32_t y = mine[c * a.n + j].x;
+                r += y > x || (y == x && d < i) ? 1 : 0;
+              }
+            if (r == a.n - 1) bound = x;
+          }
         }
+        bound = __reduce_max_sync(0xffffffffu, bound);
+        bound = max(bound, 1u);  // 0 is no entry
+        count = 0;
+        for (int c0 = 0; c0 < a.chunks; c0 += 32) {
+          const uint2 *list = mine + (c0 + lane) * a.n;
+          int have = 0;
+          if (c0 + lane < a.chunks)
+            while (have < a.n && list[have].x >= bound) ++have;
+          int before_me = have;
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, before_me, d);
+            if (lane >= d) before_me += y;
+          }
+          for (int i = 0; i < have; ++i) some[count + before_me - have + i] = list[i];
+          count += __shfl_sync(0xffffffffu, before_me, 31);
+        }
+        __syncwarp();
+      }
+      for (int i = lane; i < count; i += 32) {
+        const uint2 x = some[i];
+        if (x.x == 0u) continue;
+        const int r = place_of(some, count, x, a.n);
         if (r >= a.n) continue;
         key[(k0 + k) * a.n + r] = x.x;
         tok[(k0 + k) * a.n + r] = static_cast<int>(x.y);
       }
     }
-    __syncthreads();
+    listed();
   }
+  if (!apart) sums();
+  __syncthreads();
   // logits to scores: s + ((x - top) - log(sum of e^(x - top))), the last log from the
   // stored sum in 64 bits (once per beam and thread), rounded once
   for (int k = tid >> 5; k < a.beams; k += kT / 32) {
@@ -551,26 +598,31 @@ __global__ void __launch_bounds__(kT) beam_merge_kernel(MergeArgs a) {
         s += top == -INFINITY ? -INFINITY : (v == top ? 0.f : v - top) - log_sum;
       }
       key[k * a.n + j] = key_of(fmaxf(s, -INFINITY));
-      place[k * a.n + j] = j;
     }
   }
   __syncthreads();
-  // places in the joint list: a thread per candidate and other beam
-  const int total = a.beams * a.n;
-  for (int i = tid; i < total * a.beams; i += kT) {
-    const int c = i / a.beams, o = i - c * a.beams, beam = c / a.n;
-    if (o == beam) continue;
-    const int r = entries_before(key + o * a.n, 1, a.n, key[c], o < beam);
-    if (r) atomicAdd(&place[c], r);
-  }
-  __syncthreads();
-  for (int i = tid; i < total; i += kT) {
-    const int beam = i / a.n, r = place[i];
-    if (r >= a.n) continue;
-    const int64_t at = static_cast<int64_t>(b) * a.n + r;
-    a.scores_out[at] = value_of(key[i]);
-    a.parents_out[at] = beam;
-    a.tokens_out[at] = tok[i];
+  // Places in the joint list: a candidate's is the number of those ahead, by score, then in
+  // the order they stand (the beam, then its list).  A few neighbouring threads share one.
+  int share = 1;
+  while (share < 16 && share * 2 * total <= kT) share *= 2;
+  const int part = tid & (share - 1);
+  for (int c0 = 0; c0 < total; c0 += kT / share) {
+    const int c = c0 + tid / share;
+    const uint32_t x = c < total ? key[c] : 0xffffffffu;
+    int r = 0;
+#pragma unroll 4
+    for (int d = part * 4; d < total4; d += share * 4) {
+      const uint4 y = *reinterpret_cast<const uint4 *>(key + d);
+      r += (y.x > x || (y.x == x && d < c) ? 1 : 0) + (y.y > x || (y.y == x && d + 1 < c) ? 1 : 0) +
+           (y.z > x || (y.z == x && d + 2 < c) ? 1 : 0) + (y.w > x || (y.w == x && d + 3 < c) ? 1 : 0);
+    }
+    for (int d = 1; d < share; d <<= 1) r += __shfl_xor_sync(0xffffffffu, r, d);
+    if (part == 0 && c < total && r < a.n) {
+      const int64_t at = static_cast<int64_t>(b) * a.n + r;
+      a.scores_out[at] = value_of(x);
+      a.parents_out[at] = c / a.n;
+      a.tokens_out[at] = tok[c];
+    }
   }
 }
 
@@ -609,11 +661,14 @@ int launch_beam_select(const void *logits, int dtype, int64_t batch_stride, int6
   const int st = dtype == QS_F32 ? run_scan<float>(a, rows, s)
                  : dtype == QS_F16 ? run_scan<__half>(a, rows, s) : run_scan<__nv_bfloat16>(a, rows, s);
   if (st) return st;
-  const MergeArgs m{static_cast<int>(beams), n, chunks, pad, stats, cand, scores, finished, scores_out, parents_out,
+  const int per = chunks * n, group = static_cast<int>(std::min<int64_t>(beams, kLists / per)), room = round4(group * per);
+  const MergeArgs m{static_cast<int>(beams), n, chunks, pad, group, room, stats, cand, scores, finished, scores_out, parents_out,
                     tokens_out};
-  const size_t smem = static_cast<size_t>(kLists) * 10 + round4(static_cast<int>(3 * beams * n)) * 4 + beams * sizeof(Beam);
+  // as much as this call needs: SMs that have to change their split of memory wait for the
+  // kernel before (3 us)
+  const size_t smem = static_cast<size_t>(room) * (per <= kDirect ? 8 : 16) + round4(static_cast<int>(beams * n)) * 8 + beams * sizeof(Beam);
   static const cudaError_t attr = cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                       kLists * 10 + kBeamMaxBeams * kBeamMaxN * 12 + kBeamMaxBeams * (int)sizeof(Beam));
+                                                       kLists * 16 + kBeamMaxBeams * kBeamMaxN * 8 + kBeamMaxBeams * (int)sizeof(Beam));
   if (attr != cudaSuccess) return fail(QS_ERR_CUDA, "beam merge: %s", cudaGetErrorString(attr));
   return launch_pdl("beam merge", beam_merge_kernel, dim3(static_cast<unsigned>(batch)), dim3(kT), smem, s, m);
 }
