@@ -70,6 +70,13 @@ def test_select(B, K, V, n, dtype):
     check(x, s, n)
 
 
+@pytest.mark.parametrize("B,K,V,n", [
+    (1, 64, 40000, 64), (2, 9, 30000, 16), (8, 6, 30004, 16), (2, 8, 60000, 17), (1, 1, 128000, 33), (4, 16, 9000, 3)])
+def test_lists_of_every_shape(B, K, V, n):
+    """Fewer and more chunks than n, beams merged some at a time, more beams than half the warps."""
+    check(*spread(B, K, V, torch.float16, 3), n)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_ties_go_to_the_lower_token_and_beam(dtype):
     x = torch.zeros(2, 3, 5000, device=DEV, dtype=dtype)  # every logit equal, in every chunk
