@@ -13,12 +13,14 @@
 // segment that several ranges share leaves partial results (maximum, sum, output in
 // float32), which attn_join_kernel puts together in order.  Where no row can see more than
 // kWholeGroups groups (short tables, short windows), a CTA takes a segment whole and
-// there is nothing to join.
+// there is nothing to join; where segments are few, the CTAs of a cluster share it and join
+// over each other's shared memory.
 //
 // Bound: the keys and values seen, once, at HBM rate.  Measured: 64 rows of 100 to 16000
 // tokens, 64 query heads over 8 of 128, bfloat16: 318 us for 2.0 GB (6.3 TB/s); 48 rows
 // under a window of 1000, 28 heads over 4 of 64: 13.7 us (46 MB, 3.4 TB/s: 192 segments of
-// unequal length, and a step's latency); one row of 203 tokens 5.2 us, latency alone.
+// unequal length, and a step's latency); one row of 203 tokens 5.2 us, latency alone;
+// one row of 1500, 8 key heads, 6.9.
 #include <cmath>
 #include <type_traits>
 
@@ -37,7 +39,7 @@ constexpr int kDealWarps = 4;     // warps of a CTA that is dealt ranges
 constexpr int kRanges = 148 * kCtasPerSm * kRangesPerCta;
 constexpr int kMinRange = 16;     // groups of a range at least: 4 per warp, or the joins cost more than the split saves
 constexpr int kLongRange = 128;   // the start of a shorter range is not paid for by the evener shares
-constexpr int kWholeGroups = 80;  // a CTA of four warps takes 20 steps for them
+constexpr int kWholeGroups = 80;  // for each CTA of a segment; one of four warps takes 20 steps for them
 
 // The groups of 16 keys that a row's newest token sees: the first `sink` groups, then
 // those from `from` on.
@@ -79,9 +81,32 @@ template <typename T, int DP, int W>
 struct Smem {
   T kv[W][kStages][2][kKeys * DP];
   float ml[W][kRows][2];
+  float joined[kRows][2];  // of this CTA's warps
   int64_t sums[W * 32 + 1][2];
   int lengths[W * 32];  // of the first rows
 };
+
+// The CTAs of a cluster (where a segment is shared by several).
+__device__ __forceinline__ int cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return static_cast<int>(r);
+}
+__device__ __forceinline__ int cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return static_cast<int>(r);
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float2 peer_pair(const float *mine, int rank) {  // the same place in another CTA's memory
+  uint32_t at;
+  float2 x;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(mine)), "r"(rank));
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x.x), "=f"(x.y) : "r"(at) : "memory");
+  return x;
+}
 
 // One warp's softmax state over 16 query rows (R8: only the first 8 are real).
 template <typename T, int DP, bool R8>
@@ -289,6 +314,16 @@ attn_decode_kernel(AttnArgs a, Ws ws, int blocks, int share) {
     }
     __syncthreads();
     const bool whole = u0 == 0 && u1 == seen.count;
+    auto finish = [&](int r, int c2, float m, float l, float2 o) {
+      const int64_t out = static_cast<int64_t>(row) * a.q_heads + h0 + r;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      uint32_t packed;
+      split16<T>(o.x * inv, o.y * inv, packed);
+      if (c2 < a.dim) *reinterpret_cast<uint32_t *>(static_cast<T *>(a.out) + out * a.dim + c2) = packed;
+      if (c2 == 0 && a.lse) a.lse[out] = l == 0.f ? -INFINITY : (m - kBias + log2f(l)) * kLn2;
+    };
+    const int ctas = WHOLE ? cluster_size() : 1;
+    float *first = reinterpret_cast<float *>(&sm.kv[0][0][0][0]);
     for (int i = tid; i < hn * (DP / 2); i += kThreads) {
       const int r = i / (DP / 2), c2 = i % (DP / 2) * 2;
       float m = -INFINITY, l = 0.f;
@@ -303,26 +338,43 @@ attn_decode_kernel(AttnArgs a, Ws ws, int blocks, int share) {
         o.x += f * x.x;
         o.y += f * x.y;
       }
-      if (WHOLE || whole) {
-        const int64_t out = static_cast<int64_t>(row) * a.q_heads + h0 + r;
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        uint32_t packed;
-        split16<T>(o.x * inv, o.y * inv, packed);
-        if (c2 < a.dim) *reinterpret_cast<uint32_t *>(static_cast<T *>(a.out) + out * a.dim + c2) = packed;
-        if (c2 == 0 && a.lse) a.lse[out] = l == 0.f ? -INFINITY : (m - kBias + log2f(l)) * kLn2;
+      if (WHOLE && ctas > 1) {  // over what this thread alone has read
+        *reinterpret_cast<float2 *>(first + r * DP + c2) = o;
+        if (c2 == 0) sm.joined[r][0] = m, sm.joined[r][1] = l;
+      } else if (WHOLE || whole) {
+        finish(r, c2, m, l, o);
       } else {
         *reinterpret_cast<float2 *>(ws.o + (slot * kRows + r) * DP + c2) = o;
         if (c2 == 0) ws.ml[(slot * kRows + r) * 2] = m, ws.ml[(slot * kRows + r) * 2 + 1] = l;
       }
+    }
+    if (WHOLE && ctas > 1) {  // each CTA takes its part of the outputs, over all CTAs' sums
+      cluster_barrier();
+      for (int i = cluster_rank() * kThreads + tid; i < hn * (DP / 2); i += ctas * kThreads) {
+        const int r = i / (DP / 2), c2 = i % (DP / 2) * 2;
+        float m = -INFINITY, l = 0.f;
+        float2 o = make_float2(0.f, 0.f);
+        for (int v = 0; v < ctas; ++v) m = fmaxf(m, peer_pair(sm.joined[r], v).x);
+        for (int v = 0; v < ctas; ++v) {
+          const float2 ml = peer_pair(sm.joined[r], v), x = peer_pair(first + r * DP + c2, v);
+          const float f = weight(ml.x, m);
+          l += f * ml.y;
+          o.x += f * x.x;
+          o.y += f * x.y;
+        }
+        finish(r, c2, m, l, o);
+      }
+      cluster_barrier();  // no CTA leaves while another reads from it
+      return;
     }
     __syncthreads();
   };
 
   const int heads = a.kv_heads * blocks;  // segments per row
   if (WHOLE) {
-    const int row = blockIdx.x / heads;
+    const int ctas = cluster_size(), at = blockIdx.x / ctas, row = at / heads, rank = cluster_rank();
     const Seen seen = seen_of(a.lengths[row], a);
-    segment(row, blockIdx.x % heads, seen, 0, seen.count, 0);
+    segment(row, at % heads, seen, seen.count * rank / ctas, seen.count * (rank + 1) / ctas, 0);
     return;
   }
 
@@ -506,12 +558,50 @@ int64_t most_groups(int64_t page, int64_t width, int64_t window, int64_t sinks) 
   return ceil_div(keys, kKeys);
 }
 
+// CTAs (of four warps) that share a segment as a cluster: where segments are few, as many as
+// the SMs hold, each with two groups a warp or more.  Eight heads of 128 under a window of
+// 1000: one row 11.5 us with one CTA of eight warps, 7.4 with clusters of 4, 6.0 of 8; 8 rows
+// 12.7, 10.0, 15.1; 16 rows 15.2 and 21 (each CTA alone again).  30 keys: 3.6, 5.0, 5.1.
+int ctas_of(int64_t segments, int64_t most) {
+  if (segments * 8 <= 148 * kCtasPerSm && most >= 64) return 8;
+  if (segments * 4 <= 148 * kCtasPerSm && most >= 32) return 4;
+  return 1;
+}
+
+// Whether each segment is taken whole (see kWholeGroups).  More CTAs take longer ones: 1500
+// keys of one row 9.9 us dealt and 6.9 whole, 3800 10.4 both; 8 rows of up to 2000 18.9 and 14.4.
+bool taken_whole(int64_t segments, int64_t most) {
+  const int ctas = ctas_of(segments, most);
+  return most <= kWholeGroups * (ctas == 8 ? 3 : ctas == 4 ? 2 : 1);
+}
+
+template <typename... KArgs>
+int launch_clusters(void (*kern)(KArgs...), int64_t clusters, int ctas, int threads, int smem, cudaStream_t s,
+                    KArgs... args) {
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ctas;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(clusters * ctas));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  return e == cudaSuccess ? QS_OK : fail(QS_ERR_CUDA, "attention (decode): %s", cudaGetErrorString(e));
+}
+
 template <typename T, int DP, bool R8, int W, bool WHOLE>
-int run(const AttnArgs &a, const Ws &ws, int blocks, int share, int64_t grid, cudaStream_t s) {
+int run(const AttnArgs &a, const Ws &ws, int blocks, int share, int64_t grid, cudaStream_t s, int ctas = 1) {
   auto kern = attn_decode_kernel<T, DP, R8, W, WHOLE>;
   constexpr int smem = static_cast<int>(sizeof(Smem<T, DP, W>));
   static const cudaError_t attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (attr != cudaSuccess) return fail(QS_ERR_CUDA, "attention (decode): %s", cudaGetErrorString(attr));
+  if (ctas > 1) return launch_clusters(kern, grid, ctas, W * 32, smem, s, a, ws, blocks, share);
   return launch_pdl("attention (decode)", kern, dim3(static_cast<unsigned>(grid)), dim3(W * 32), smem, s, a, ws, blocks,
                     share);
 }
@@ -519,7 +609,9 @@ int run(const AttnArgs &a, const Ws &ws, int blocks, int share, int64_t grid, cu
 template <typename T, int DP, bool R8>
 int run_shape(const AttnArgs &a, const Ws &ws, int blocks, int share, cudaStream_t s) {
   const int64_t segments = static_cast<int64_t>(a.rows) * a.kv_heads * blocks, most = most_groups(int64_t(1) << a.page_shift, a.width, a.window, a.sinks);
-  if (most <= kWholeGroups) {
+  if (taken_whole(segments, most)) {
+    const int ctas = ctas_of(segments, most);
+    if (ctas > 1) return run<T, DP, R8, 4, true>(a, ws, blocks, share, segments, s, ctas);
     // eight warps where all segments run at once anyway
     if (segments <= 148 * (DP == 64 ? 2 : 1)) return run<T, DP, R8, 8, true>(a, ws, blocks, share, segments, s);
     return run<T, DP, R8, 4, true>(a, ws, blocks, share, segments, s);
@@ -545,8 +637,9 @@ int run_type(const AttnArgs &a, const Ws &ws, int blocks, int share, cudaStream_
 
 int64_t attn_decode_workspace_bytes(int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t page,
                                     int64_t width, int64_t window, int64_t sinks) {
-  if (most_groups(page, width, window, sinks) <= kWholeGroups) return 0;
   const Shape s = shape_of(rows, q_heads, kv_heads, dim);
+  const int64_t most = most_groups(page, width, window, sinks);
+  if (taken_whole(rows * s.heads, most)) return 0;
   return round_up((rows + 1) * 8 + 8, 256) + s.slots * kRows * (s.dp + 2) * 4;
 }
 

@@ -101,6 +101,10 @@ DECODE = [
     ([20000, 130, 11000], 16, 2, 64, 128, 0, 0),          # ranges shared by several CTAs
     ([9000] * 3 + [3] * 50, 8, 2, 16, 128, 0, 0),
     ([50 + 7 * i for i in range(200)], 4, 4, 16, 64, 0, 0),  # more rows than threads
+    ([1100, 3, 0, 64, 1090], 8, 2, 16, 64, 0, 0),            # eight CTAs share a segment, some with nothing
+    ([550, 1, 0, 300, 512, 20, 77, 490], 16, 8, 32, 128, 0, 0),  # four
+    ([1500, 20, 3700], 48, 2, 64, 96, 0, 0),                 # two blocks of rows a key head
+    ([3000, 4000, 10], 14, 2, 32, 64, 1100, 40),
 ]
 
 
