@@ -183,7 +183,8 @@ def build_fast(verbose: bool, force: bool) -> str:
            "-I", os.path.join(inc, "torch", "csrc", "api", "include"), "-I", cuda,
            src, "-o", out, "-L", LIBDIR, f"-l:{LIBNAME}", "-Wl,-rpath,$ORIGIN",
            # torch's own libraries are loaded by the time this is
-           "-L", os.path.join(os.path.dirname(inc), "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+           "-L", os.path.join(os.path.dirname(inc), "lib"), "-ltorch_python",
+           "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
