@@ -42,7 +42,7 @@ def test_cache_arguments():
     assert need > 0 and lib.qs_cache_workspace_bytes(8193, 4) == -1 and lib.qs_cache_workspace_bytes(1, 0) == -1
 
     def fork(table_out=at(2560), ws=at(1 << 16), nb=need, rows=1, parents=at(1024)):
-        return lib.qs_cache_fork(N.ref(p), rows, 1, at(256), at(512), at(768), parents, table_out, at(3072), at(3584), ws, nb,
+        return lib.qs_cache_fork(N.ref(p), rows, 1, at(256), at(512), at(768), parents, table_out, at(2816), at(3584), ws, nb,
                                  None)
 
     assert fork(parents=None) == N.QS_ERR_INVALID_ARG
@@ -62,12 +62,12 @@ def test_cache_arguments():
 def test_attention_arguments():
     lib, p, at = N.lib(), pool(), ctypes.c_void_p
     sizes = lib.qs_attn_decode_workspace_bytes
-    need = sizes(3, 4, 2, 64, 16, 100, 0, 0)
+    need = sizes(3, 4, 2, 64, 16, 400, 0, 0)
     assert need > 0 and sizes(3, 4, 2, 64, 16, 10, 0, 0) == sizes(3, 4, 2, 64, 16, 100, 500, 4) == 0  # few keys: no joins
     assert sizes(3, 5, 2, 64, 16, 100, 0, 0) == sizes(3, 4, 2, 136, 16, 100, 0, 0) == sizes(3, 4, 2, 64, 16, -1, 0, 0) == -1
 
     def decode(q=at(4096), heads=4, scale=0.1, window=0, sinks=0, ws=at(1 << 16), nb=need, pool=p, q_head=64):
-        return lib.qs_attn_decode(q, 256, q_head, N.ref(pool), 3, heads, 100, at(256), at(512), scale, window, sinks, at(8192),
+        return lib.qs_attn_decode(q, 256, q_head, N.ref(pool), 3, heads, 400, at(256), at(512), scale, window, sinks, at(8192),
                                   None, ws, nb, None)
 
     assert decode(q=None) == N.QS_ERR_INVALID_ARG and decode(heads=5) == N.QS_ERR_INVALID_ARG
