@@ -125,7 +125,7 @@ struct ScanArgs {
   const void *logits;
   int64_t batch_stride, beam_stride;
   int beams, vocab, n, chunks, chunk;  // chunk: 16-byte pieces per CTA
-  float2 *stats;                       // [row][chunk]: reference b, sum of 2^(x c - b), c = log2(e) in float32
+  float2 *stats;                       // [row][chunk]: a logit r near the largest, sum of e^(x - r)
   uint2 *cand;                         // [row][chunk][n]: key, token
 };
 
@@ -156,19 +156,29 @@ struct Row {
   }
 };
 
-// A thread's sum of 2^(x c - b).  The reference b is a float32 near the maximum times c
-// and is itself exact: x c - b is rounded once, so no term is off by more than its own
-// distance to b, and it may lag behind the maximum by kLag, which float32 sums hold.
+// A thread's sum.  Beside an ordinary reference (the largest logit, or kLag below it, which
+// float32 sums hold) it is of 2^(x c - b) with c = log2(e) and b = ref c, both in float32:
+// x c - b is rounded once, so no term is off by more than its own distance to b.  What b was
+// rounded by grows with it, though, and past some 2^31 would take 2^(x c - b) out of float32's
+// range (a vocabulary masked with the type's lowest number, in float32 or bfloat16), so beside
+// a larger reference the sum is of 2^((x - ref) c).
 constexpr float kLag = 8.f;
+constexpr float kOrdinary = 0x1p20f;  // b is off by 2^-4 at most
 struct Sum {
   float ref = -INFINITY, b = -INFINITY, l = 0.f;  // b = ref * c
+  float limit = -INFINITY;                        // ordinary numbers up to here need no other reference
 
-  __device__ __forceinline__ void renew(float top) {
+  __device__ __forceinline__ bool ordinary() const { return fabsf(ref) < kOrdinary; }
+  __device__ __forceinline__ void renew(float top) {  // both references ordinary, or the old one -inf
     const float nb = top * kLog2e;
     l *= b == nb ? 1.f : ex2(b - nb);
     ref = top;
     b = nb;
+    limit = ref + kLag;
   }
+  // What b was rounded by: the sum is of e^(x - ref) times 2^this.
+  __device__ __forceinline__ float off() const { return ordinary() ? fmaf(ref, kLog2e, -b) : 0.f; }
+  __device__ __forceinline__ float natural() const { return l * ex2(-off()); }
   // Whatever the values: +inf counts alone, -inf nothing.
   template <int NV>
   __device__ __noinline__ void add_any(const float (&v)[NV]) {
@@ -180,19 +190,22 @@ struct Sum {
 #pragma unroll
       for (int i = 0; i < NV; ++i) l += v[i] == INFINITY ? 1.f : 0.f;
     } else if (ref != INFINITY) {
-      if (top > ref) renew(top);
+      float s = natural();
+      if (top > ref) s *= ex2((ref - top) * kLog2e), ref = top, b = top * kLog2e;
       if (ref != -INFINITY)
 #pragma unroll
-        for (int i = 0; i < NV; ++i) l += ex2(fmaf(v[i], kLog2e, -b));
+        for (int i = 0; i < NV; ++i) s += ex2((v[i] - ref) * kLog2e);
+      l = s * ex2(off());
     }
+    limit = ordinary() ? ref + kLag : -INFINITY;
   }
   // Pieces of ordinary numbers with maximum `top`; false (and nothing added) where there
-  // are others.  Per number: half a multiply-add and half an addition (two at a time)
+  // are others, or were until now.  Per number: half a multiply-add and half an addition (two at a time)
   // and the exponential.
   template <typename T, int U>
   __device__ __forceinline__ bool add(const uint4 (&w)[U], float top) {
-    if (!(top <= ref + kLag)) {
-      if (!(fabsf(top) < INFINITY)) return false;
+    if (!(top <= limit)) {
+      if (!(fabsf(top) < kOrdinary) || !(ordinary() || ref == -INFINITY)) return false;
       renew(top);
     }
     const uint64_t c2 = pack2(kLog2e, kLog2e), b2 = pack2(-b, -b);
@@ -214,11 +227,11 @@ struct Sum {
   }
 };
 
-// Joins (b2, l2) into (b, l).
-__device__ __forceinline__ void join(float &b, float &l, float b2, float l2) {
-  const float m = fmaxf(b, b2);
-  l = l * (b == m ? 1.f : ex2(b - m)) + l2 * (b2 == m ? 1.f : ex2(b2 - m));
-  b = m;
+// Joins a sum l2 of e^(x - r2) into l, of e^(x - r).
+__device__ __forceinline__ void join(float &r, float &l, float r2, float l2) {
+  const float m = fmaxf(r, r2);
+  l = l * (r == m ? 1.f : ex2((r - m) * kLog2e)) + l2 * (r2 == m ? 1.f : ex2((r2 - m) * kLog2e));
+  r = m;
 }
 
 __device__ __forceinline__ bool before(uint32_t k1, int t1, uint32_t k2, int t2) {
@@ -333,10 +346,10 @@ __global__ void __launch_bounds__(kS, kScanCtas) beam_scan_kernel(ScanArgs a) {
   const bool any = lo + tid < hi;
   const uint32_t key = any ? key_of(top) : 0u;
   tops[tid] = key;
+  float r = sum.ref, l = sum.natural();
 #pragma unroll
-  for (int d = 16; d; d >>= 1)
-    join(sum.b, sum.l, __shfl_xor_sync(0xffffffffu, sum.b, d), __shfl_xor_sync(0xffffffffu, sum.l, d));
-  if (lane == 0) part[warp] = make_float2(sum.b, sum.l);
+  for (int d = 16; d; d >>= 1) join(r, l, __shfl_xor_sync(0xffffffffu, r, d), __shfl_xor_sync(0xffffffffu, l, d));
+  if (lane == 0) part[warp] = make_float2(r, l);
   __syncthreads();
   if (warp == 0) {
     // A bound that at least n thread maxima, and so n logits, reach, by one warp (every
@@ -370,9 +383,9 @@ __global__ void __launch_bounds__(kS, kScanCtas) beam_scan_kernel(ScanArgs a) {
     }
     if (lane == 0) bound_s = bound;
   } else if (tid == 32) {
-    float b = part[0].x, l = part[0].y;
-    for (int w = 1; w < W; ++w) join(b, l, part[w].x, part[w].y);
-    a.stats[static_cast<int64_t>(row) * a.chunks + chunk] = make_float2(b, l);
+    r = part[0].x, l = part[0].y;
+    for (int w = 1; w < W; ++w) join(r, l, part[w].x, part[w].y);
+    a.stats[static_cast<int64_t>(row) * a.chunks + chunk] = make_float2(r, l);
   }
   __syncthreads();
   const uint32_t bound = bound_s;
@@ -460,8 +473,8 @@ __host__ __device__ constexpr int round4(int v) { return (v + 3) / 4 * 4; }
 
 // A beam as the merge needs it.
 struct Beam {
-  double log_sum;  // log of the row's sum of e^(x - b / c) (see ScanArgs::stats)
-  float b;
+  double log_sum;  // log of the row's sum of e^(x - r) (see ScanArgs::stats)
+  float r;
   float score;     // so far
   int ended;
 };
@@ -492,14 +505,14 @@ __global__ void __launch_bounds__(kT) beam_merge_kernel(MergeArgs a) {
       const int64_t row = static_cast<int64_t>(b) * a.beams + k;
       const float score = a.scores[row];
       const int ended = a.finished ? a.finished[row] : 0;
-      float sb = -INFINITY, sl = 0.f;
+      float sr = -INFINITY, sl = 0.f;
       for (int c = lane; c < a.chunks; c += 32) {
         const float2 s = a.stats[row * a.chunks + c];
-        join(sb, sl, s.x, s.y);
+        join(sr, sl, s.x, s.y);
       }
       for (int d = 1; d < a.chunks && d < 32; d <<= 1)
-        join(sb, sl, __shfl_xor_sync(0xffffffffu, sb, d), __shfl_xor_sync(0xffffffffu, sl, d));
-      if (lane == 0) beams[k] = Beam{log(static_cast<double>(sl)), sb, score, ended};
+        join(sr, sl, __shfl_xor_sync(0xffffffffu, sr, d), __shfl_xor_sync(0xffffffffu, sl, d));
+      if (lane == 0) beams[k] = Beam{log(static_cast<double>(sl)), sr, score, ended};
     }
   };
   const bool apart = a.beams <= kT / 64 && group == a.beams;
@@ -585,8 +598,8 @@ __global__ void __launch_bounds__(kT) beam_merge_kernel(MergeArgs a) {
   for (int k = tid >> 5; k < a.beams; k += kT / 32) {
     const Beam x = beams[k];
     const float top = value_of(key[k * a.n]);
-    const double shift = top == INFINITY ? 0.0 : static_cast<double>(x.b) - static_cast<double>(top) * kLog2e;
-    const float log_sum = static_cast<float>(shift * 0.6931471805599453 + x.log_sum);
+    const double shift = x.r == top ? 0.0 : static_cast<double>(x.r) - static_cast<double>(top);
+    const float log_sum = static_cast<float>(shift + x.log_sum);
     __syncwarp();
     for (int j = lane; j < a.n; j += 32) {
       const float v = value_of(key[k * a.n + j]);
