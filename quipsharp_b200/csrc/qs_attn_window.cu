@@ -666,7 +666,8 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       const int token = j.t0 + t * w.tokens_per_tile + tok;
       const bool real = tok < w.tokens_per_tile && token < j.q1;
       const int pos = j.pos0 + t * w.tokens_per_tile + tok;
-      // keys seen: k <= pos, and k > pos - window or k < sinks
+      // keys seen: k <= pos, where the row's line has so many, and k > pos - window or k < sinks
+      const int last = min(pos, j.keys - 1);
       const int low = static_cast<int>(max(static_cast<int64_t>(-1), pos - win));  // keys above it are recent
       float m = -INFINITY, l = 0.f;  // m in the units of S
       for (int i = 0; i < n; ++i) {
@@ -740,7 +741,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         // of 32 keys from b on, what the row does not see becomes -inf: as bits, the places up
         // to hi that are above lo or below sk
         auto mask = [&](float *s, int b) {
-          const int hi = pos - k0, lo = low - k0, sk = sinks - k0;
+          const int hi = last - k0, lo = low - k0, sk = sinks - k0;
           uint32_t see = ones_below(hi + 1 - b) & (~ones_below(lo + 1 - b) | ones_below(sk - b));
           const uint32_t gone = span >> (kGaps + b / 16);
           see &= ~((gone & 1u ? 0xffffu : 0u) | (gone & 2u ? 0xffff0000u : 0u));
