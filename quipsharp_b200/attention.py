@@ -92,9 +92,7 @@ def window_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor,
     q (tokens, q_heads, dim) packed: row r's tokens are [cu[r], cu[r+1]) (cu int32
     (rows + 1,)) and take its last places, which `lengths` counts and whose keys
     and values are already in the cache; everything else as in decode_attention.
-    Up to 128 query heads share a key head.  Values that are infinite or NaN are
-    only kept from tokens that do not see them where no token of the same tile
-    does (places past a row's length never enter)."""
+    Up to 128 query heads share a key head."""
     got = N.fast().attend(q, k_pages, v_pages, table, lengths, cu, window, sinks, scale, return_lse)
     if got is not None:
         return got

@@ -192,6 +192,18 @@ constexpr uint32_t idesc_of(int n, bool b_mn_major) {
   return sm100::idesc_f16_f32(kTile, n) | (f << 7) | (f << 10) | ((b_mn_major ? 1u : 0u) << 16);
 }
 
+// Whether a word of two values holds an infinity or NaN.
+template <typename T>
+__device__ __forceinline__ bool strange(uint32_t w) {
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  return (w & e) == e || (w >> 16 & e) == e;
+}
+template <typename T>
+__device__ __forceinline__ float2 floats_of(uint32_t w) {
+  if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+  else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&w));
+}
+
 // The lowest n bits (none for n <= 0, all for n >= 32).
 __device__ __forceinline__ uint32_t ones_below(int n) {
   return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u;
@@ -814,6 +826,99 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         }
         __syncwarp();
       };
+      // A value that a row does not see has weight 0 in it, and 0 x inf is NaN.  So the rows
+      // whose sums are not finite (`test`: 0 for the others) are summed again, key by key,
+      // by the whole warp, if a key of their tiles that they do not see has such a value.
+      uint64_t test = 0;
+      auto look = [&](uint32_t x, uint32_t y) { test = fma2(pack2(__uint_as_float(x), __uint_as_float(y)), 0, test); };
+      auto amend = [&] {
+        const float2 z = unpack2(test);
+        uint32_t bad = __ballot_sync(0xffffffffu, real && l < INFINITY && !(z.x + z.y == 0.f));
+        constexpr int PER = DP / 32;  // outputs per lane
+        const int *table = a.table + static_cast<int64_t>(j.row) * a.width;
+        const int kvh = j.head, pieces = a.dim / 8;
+        while (bad) {
+          const int who = __ffs(bad) - 1;
+          bad &= bad - 1;
+          const int last_r = __shfl_sync(0xffffffffu, last, who), low_r = __shfl_sync(0xffffffffu, low, who);
+          const float m_r = __shfl_sync(0xffffffffu, m, who), l_r = __shfl_sync(0xffffffffu, l, who);
+          const int64_t at_r = __shfl_sync(0xffffffffu, at, who);
+          // the page of a key of the row's tiles, -1 where there is none
+          auto page_of = [&](int key) {
+            if (key >= j.keys) return -1;
+            const int p = table[key >> a.page_shift];
+            return p >= 0 && p < a.pages ? p : -1;
+          };
+          auto place = [&](const void *pool, const int64_t (&st)[3], int page, int key) {
+            return static_cast<const T *>(pool) + page * st[0] + kvh * st[1] + (key & ((1 << a.page_shift) - 1)) * st[2];
+          };
+          auto seen = [&](int key) { return key <= last_r && (key > low_r || key < sinks); };
+          bool unseen = false;
+          for (int i = 0; i < n; ++i)
+#pragma unroll 1
+            for (int key = key_of_tile(j, i) + lane, end = key + kTile; key < end; key += 32) {
+              const int page = seen(key) ? -1 : page_of(key);
+              if (page < 0) continue;
+              const uint4 *v = reinterpret_cast<const uint4 *>(place(a.v, a.vs, page, key));
+#pragma unroll 1
+              for (int c = 0; c < pieces; ++c)
+                unseen |= strange<T>(v[c].x) || strange<T>(v[c].y) || strange<T>(v[c].z) || strange<T>(v[c].w);
+            }
+          if (!__any_sync(0xffffffffu, unseen)) continue;
+          const int64_t token_r = at_r / a.q_heads;
+          const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + token_r * a.q_token +
+                                                           (at_r - token_r * a.q_heads) * a.q_head);
+          const float shift = m_r == -INFINITY ? 0.f : kBias - m_r * scale2;
+          float o[PER] = {};
+          for (int i = 0; i < n; ++i)
+#pragma unroll 1
+            for (int key = key_of_tile(j, i) + lane, end = key + kTile; key < end; key += 32) {
+              const int page = seen(key) ? page_of(key) : -1;
+              float p = 0.f;
+              if (page >= 0) {
+                const uint4 *k = reinterpret_cast<const uint4 *>(place(a.k, a.ks, page, key));
+                float dot = 0.f;
+#pragma unroll 1
+                for (int c = 0; c < pieces; ++c) {
+                  const uint4 x = q[c], y = k[c];
+                  auto add = [&](uint32_t s, uint32_t t) {
+                    const float2 f = floats_of<T>(s), g = floats_of<T>(t);
+                    dot = fmaf(f.x, g.x, fmaf(f.y, g.y, dot));
+                  };
+                  add(x.x, y.x), add(x.y, y.y), add(x.z, y.z), add(x.w, y.w);
+                }
+                p = ex2(fmaf(dot, scale2, shift));
+              }
+              uint32_t some = __ballot_sync(0xffffffffu, page >= 0);
+              while (some) {
+                const int of = __ffs(some) - 1;
+                some &= some - 1;
+                const float pk = __shfl_sync(0xffffffffu, p, of);
+                const T *v = place(a.v, a.vs, __shfl_sync(0xffffffffu, page, of), key - lane + of) + lane * PER;
+                if (lane * PER < a.dim)
+#pragma unroll
+                  for (int c = 0; c < PER; c += 2) {
+                    const float2 f = floats_of<T>(*reinterpret_cast<const uint32_t *>(v + c));
+                    o[c] = fmaf(pk, f.x, o[c]);
+                    o[c + 1] = fmaf(pk, f.y, o[c + 1]);
+                  }
+              }
+            }
+          const float inv_r = l_r == 0.f ? 0.f : 1.f / l_r;
+          if (lane * PER < a.dim)
+#pragma unroll
+            for (int c = 0; c < PER; c += 2) {
+              if (w.splits > 1) {
+                float *to = w.part_o + (j.split * a.tokens * a.q_heads + at_r) * DP + lane * PER + c;
+                to[0] = o[c], to[1] = o[c + 1];
+              } else {
+                uint32_t packed;
+                split16<T>(o[c] * inv_r, o[c + 1] * inv_r, packed);
+                *reinterpret_cast<uint32_t *>(static_cast<T *>(a.out) + at_r * a.dim + lane * PER + c) = packed;
+              }
+            }
+        }
+      };
       if (w.splits > 1) {
         const int64_t base = j.split * a.tokens * a.q_heads;
 #pragma unroll
@@ -821,8 +926,11 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           uint32_t o[32];
           tmem_ld_32(o_at + c, o);
           sm100::tmem_ld_wait();
+#pragma unroll
+          for (int x = 0; x < 32; x += 2) look(o[x], o[x + 1]);
           send(o, reinterpret_cast<char *>(w.part_o + base * DP + c), DP * 4, 128);
         }
+        amend();
         if (real) w.part_ml[base + at] = make_float2(m == -INFINITY ? -INFINITY : m * scale2 - kBias, l);
         sm100::tc_fence_before_sync();
         continue;
@@ -834,10 +942,13 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         tmem_ld_32(o_at + c + 32, o + 32);
         sm100::tmem_ld_wait();
 #pragma unroll
+        for (int x = 0; x < 64; x += 2) look(o[x], o[x + 1]);
+#pragma unroll
         for (int x = 0; x < 32; ++x)
           split16<T>(__uint_as_float(o[2 * x]) * inv, __uint_as_float(o[2 * x + 1]) * inv, o[x]);
         send(o, reinterpret_cast<char *>(static_cast<T *>(a.out) + c), a.dim * 2, (a.dim - c) * 2);
       }
+      amend();
       sm100::tc_fence_before_sync();  // O is read: the next job's first weights release it
       if (real && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : (m * scale2 - kBias) * kLn2) + logf(l);
     }

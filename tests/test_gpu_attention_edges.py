@@ -56,3 +56,36 @@ def bounded(q, k, v, table, lengths, held, new, window, sinks):
         parts.append((torch.einsum("htn,nhd->thd", p, vv), lse.T, torch.einsum("htn,nhd->thd", p, vv.abs())))
         i += t
     return [torch.cat(x) for x in zip(*parts)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("new,past,q_heads,kv_heads,page,dim,window,sinks,bad", [
+    ([300, 40], [0, 77], 8, 2, 16, 64, 0, 0, [[0, 5, 130, 131, 299], [80, 116]]),   # seen by later tokens alone
+    ([200], [300], 14, 2, 128, 80, 0, 0, [[310, 499]]),
+    ([600, 9], [0, 800], 8, 1, 16, 128, 100, 4, [[4, 3, 250, 599], [2, 50, 650, 704, 805]]),  # before, after and between
+    ([5], [5000], 4, 1, 64, 64, 100, 4, [[4, 50, 100, 4890, 4903]]),                # few tokens: shares of the keys
+    ([3, 2], [9000, 40], 6, 2, 32, 96, 0, 0, [[9001, 9002], [41]]),
+    ([130], [20], 128, 1, 32, 64, 33, 1, [[1, 60, 149]])])
+def test_values_that_a_token_does_not_see_do_not_enter(new, past, q_heads, kv_heads, page, dim, window, sinks, bad, dtype):
+    """NaN and infinite values of a key reach the tokens that see it, in their dimension,
+    and no others: not those of the same tile either."""
+    rs = np.random.RandomState(sum(new))
+    k, v, table, n = make(rs, [a + b for a, b in zip(new, past)], kv_heads, page, dim, dtype, junk=float("nan"))
+    q = torch.randn(sum(new), q_heads, dim, device=DEV).to(dtype)
+    want = exact(q, k, v, table, n, new, window, sinks)
+    hit = torch.zeros(sum(new), dim, dtype=torch.bool, device=DEV)
+    start = 0
+    for r, places in enumerate(bad):
+        pos = past[r] + torch.arange(new[r], device=DEV)
+        for i, place in enumerate(places):
+            d = (7 * i + 3) % dim
+            v[int(table[r, place // page]), :, place % page, d] = (float("nan"), float("inf"), -float("inf"))[i % 3]
+            see = (place <= pos) & ((place > pos - window) | (place < sinks) if window else True)
+            hit[start:start + new[r], d] |= see
+        start += new[r]
+    out, lse = at.window_attention(q, k, v, table, n, offsets(new), window=window or None, sinks=sinks, return_lse=True)
+    hit = hit[:, None].expand(-1, q_heads, -1)
+    assert not out[hit].isfinite().any()
+    check((out.masked_fill(hit, 0), lse), (want[0].masked_fill(hit, 0), want[1], want[2]), dtype, weights=True)
+    again = at.window_attention(q, k, v, table, n, offsets(new), window=window or None, sinks=sinks)
+    assert torch.equal(again.masked_fill(hit, 0), out.masked_fill(hit, 0))
