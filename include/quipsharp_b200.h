@@ -394,7 +394,7 @@ int qs_cache_extend(int64_t page, int64_t pages, int64_t rows, int64_t width, co
  * v are (tokens, heads, dim) of the pool's type, packed by row; row r's are
  * [cu[r], cu[r+1]) and take its last places (lengths already count them).  cu
  * NULL: one token per row.  Strides in elements, multiples of 8.  Tokens whose
- * page is absent are left out. */
+ * page is absent, and those before cu[0] or past cu[rows], are left out. */
 int qs_cache_write(const qs_kv_pool *pool, int64_t rows, int64_t width, const int *table, const int *lengths,
                    const int *cu, const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v,
                    int64_t v_token_stride, int64_t v_head_stride, int64_t tokens, qs_stream_t stream);

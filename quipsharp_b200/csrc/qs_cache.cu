@@ -440,7 +440,7 @@ struct WriteArgs {
 };
 
 // A warp per token: its place is its row's length before the call plus its number
-// among the row's new tokens.  Tokens without a page are left out.
+// among the row's new tokens.  Tokens without a page, or of no row, are left out.
 __global__ void __launch_bounds__(256) write_kernel(WriteArgs a) {
   pdl_wait();
   pdl_launch_dependents();
@@ -459,7 +459,10 @@ __global__ void __launch_bounds__(256) write_kernel(WriteArgs a) {
       n = min(step - 1, end - lo);
     }
     row = min(lo, a.rows);
-    if (row < a.rows) back = a.cu[row + 1] - tok;
+    if (row < a.rows) {
+      if (tok < a.cu[row]) return;  // before the first row's
+      back = a.cu[row + 1] - tok;
+    }
   }
   if (row >= a.rows) return;
   const int pos = a.lengths[row] - back;

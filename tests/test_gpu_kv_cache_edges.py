@@ -1,0 +1,29 @@
+"""Page moves of the key-value cache at the edges of what tables and arguments may hold."""
+import numpy as np
+import pytest
+import torch
+
+from quipsharp_b200 import kv_cache as kc
+from test_gpu_kv_cache import DEV, on, same
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("first", [1, 3, 40])
+def test_write_leaves_out_tokens_before_the_first_row(first):
+    """cu[0] > 0, as of a slice of a larger batch: the tokens before it belong to no row, and
+    what the cache held stays."""
+    page = 16
+    g = torch.Generator(device=DEV).manual_seed(first)
+    k, v = (torch.randn(6, 2, page, 8, generator=g, device=DEV).half() for _ in range(2))
+    kn, vn = (torch.randn(first + 9, 2, 8, generator=g, device=DEV).half() for _ in range(2))
+    table, lengths, cu = on(np.array([[4, 1], [2, 5]], np.int32), np.array([22, 7], np.int32),
+                            np.array([first, first + 5, first + 9], np.int32))
+    wk, wv = k.clone(), v.clone()
+    for w, new in ((wk, kn), (wv, vn)):
+        for row, n, at, count in ((0, 22, first, 5), (1, 7, first + 5, 4)):
+            for j in range(count):
+                pos = n - count + j
+                w[int(table[row, pos // page]), :, pos % page] = new[at + j]
+    kc.write_kv(kn, vn, k, v, table, lengths, cu)
+    same(k, wk.cpu(), "keys"), same(v, wv.cpu(), "values")
