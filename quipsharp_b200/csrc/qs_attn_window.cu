@@ -40,8 +40,9 @@
 // around two bodies of them, or one that leaves out tiles that nothing sees, cost the
 // issuing warp more than the smaller tiles save: chunks 89 us).
 //
-// Warps: 0 loads, 1 issues the products (2 and 3 only fill their warpgroup), then four
-// per query tile for the softmax, to which the first four leave most of the registers.
+// Warps: 0 loads, 1 issues the products, 2 and 3 sum rows again where an unseen value spoilt
+// them (see amend_row), then four per query tile for the softmax, to which the first four
+// leave most of the registers.
 #include <cuda.h>
 
 #include <cmath>
@@ -71,7 +72,7 @@ struct Cfg {
   static constexpr int stages = room > 8 ? 8 : room;
   static constexpr int threads = 128 + NQ * 128;
   static constexpr int tmem_cols = NQ * (kTile + DP) <= 256 ? 256 : 512;
-  static constexpr int bars = 3 * stages + 5 * NQ + 8;
+  static constexpr int bars = 3 * stages + 5 * NQ + 10;
   static constexpr int smem = (NQ + stages) * tile_bytes + out_bytes + bars * 8 + 16 + 1024;
 };
 
@@ -354,6 +355,117 @@ __device__ __forceinline__ uint32_t span_of(const WindowArgs &w, const Job &j, i
   return gaps << kGaps | (tokens <= 0 || hi <= lo * 32 + 64 ? kNarrow | lo << kFrom : 0u);
 }
 
+// Key `key` (from 0) of the job's key tile i, in tile order.
+__device__ __forceinline__ int first_key(const Job &j, int i) {
+  i += j.first;
+  return i < j.sink_tiles ? i * kTile : j.from + (i - j.sink_tiles) * kTile;
+}
+
+// A value that a row does not see has weight 0 in its sum, and 0 x inf is NaN.  So a row
+// (r of query tile t) whose sum is not finite is summed again, key by key, by a whole warp, if
+// a key of its tiles that it does not see has an infinite or NaN value.  By a warp that has
+// nothing else to do: in the softmax warps' epilogue the same code took registers from their
+// loop (a prompt of 8192 tokens 968 -> 1022 us).
+template <typename T, int DP>
+__device__ __forceinline__ void amend_row(const WindowArgs &w, const Job &j, int t, int r, int lane) {
+  constexpr int PER = DP / 32;  // outputs per lane
+  const AttnArgs &a = w.a;
+  const int ahead = t * w.tokens_per_tile + r / w.share, token = j.t0 + ahead, pos = j.pos0 + ahead;
+  const int last = min(pos, j.keys - 1);
+  const int low = a.window > 0 && pos > a.window ? static_cast<int>(pos - a.window) : -1;
+  const int head = j.head * w.share + r % w.share, pieces = a.dim / 8, slots = (1 << a.page_shift) - 1;
+  const int *table = a.table + static_cast<int64_t>(j.row) * a.width;
+  auto seen = [&](int key) { return key <= last && (key > low || key < a.sinks); };
+  auto page_of = [&](int key) {  // -1 where there is none
+    if (key >= j.keys) return -1;
+    const int p = table[key >> a.page_shift];
+    return p >= 0 && p < a.pages ? p : -1;
+  };
+  const T *keys = static_cast<const T *>(a.k) + j.head * a.ks[1], *values = static_cast<const T *>(a.v) + j.head * a.vs[1];
+  bool unseen = false;
+  for (int i = 0; i < j.tiles; ++i) {
+    const int k0 = first_key(j, i);
+#pragma unroll 1
+    for (int key = k0 + lane; key < k0 + kTile; key += 32) {
+      const int page = seen(key) ? -1 : page_of(key);
+      if (page < 0) continue;
+      const uint4 *v = reinterpret_cast<const uint4 *>(values + page * a.vs[0] + (key & slots) * a.vs[2]);
+#pragma unroll 1
+      for (int c = 0; c < pieces; ++c) {
+        const uint4 x = v[c];
+        unseen |= strange<T>(x.x) || strange<T>(x.y) || strange<T>(x.z) || strange<T>(x.w);
+      }
+    }
+  }
+  if (!__any_sync(0xffffffffu, unseen)) return;  // the row sees what is not finite
+  const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + token * a.q_token + head * a.q_head);
+  const float scale2 = a.scale * kLog2e;
+  float m = -INFINITY, l = 0.f, o[PER] = {};
+  for (int i = 0; i < j.tiles; ++i) {
+    const int k0 = first_key(j, i);
+#pragma unroll 1
+    for (int key = k0 + lane; key < k0 + kTile; key += 32) {  // the same number of turns for every lane
+      const int page = seen(key) ? page_of(key) : -1;
+      float s = -INFINITY;
+      if (page >= 0) {
+        const uint4 *k = reinterpret_cast<const uint4 *>(keys + page * a.ks[0] + (key & slots) * a.ks[2]);
+        float dot = 0.f;
+#pragma unroll 1
+        for (int c = 0; c < pieces; ++c) {
+          const uint4 x = q[c], y = k[c];
+          auto add = [&](uint32_t u, uint32_t v) {
+            const float2 f = floats_of<T>(u), g = floats_of<T>(v);
+            dot = fmaf(f.x, g.x, fmaf(f.y, g.y, dot));
+          };
+          add(x.x, y.x), add(x.y, y.y), add(x.z, y.z), add(x.w, y.w);
+        }
+        s = dot * scale2;
+      }
+      float top = s;
+#pragma unroll
+      for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      if (top > m) {
+        const float f = ex2(m - top);
+        l *= f;
+#pragma unroll
+        for (int c = 0; c < PER; ++c) o[c] *= f;
+        m = top;
+      }
+      const float p = s == -INFINITY ? 0.f : ex2(s - m);
+      l += p;
+      for (uint32_t some = __ballot_sync(0xffffffffu, page >= 0); some; some &= some - 1) {
+        const int of = __ffs(some) - 1;
+        const float pk = __shfl_sync(0xffffffffu, p, of);
+        const T *v = values + __shfl_sync(0xffffffffu, page, of) * a.vs[0] + ((key - lane + of) & slots) * a.vs[2] + lane * PER;
+        if (lane * PER < a.dim)
+#pragma unroll
+          for (int c = 0; c < PER; c += 2) {
+            const float2 f = floats_of<T>(*reinterpret_cast<const uint32_t *>(v + c));
+            o[c] = fmaf(pk, f.x, o[c]);
+            o[c + 1] = fmaf(pk, f.y, o[c + 1]);
+          }
+      }
+    }
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+  const int64_t at = static_cast<int64_t>(token) * a.q_heads + head;
+  if (w.splits > 1) {
+    const int64_t to = j.split * a.tokens * a.q_heads + at;
+#pragma unroll
+    for (int c = 0; c < PER; ++c) w.part_o[to * DP + lane * PER + c] = o[c];
+    if (lane == 0) w.part_ml[to] = make_float2(m, l);
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int c = 0; c < PER; c += 2) {
+    uint32_t packed;
+    split16<T>(o[c] * inv, o[c + 1] * inv, packed);
+    if (lane * PER < a.dim) *reinterpret_cast<uint32_t *>(static_cast<T *>(a.out) + at * a.dim + lane * PER + c) = packed;
+  }
+}
+
 template <typename T, int DP, int NQ>
 __global__ void __launch_bounds__(Cfg<DP, NQ>::threads, 1)
 attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
@@ -366,6 +478,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   static_assert(kSpans >= S / 2 + 3, "loads run ahead by half the ring");
   __shared__ uint32_t spans[kSpans][NQ];  // of the last key tiles
   __shared__ __align__(16) uint8_t answer_s[16];
+  __shared__ uint32_t bads[2][NQ * 4];  // a job's rows whose sums are not finite, by softmax warp
   const AttnArgs &a = w.a;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   uint8_t *base = dsm + ((1024u - (smem_u32(dsm) & 1023u)) & 1023u);
@@ -382,6 +495,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   auto job_full = [&](int s) { return bar0 + 8u * (3 * S + 5 * NQ + s); };
   auto job_empty = [&](int s) { return bar0 + 8u * (3 * S + 5 * NQ + 2 + s); };
   const uint32_t q_full = bar0 + 8u * (3 * S + 5 * NQ + 4), q_empty = q_full + 8, asked = q_full + 16, drain = q_full + 24;
+  auto summed = [&](int s) { return q_full + 32 + 8u * s; };  // a job's outputs are stored
   uint32_t *holder = reinterpret_cast<uint32_t *>(base + (NQ + S) * C::tile_bytes + C::out_bytes + C::bars * 8);
 
   if (tid == 0) {
@@ -399,7 +513,8 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     }
     for (int s = 0; s < 2; ++s) {
       sm100::mbar_init(job_full(s), 1);
-      sm100::mbar_init(job_empty(s), 1 + NQ * 128);
+      sm100::mbar_init(job_empty(s), 3 + NQ * 128);
+      sm100::mbar_init(summed(s), NQ * 4);
     }
     sm100::mbar_init(q_full, 1);
     sm100::mbar_init(q_empty, 1);
@@ -638,6 +753,29 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       if (!ok) *w.error = 1;
       commit(drain);
       if (!sm100::mbar_wait_warp(drain, 0, kDrainNs)) *w.error = 1;
+    } else {
+      // ---- rows to be summed again, every second softmax warp's each
+      bool ok = true;
+      uint32_t summed_phase = 0;
+      for (int num = 0; ok; ++num) {
+        const int slot = num & 1;
+        ok = sm100::mbar_wait_warp(job_full(slot), (num >> 1) & 1, w.wait_ns);
+        if (!ok) break;
+        const int n = __shfl_sync(0xffffffffu, jobs[slot].tiles, 0);
+        if (n < 0) break;
+        if (n > 0) {
+          ok = sm100::mbar_wait_warp(summed(slot), (summed_phase >> slot) & 1, w.wait_ns);
+          summed_phase ^= 1u << slot;
+          if (!ok) break;
+          for (int from = warp - 2; from < NQ * 4; from += 2) {
+            uint32_t bad = *const_cast<volatile uint32_t *>(&bads[slot][from]);
+            for (; bad; bad &= bad - 1) amend_row<T, DP>(w, jobs[slot], from >> 2, (from & 3) * 32 + __ffs(bad) - 1, lane);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) sm100::mbar_arrive(job_empty(slot));
+      }
+      if (!ok) *w.error = 1;
     }
   } else {
     if (NQ == 2) registers_up<216>();
@@ -826,97 +964,19 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         }
         __syncwarp();
       };
-      // A value that a row does not see has weight 0 in it, and 0 x inf is NaN.  So the rows
-      // whose sums are not finite (`test`: 0 for the others) are summed again, key by key,
-      // by the whole warp, if a key of their tiles that they do not see has such a value.
-      uint64_t test = 0;
-      auto look = [&](uint32_t x, uint32_t y) { test = fma2(pack2(__uint_as_float(x), __uint_as_float(y)), 0, test); };
-      auto amend = [&] {
-        const float2 z = unpack2(test);
-        uint32_t bad = __ballot_sync(0xffffffffu, real && l < INFINITY && !(z.x + z.y == 0.f));
-        constexpr int PER = DP / 32;  // outputs per lane
-        const int *table = a.table + static_cast<int64_t>(j.row) * a.width;
-        const int kvh = j.head, pieces = a.dim / 8;
-        while (bad) {
-          const int who = __ffs(bad) - 1;
-          bad &= bad - 1;
-          const int last_r = __shfl_sync(0xffffffffu, last, who), low_r = __shfl_sync(0xffffffffu, low, who);
-          const float m_r = __shfl_sync(0xffffffffu, m, who), l_r = __shfl_sync(0xffffffffu, l, who);
-          const int64_t at_r = __shfl_sync(0xffffffffu, at, who);
-          // the page of a key of the row's tiles, -1 where there is none
-          auto page_of = [&](int key) {
-            if (key >= j.keys) return -1;
-            const int p = table[key >> a.page_shift];
-            return p >= 0 && p < a.pages ? p : -1;
-          };
-          auto place = [&](const void *pool, const int64_t (&st)[3], int page, int key) {
-            return static_cast<const T *>(pool) + page * st[0] + kvh * st[1] + (key & ((1 << a.page_shift) - 1)) * st[2];
-          };
-          auto seen = [&](int key) { return key <= last_r && (key > low_r || key < sinks); };
-          bool unseen = false;
-          for (int i = 0; i < n; ++i)
-#pragma unroll 1
-            for (int key = key_of_tile(j, i) + lane, end = key + kTile; key < end; key += 32) {
-              const int page = seen(key) ? -1 : page_of(key);
-              if (page < 0) continue;
-              const uint4 *v = reinterpret_cast<const uint4 *>(place(a.v, a.vs, page, key));
-#pragma unroll 1
-              for (int c = 0; c < pieces; ++c)
-                unseen |= strange<T>(v[c].x) || strange<T>(v[c].y) || strange<T>(v[c].z) || strange<T>(v[c].w);
-            }
-          if (!__any_sync(0xffffffffu, unseen)) continue;
-          const int64_t token_r = at_r / a.q_heads;
-          const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + token_r * a.q_token +
-                                                           (at_r - token_r * a.q_heads) * a.q_head);
-          const float shift = m_r == -INFINITY ? 0.f : kBias - m_r * scale2;
-          float o[PER] = {};
-          for (int i = 0; i < n; ++i)
-#pragma unroll 1
-            for (int key = key_of_tile(j, i) + lane, end = key + kTile; key < end; key += 32) {
-              const int page = seen(key) ? page_of(key) : -1;
-              float p = 0.f;
-              if (page >= 0) {
-                const uint4 *k = reinterpret_cast<const uint4 *>(place(a.k, a.ks, page, key));
-                float dot = 0.f;
-#pragma unroll 1
-                for (int c = 0; c < pieces; ++c) {
-                  const uint4 x = q[c], y = k[c];
-                  auto add = [&](uint32_t s, uint32_t t) {
-                    const float2 f = floats_of<T>(s), g = floats_of<T>(t);
-                    dot = fmaf(f.x, g.x, fmaf(f.y, g.y, dot));
-                  };
-                  add(x.x, y.x), add(x.y, y.y), add(x.z, y.z), add(x.w, y.w);
-                }
-                p = ex2(fmaf(dot, scale2, shift));
-              }
-              uint32_t some = __ballot_sync(0xffffffffu, page >= 0);
-              while (some) {
-                const int of = __ffs(some) - 1;
-                some &= some - 1;
-                const float pk = __shfl_sync(0xffffffffu, p, of);
-                const T *v = place(a.v, a.vs, __shfl_sync(0xffffffffu, page, of), key - lane + of) + lane * PER;
-                if (lane * PER < a.dim)
+      // whether the sums are finite: 0 times them is then 0 (see amend_row)
+      uint64_t test[4] = {};
+      auto look = [&](const uint32_t *o) {
 #pragma unroll
-                  for (int c = 0; c < PER; c += 2) {
-                    const float2 f = floats_of<T>(*reinterpret_cast<const uint32_t *>(v + c));
-                    o[c] = fmaf(pk, f.x, o[c]);
-                    o[c + 1] = fmaf(pk, f.y, o[c + 1]);
-                  }
-              }
-            }
-          const float inv_r = l_r == 0.f ? 0.f : 1.f / l_r;
-          if (lane * PER < a.dim)
-#pragma unroll
-            for (int c = 0; c < PER; c += 2) {
-              if (w.splits > 1) {
-                float *to = w.part_o + (j.split * a.tokens * a.q_heads + at_r) * DP + lane * PER + c;
-                to[0] = o[c], to[1] = o[c + 1];
-              } else {
-                uint32_t packed;
-                split16<T>(o[c] * inv_r, o[c + 1] * inv_r, packed);
-                *reinterpret_cast<uint32_t *>(static_cast<T *>(a.out) + at_r * a.dim + lane * PER + c) = packed;
-              }
-            }
+        for (int x = 0; x < 32; x += 2)
+          test[x / 2 % 4] = fma2(pack2(__uint_as_float(o[x]), __uint_as_float(o[x + 1])), 0, test[x / 2 % 4]);
+      };
+      auto report = [&] {
+        const float2 z = unpack2(add2(add2(test[0], test[1]), add2(test[2], test[3])));
+        const uint32_t bad = __ballot_sync(0xffffffffu, real && l < INFINITY && !(z.x + z.y == 0.f));
+        if (lane == 0) {
+          *const_cast<volatile uint32_t *>(&bads[slot][warp - 4]) = bad;
+          sm100::mbar_arrive(summed(slot));
         }
       };
       if (w.splits > 1) {
@@ -926,13 +986,13 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           uint32_t o[32];
           tmem_ld_32(o_at + c, o);
           sm100::tmem_ld_wait();
-#pragma unroll
-          for (int x = 0; x < 32; x += 2) look(o[x], o[x + 1]);
+          look(o);
           send(o, reinterpret_cast<char *>(w.part_o + base * DP + c), DP * 4, 128);
         }
-        amend();
         if (real) w.part_ml[base + at] = make_float2(m == -INFINITY ? -INFINITY : m * scale2 - kBias, l);
         sm100::tc_fence_before_sync();
+        __syncwarp();
+        report();
         continue;
       }
 #pragma unroll
@@ -941,16 +1001,17 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         tmem_ld_32(o_at + c, o);
         tmem_ld_32(o_at + c + 32, o + 32);
         sm100::tmem_ld_wait();
-#pragma unroll
-        for (int x = 0; x < 64; x += 2) look(o[x], o[x + 1]);
+        look(o);
+        look(o + 32);
 #pragma unroll
         for (int x = 0; x < 32; ++x)
           split16<T>(__uint_as_float(o[2 * x]) * inv, __uint_as_float(o[2 * x + 1]) * inv, o[x]);
         send(o, reinterpret_cast<char *>(static_cast<T *>(a.out) + c), a.dim * 2, (a.dim - c) * 2);
       }
-      amend();
       sm100::tc_fence_before_sync();  // O is read: the next job's first weights release it
       if (real && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : (m * scale2 - kBias) * kLn2) + logf(l);
+      __syncwarp();
+      report();
     }
     if (!ok) *w.error = 1;
   }
