@@ -420,7 +420,7 @@ int qs_attn_decode(const void *q, int64_t q_row_stride, int64_t q_head_stride, c
                    qs_stream_t stream);
 /* Many tokens per row, packed: row r's are [cu[r], cu[r+1]) of q (tokens, q_heads,
  * dim) and take its last places, their keys and values already written (lengths
- * count them).  Tokens past cu[rows] give 0. */
+ * count them).  Tokens before cu[0] and past cu[rows] give 0 (lse -inf). */
 int64_t qs_attn_window_workspace_bytes(int64_t tokens, int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t dim,
                                        int64_t page, int64_t width, int64_t window, int64_t sinks);
 int qs_attn_window(const void *q, int64_t q_token_stride, int64_t q_head_stride, const qs_kv_pool *pool,

@@ -214,8 +214,8 @@ __device__ __forceinline__ uint32_t ones_below(int n) {
 struct Job {
   int row;          // -1: none
   int head;         // key head
-  int q0, q1;       // the row's tokens in q
-  int t0;           // first token (in q)
+  int q0, q1;       // the row's tokens in q; without a row, those of all rows
+  int t0;           // first token (in q; without a row, counted over the tokens of no row)
   int pos0;         // its place in the row
   int keys;         // keys that any of the tokens sees end before this
   int sink_tiles;   // key tiles from 0
@@ -323,8 +323,11 @@ __device__ __forceinline__ Job job_of(const WindowArgs &w, int x, int y, int z, 
     const int all = j.sink_tiles + max(0, (j.keys - j.from + kTile - 1) / kTile);
     j.first = static_cast<int>(static_cast<int64_t>(all) * z / w.splits);
     j.tiles = static_cast<int>(static_cast<int64_t>(all) * (z + 1) / w.splits) - j.first;
-  } else {  // a block beyond the tiles clears its share of the tokens that belong to no row
-    j.t0 = end + want * per;
+  } else {  // a block beyond the tiles clears its share of the tokens that belong to no row:
+            // with ceil(tokens / per) blocks and one for each row with tokens there are enough
+    j.q0 = a.rows > 0 ? clampi(a.cu[0], 0, total_tokens) : 0;
+    j.q1 = end;
+    j.t0 = want * per;
     j.tiles = 0;
   }
   return j;
@@ -797,12 +800,13 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       const int n = j.tiles;
       if (n < 0) break;
       if (n == 0) {
-        const int total = static_cast<int>(a.tokens);
-        const int end = j.row >= 0 ? min(j.q1, j.t0 + per) : min(total, j.t0 + per);
-        const int count = max(0, end - j.t0) * w.share;
+        const int begin = jobs[slot].q0, held = jobs[slot].row >= 0 ? 0 : j.q1 - begin;  // tokens of the rows
+        const int end = jobs[slot].row >= 0 ? j.q1 : static_cast<int>(a.tokens) - held;
+        const int count = max(0, min(end - j.t0, per)) * w.share;
         for (int i = tid - 128; i < count * a.dim; i += NQ * 128) {
-          const int64_t at =
-              static_cast<int64_t>(j.t0 + i / a.dim / w.share) * a.q_heads + j.head * w.share + i / a.dim % w.share;
+          int token = j.t0 + i / a.dim / w.share;
+          if (token >= begin) token += held;
+          const int64_t at = static_cast<int64_t>(token) * a.q_heads + j.head * w.share + i / a.dim % w.share;
           if (w.splits > 1) {  // an empty share
             if (i % a.dim == 0) w.part_ml[j.split * a.tokens * a.q_heads + at] = make_float2(-INFINITY, 0.f);
             continue;

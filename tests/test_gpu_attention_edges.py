@@ -89,3 +89,22 @@ def test_values_that_a_token_does_not_see_do_not_enter(new, past, q_heads, kv_he
     check((out.masked_fill(hit, 0), lse), (want[0].masked_fill(hit, 0), want[1], want[2]), dtype, weights=True)
     again = at.window_attention(q, k, v, table, n, offsets(new), window=window or None, sinks=sinks)
     assert torch.equal(again.masked_fill(hit, 0), out.masked_fill(hit, 0))
+
+
+@pytest.mark.parametrize("first,new,past", [(1, [30, 15], [20, 5]), (300, [30, 15], [20, 5]), (45, [0, 200], [0, 7]),
+                                            (5, [1], [3000])])
+def test_tokens_before_the_first_row_are_zero(first, new, past):
+    """cu[0] > 0, as of a slice of a larger batch: the tokens before it belong to no row."""
+    rs = np.random.RandomState(first)
+    k, v, table, n = make(rs, [a + b for a, b in zip(new, past)], 2, 16, 64, torch.float16)
+    total = first + sum(new) + 33
+    q = torch.randn(total, 8, 64, device=DEV).half()
+    left = [torch.full(shape, float("nan"), device=DEV, dtype=t) for shape, t in
+            (((total, 8, 64), torch.float16), ((total, 8), torch.float32))]  # what the outputs' memory held
+    torch.cuda.synchronize()
+    del left
+    out, lse = at.window_attention(q, k, v, table, n, offsets(new, first), return_lse=True)
+    mine = slice(first, first + sum(new))
+    check((out[mine], lse[mine]), exact(q[mine], k, v, table, n, new, 0, 0), torch.float16, True)
+    for rest in (slice(0, first), slice(first + sum(new), total)):
+        assert not out[rest].any() and torch.isneginf(lse[rest]).all()
