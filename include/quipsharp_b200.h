@@ -367,10 +367,10 @@ int64_t qs_cache_workspace_bytes(int64_t rows, int64_t pages);
  * its pages are freed unless others hold them): fork, free and reorder in one.
  * Whole pages are shared.  A part-filled last page stays with the lowest child of
  * a row, and each other child gets the lowest free page, in row order, with the
- * filled tokens of all layers copied into it.  The new counts are the old ones
- * plus references after minus references before, taken before pages are handed
- * out, so pages freed by this call serve it.  The outputs must not overlap the
- * inputs.  A row that finds no free page gets -1 there (QS_ERR_PAGES from
+ * filled tokens of all layers copied into it (an absent one stays absent).  The
+ * new counts are the old ones plus references after minus references before,
+ * taken before pages are handed out, so pages freed by this call serve it.  The
+ * outputs must not overlap the inputs.  A row that finds no free page gets -1 there (QS_ERR_PAGES from
  * qs_device_status); a parent outside [-1, rows) makes an empty row
  * (QS_ERR_INDEX). */
 int qs_cache_fork(const qs_kv_pool *pool, int64_t rows, int64_t width, const int *table, const int *lengths,

@@ -196,8 +196,11 @@ __global__ void __launch_bounds__(kThreads, 1) fork_kernel(Tables t, const int *
     const int i = i0 + threadIdx.x;
     bool dup = false;
     if (i < t.rows && par[i] >= 0 && first[par[i]] != i) {
-      const int n = len[par[i]];
-      dup = (n & fill_mask) != 0 && (n >> t.page_shift) < t.width;
+      const int n = len[par[i]], c = n >> t.page_shift;
+      if ((n & fill_mask) != 0 && c < t.width) {
+        const int page = t.table[static_cast<int64_t>(par[i]) * t.width + c];
+        dup = page >= 0 && page < t.pages;  // an absent page is absent in every child
+      }
     }
     int n;
     const int r = want + block_prefix(dup ? 1 : 0, &n, tmp);

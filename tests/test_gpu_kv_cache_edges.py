@@ -27,3 +27,27 @@ def test_write_leaves_out_tokens_before_the_first_row(first):
                 w[int(table[row, pos // page]), :, pos % page] = new[at + j]
     kc.write_kv(kn, vn, k, v, table, lengths, cu)
     same(k, wk.cpu(), "keys"), same(v, wv.cpu(), "values")
+
+
+@pytest.mark.parametrize("rows,pages", [(4, 6), (4, 40000), (8000, 8000)])
+def test_children_of_a_row_whose_last_page_is_absent(rows, pages):
+    """A part-filled page that was never found (-1) is absent in every child: no page is taken
+    for it, and nothing becomes visible in its place."""
+    page = 16
+    k, v = (torch.randn(1, pages, 1, page, 8, device=DEV).half() for _ in range(2))
+    table = np.full((rows, 3), -1, np.int32)
+    table[0, 0], table[1, :2] = 2, (3, 0)
+    lengths = np.zeros(rows, np.int32)
+    lengths[:2] = 20, 25
+    refcount = np.zeros(pages, np.int32)
+    refcount[[2, 3, 0]] = 1
+    parents = np.full(rows, -1, np.int32)
+    parents[:4] = 0, 0, 1, 1
+    wk, wv = k.clone(), v.clone()
+    for w in (wk, wv):
+        w[:, 1, :, :9] = w[:, 0, :, :9]
+    t, n, c = kc.fork_pages(k, v, *on(table, lengths, refcount, parents))
+    assert t[:4].tolist() == [[2, -1, -1], [2, -1, -1], [3, 0, -1], [3, 1, -1]] and bool((t[4:] == -1).all())
+    assert n[:4].tolist() == [20, 20, 25, 25] and c[:6].tolist() == [1, 1, 2, 2, 0, 0] and int(c.sum()) == 6
+    same(k, wk.cpu(), "keys"), same(v, wv.cpu(), "values")
+    kc.check_device()
