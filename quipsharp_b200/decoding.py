@@ -11,6 +11,8 @@ reference leaves generation to transformers.
 """
 from __future__ import annotations
 
+import sys
+
 import torch
 from torch import Tensor, nn
 
@@ -25,12 +27,74 @@ def _rotate(x: Tensor, cos: Tensor, sin: Tensor) -> Tensor:
     return x * cos[:, None] + turned * sin[:, None]
 
 
+_PARTS = {"self_attn": ("q_proj", "k_proj", "v_proj", "o_proj"), "mlp": ("gate_proj", "up_proj", "down_proj")}
+# settings of a configuration under which a model of these names computes something else
+_SETTINGS = {"embedding_multiplier": 1, "residual_multiplier": 1, "logits_scaling": 1, "logit_scale": 1, "clip_qkv": None,
+             "attn_logit_softcapping": None, "final_logit_softcapping": None}
+
+
+def _refuse_other_models(model: nn.Module, dim: int, max_len: int, window: int | None) -> None:
+    """NotImplementedError for a model that has the Llama layout's names but more in it, or
+    something else behind them, so that PagedDecoder's outputs would not be the model's."""
+    def refuse(what):
+        raise NotImplementedError(f"PagedDecoder runs the Llama layout; this model has {what}")
+
+    config, inner = model.config, model.model
+    for name, plain in _SETTINGS.items():
+        if getattr(config, name, plain) not in (plain, None):
+            refuse(f"{name} = {getattr(config, name)}")
+    rope = getattr(config, "rope_parameters", None) or {}
+    if rope.get("llama_4_scaling_beta") and max_len > rope.get("original_max_position_embeddings", 0):
+        refuse("queries scaled by their position")
+    kinds, own = getattr(config, "layer_types", None), getattr(config, "sliding_window", None)
+    if set(kinds or ()) - {"full_attention", "sliding_attention"}:
+        refuse(f"layers of the types {sorted(set(kinds))}")
+    slides = "sliding_attention" in kinds if kinds else getattr(config, "use_sliding_window", True)
+    if own and slides and max_len > own and (window is None or window > own):
+        refuse(f"a sliding window of {own} tokens, less than max_len = {max_len}: give window={own}, or less")
+
+    weight = inner.embed_tokens.weight
+    acts = {}
+    for layer in inner.layers:
+        for module, names in ((layer, ("input_layernorm", "post_attention_layernorm", *_PARTS)),
+                              *((getattr(layer, part, None), names) for part, names in _PARTS.items())):
+            gone = [n for n in names if not hasattr(module, n)]
+            if gone:
+                refuse(f"no {', '.join(gone)}")
+            more = [n for n, _ in module.named_parameters(recurse=False)]
+            more += [n for n, m in module.named_children() if n not in names and any(True for _ in m.parameters())]
+            if more:
+                refuse(f"{', '.join(more)} in {type(module).__name__}")
+        attn, act = layer.self_attn, getattr(layer.mlp, "act_fn", None)
+        scaling = getattr(attn, "scaling", None)
+        if isinstance(scaling, (int, float)) and abs(scaling * dim ** 0.5 - 1) > 1e-6:
+            refuse(f"scores scaled by {scaling}")
+        if not getattr(attn, "use_rope", True):
+            refuse("layers without positions")
+        if callable(act):
+            acts[type(act)] = act
+    x = torch.linspace(-4, 4, 2 * dim, device=weight.device).view(1, 2, 1, dim)  # two heads of a token
+    for act in acts.values():
+        if not torch.allclose(act(x), nn.functional.silu(x), atol=1e-5):
+            refuse(f"the activation {act}")
+    cos, sin = inner.rotary_emb(x.new_zeros(1, 1, weight.shape[1]), torch.tensor([[5]], device=weight.device))
+    if cos.shape[-1] != dim:
+        refuse("positions on a part of a head's dimensions")
+    turn = getattr(sys.modules.get(type(attn).__module__), "apply_rotary_pos_emb", None)
+    if turn is not None and not torch.allclose(turn(x, x, cos, sin)[0], _rotate(x.transpose(1, 2)[0], cos[0], sin[0])[:, :, None],
+                                               atol=1e-5):
+        refuse("another pairing of dimensions in its rotary positions")
+
+
 class PagedDecoder:
     """A causal language model with its keys and values in pages, for `rows`
     sequences of up to `max_len` tokens.
 
     window and sinks: every token sees the last `window` tokens (None: all) and
-    the first `sinks`.  num_pages defaults to what all rows can fill."""
+    the first `sinks`.  num_pages defaults to what all rows can fill.  Models that
+    have the Llama layout's names but compute something else (norms of queries and
+    keys, other scales, activations or positions, a shorter window of their own)
+    are refused."""
 
     def __init__(self, model: nn.Module, rows: int, max_len: int, num_pages: int | None = None, page_size: int = 16,
                  window: int | None = None, sinks: int = 0):
@@ -40,6 +104,7 @@ class PagedDecoder:
         self.heads = config.num_attention_heads
         self.kv_heads = getattr(config, "num_key_value_heads", None) or self.heads
         self.dim = getattr(config, "head_dim", None) or config.hidden_size // self.heads
+        _refuse_other_models(model, self.dim, max_len, window)
         if num_pages is None:
             num_pages = rows * (-(-max_len // page_size) + 1)
         self.cache = PagedKVCache(len(self.layers), self.kv_heads, self.dim, num_pages, rows, max_len, page_size,
