@@ -135,6 +135,8 @@ class PagedDecoder:
             raise ValueError("prompts must not be empty and their rows ascending, one for each")
         device = self.cache.lengths.device
         new = [0] * len(self.cache.lengths)
+        if rows and not 0 <= rows[0] <= rows[-1] < len(new):
+            raise IndexError(f"rows go from 0 to {len(new) - 1}, got {list(rows)}")
         for r, p in zip(rows, prompts):
             new[r] = len(p)
         counts = torch.tensor(new, dtype=torch.int32)

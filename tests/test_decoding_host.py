@@ -1,4 +1,6 @@
 """Models and arguments that the paged decoder refuses (no GPU)."""
+from types import SimpleNamespace
+
 import pytest
 import torch
 import transformers
@@ -44,3 +46,18 @@ def test_models_that_compute_something_else_are_refused(name, change, options, w
 def test_models_of_the_layout_are_taken(name, change, options):
     with pytest.raises(RuntimeError, match="CUDA tensors only"):  # the cache, which comes next
         PagedDecoder(tiny(name, **change), 2, 100, **options)
+
+
+def bare(rows=3, vocab=10):
+    """A decoder with nothing behind it: what is refused is refused before anything runs."""
+    decoder = object.__new__(PagedDecoder)
+    decoder.cache = SimpleNamespace(lengths=torch.zeros(rows, dtype=torch.int32))
+    decoder.model = SimpleNamespace(model=SimpleNamespace(embed_tokens=torch.nn.Embedding(vocab, 8)))
+    return decoder
+
+
+@pytest.mark.parametrize("rows", [[-1, 0], [-2, -1], [0, 3], [1, 7]])
+def test_rows_that_are_not_there_are_refused(rows):
+    """Row -1 as Python counts it would take another row's prompt."""
+    with pytest.raises(IndexError):
+        bare().prompt([[1], [2]], rows)
