@@ -137,6 +137,9 @@ class PagedDecoder:
         new = [0] * len(self.cache.lengths)
         if rows and not 0 <= rows[0] <= rows[-1] < len(new):
             raise IndexError(f"rows go from 0 to {len(new) - 1}, got {list(rows)}")
+        vocab = self.model.model.embed_tokens.weight.shape[0]
+        if not all(0 <= t < vocab for p in prompts for t in p):  # the embedding would stop the device
+            raise IndexError(f"prompts hold tokens from 0 to {vocab - 1}")
         for r, p in zip(rows, prompts):
             new[r] = len(p)
         counts = torch.tensor(new, dtype=torch.int32)

@@ -61,3 +61,9 @@ def test_rows_that_are_not_there_are_refused(rows):
     """Row -1 as Python counts it would take another row's prompt."""
     with pytest.raises(IndexError):
         bare().prompt([[1], [2]], rows)
+
+
+@pytest.mark.parametrize("prompt", [[3, 10], [-1], [4, 1 << 40]])
+def test_tokens_that_are_not_there_are_refused(prompt):
+    with pytest.raises(IndexError, match="tokens from 0 to 9"):
+        bare().prompt([[1], prompt], [0, 1])
