@@ -184,6 +184,7 @@ def beam_search(model: nn.Module, prompts: list[list[int]], beams: int, new_toke
         history.append((parents, tokens))
         if eos is not None:
             ended = ended.gather(1, parents.long()) | (tokens == eos)
+            tokens = tokens.masked_fill(ended, 0)  # nothing reads their logits, and `pad` need not be a token
         if i + 1 == new_tokens:
             break
         decoder.cache.fork((parents + first[:, None]).flatten())
