@@ -599,8 +599,9 @@ template <typename T, int DP, bool R8, int W, bool WHOLE>
 int run(const AttnArgs &a, const Ws &ws, int blocks, int share, int64_t grid, cudaStream_t s, int ctas = 1) {
   auto kern = attn_decode_kernel<T, DP, R8, W, WHOLE>;
   constexpr int smem = static_cast<int>(sizeof(Smem<T, DP, W>));
-  static const cudaError_t attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (attr != cudaSuccess) return fail(QS_ERR_CUDA, "attention (decode): %s", cudaGetErrorString(attr));
+  static std::atomic<uint64_t> allowed{0};
+  const int st = allow_smem("attention (decode)", kern, smem, allowed);
+  if (st) return st;
   if (ctas > 1) return launch_clusters(kern, grid, ctas, W * 32, smem, s, a, ws, blocks, share);
   return launch_pdl("attention (decode)", kern, dim3(static_cast<unsigned>(grid)), dim3(W * 32), smem, s, a, ws, blocks,
                     share);

@@ -1117,8 +1117,9 @@ int run(const AttnArgs &a, cudaStream_t s) {
     if (e) return e;
   }
   auto kern = attn_window_kernel<T, DP, NQ>;
-  static const cudaError_t attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem);
-  if (attr != cudaSuccess) return fail(QS_ERR_CUDA, "attention (window): %s", cudaGetErrorString(attr));
+  static std::atomic<uint64_t> allowed{0};
+  int st = allow_smem("attention (window)", kern, C::smem, allowed);
+  if (st) return st;
   const int64_t per = static_cast<int64_t>(NQ) * w.tokens_per_tile;
   const int64_t rows = a.tokens * a.q_heads;
   w.splits = splits_for(a.tokens, a.rows, a.q_heads, a.kv_heads, page, a.width, a.window, a.sinks);
@@ -1126,7 +1127,7 @@ int run(const AttnArgs &a, cudaStream_t s) {
   w.part_ml = reinterpret_cast<float2 *>(w.part_o + w.splits * rows * DP);
   const int64_t most_rows = a.rows < a.tokens ? a.rows : a.tokens;  // that have a token
   const dim3 grid(static_cast<unsigned>(ceil_div(a.tokens, per) + most_rows), a.kv_heads, w.splits);
-  const int st = launch_pdl("attention (window)", kern, grid, dim3(C::threads), C::smem, s, qmap, kmap, vmap, w);
+  st = launch_pdl("attention (window)", kern, grid, dim3(C::threads), C::smem, s, qmap, kmap, vmap, w);
   if (st || w.splits == 1) return st;
   return launch_pdl("attention (window, join)", window_join_kernel<T, DP>, dim3(static_cast<unsigned>(ceil_div(rows, 8))),
                     dim3(256), 0, s, w);

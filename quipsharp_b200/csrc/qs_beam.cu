@@ -671,7 +671,7 @@ int launch_beam_select(const void *logits, int dtype, int64_t batch_stride, int6
   uint2 *cand = reinterpret_cast<uint2 *>(static_cast<char *>(ws) + round_up(rows * chunks * 8, 256));
   const ScanArgs a{logits, batch_stride, beam_stride, static_cast<int>(beams), static_cast<int>(vocab), n, chunks, 0,
                    stats, cand};
-  const int st = dtype == QS_F32 ? run_scan<float>(a, rows, s)
+  int st = dtype == QS_F32 ? run_scan<float>(a, rows, s)
                  : dtype == QS_F16 ? run_scan<__half>(a, rows, s) : run_scan<__nv_bfloat16>(a, rows, s);
   if (st) return st;
   const int per = chunks * n, group = static_cast<int>(std::min<int64_t>(beams, kLists / per)), room = round4(group * per);
@@ -680,9 +680,10 @@ int launch_beam_select(const void *logits, int dtype, int64_t batch_stride, int6
   // as much as this call needs: SMs that have to change their split of memory wait for the
   // kernel before (3 us)
   const size_t smem = static_cast<size_t>(room) * (per <= kDirect ? 8 : 16) + round4(static_cast<int>(beams * n)) * 8 + beams * sizeof(Beam);
-  static const cudaError_t attr = cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                       kLists * 16 + kBeamMaxBeams * kBeamMaxN * 8 + kBeamMaxBeams * (int)sizeof(Beam));
-  if (attr != cudaSuccess) return fail(QS_ERR_CUDA, "beam merge: %s", cudaGetErrorString(attr));
+  static std::atomic<uint64_t> allowed{0};
+  st = allow_smem("beam merge", beam_merge_kernel,
+                  kLists * 16 + kBeamMaxBeams * kBeamMaxN * 8 + kBeamMaxBeams * (int)sizeof(Beam), allowed);
+  if (st) return st;
   return launch_pdl("beam merge", beam_merge_kernel, dim3(static_cast<unsigned>(batch)), dim3(kT), smem, s, m);
 }
 

@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/quipsharp_b200.h"
 
 namespace qs {
@@ -47,6 +49,20 @@ inline int launch_pdl(const char *what, void (*kern)(KArgs...), dim3 grid, dim3 
   cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
   if (e != cudaSuccess) return fail(QS_ERR_CUDA, "%s launch failed: %s", what, cudaGetErrorString(e));
+  return QS_OK;
+}
+
+// Lets kern take `bytes` of dynamic shared memory a block on the current device.  The limit
+// belongs to the device: `done` (one for each kern, zero at first) remembers which have it.
+template <typename... KArgs>
+inline int allow_smem(const char *what, void (*kern)(KArgs...), int bytes, std::atomic<uint64_t> &done) {
+  int dev = 0;
+  QS_CUDA_TRY(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return QS_OK;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return fail(QS_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+  done.fetch_or(bit, std::memory_order_relaxed);
   return QS_OK;
 }
 
