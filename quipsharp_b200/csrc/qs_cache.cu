@@ -483,16 +483,21 @@ __global__ void __launch_bounds__(256) write_kernel(WriteArgs a) {
   }
 }
 
-constexpr size_t kNearBytes = 160 * 1024;
+constexpr int kNearBytes = 160 * 1024;
 
 // One CTA while a scan of the counts and the tables is short; a cluster of eight
 // shares longer ones.
 int cluster_for(int64_t rows, int64_t width, int64_t pages) { return rows * width + pages <= 32768 ? 1 : 8; }
 
+// The most shared memory that a kernel may ask for, whatever this call needs: a limit that
+// followed the calls could be lowered by another thread between its setting and the launch.
+template <bool NEAR>
+constexpr int kForkMost = NEAR ? kNearBytes : kCacheMaxRows * 20;
+template <bool NEAR>
+constexpr int kExtendMost = NEAR ? kNearBytes : kCacheMaxRows * 12;
+
 template <typename... KArgs, typename... Args>
-int launch_cluster(const char *what, void (*kern)(KArgs...), int ctas, size_t smem, cudaStream_t s, Args... args) {
-  if (smem > 48 * 1024)
-    QS_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+int launch_kernel(const char *what, void (*kern)(KArgs...), int ctas, size_t smem, cudaStream_t s, Args... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kThreads);
@@ -510,6 +515,13 @@ int launch_cluster(const char *what, void (*kern)(KArgs...), int ctas, size_t sm
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
   if (e != cudaSuccess) return fail(QS_ERR_CUDA, "%s launch failed: %s", what, cudaGetErrorString(e));
   return QS_OK;
+}
+
+template <auto kern, int most, typename... Args>
+int launch_cluster(const char *what, int ctas, size_t smem, cudaStream_t s, Args... args) {
+  static std::atomic<uint64_t> allowed{0};
+  const int st = most > 48 * 1024 ? allow_smem(what, kern, most, allowed) : QS_OK;
+  return st ? st : launch_kernel(what, kern, ctas, smem, s, args...);
 }
 
 int log2_of(int64_t v) {
@@ -559,8 +571,9 @@ int launch_cache_fork(const qs_kv_pool &pool, int rows, int width, const int *ta
   const int ctas = cluster_for(rows, width, pool.pages);
   const size_t near = static_cast<size_t>(rows) * 24 + pool.pages * 4;
   const int st = ctas == 1 && near <= kNearBytes
-                     ? launch_cluster("cache fork", fork_kernel<true>, ctas, near, s, t, parents, w)
-                     : launch_cluster("cache fork", fork_kernel<false>, ctas, static_cast<size_t>(rows) * 20, s, t, parents, w);
+                     ? launch_cluster<fork_kernel<true>, kForkMost<true>>("cache fork", ctas, near, s, t, parents, w)
+                     : launch_cluster<fork_kernel<false>, kForkMost<false>>("cache fork", ctas, static_cast<size_t>(rows) * 20, s,
+                                                                            t, parents, w);
   return st ? st : launch_copy(pool, w, s);
 }
 
@@ -570,8 +583,7 @@ int launch_cache_compact(const qs_kv_pool &pool, int rows, int width, const int 
   const Tables t{rows, width, static_cast<int>(pool.pages), log2_of(pool.page), table, lengths, refcount,
                  table_out, nullptr, refcount_out};
   const Work w = split_work(ws, rows, pool.pages);
-  const int st = launch_cluster("cache compact", compact_kernel, cluster_for(rows, width, pool.pages), 0, s, t,
-                                used_out, w);
+  const int st = launch_cluster<compact_kernel, 0>("cache compact", cluster_for(rows, width, pool.pages), 0, s, t, used_out, w);
   return st ? st : launch_copy(pool, w, s);
 }
 
@@ -583,8 +595,10 @@ int launch_cache_extend(int64_t page, int64_t pages, int rows, int width, const 
   const Work w = split_work(ws, rows, pages);
   const int ctas = cluster_for(rows, width, pages);
   const size_t near = static_cast<size_t>(rows) * 12 + pages * 8;
-  if (ctas == 1 && near <= kNearBytes) return launch_cluster("cache extend", extend_kernel<true>, ctas, near, s, t, add, w);
-  return launch_cluster("cache extend", extend_kernel<false>, ctas, static_cast<size_t>(rows) * 12, s, t, add, w);
+  if (ctas == 1 && near <= kNearBytes)
+    return launch_cluster<extend_kernel<true>, kExtendMost<true>>("cache extend", ctas, near, s, t, add, w);
+  return launch_cluster<extend_kernel<false>, kExtendMost<false>>("cache extend", ctas, static_cast<size_t>(rows) * 12, s, t,
+                                                                  add, w);
 }
 
 int launch_cache_write(const qs_kv_pool &pool, int rows, int width, const int *table, const int *lengths,

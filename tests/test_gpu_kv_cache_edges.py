@@ -1,8 +1,11 @@
 """Page moves of the key-value cache at the edges of what tables and arguments may hold."""
+import threading
+
 import numpy as np
 import pytest
 import torch
 
+from quipsharp_b200 import _native as N
 from quipsharp_b200 import kv_cache as kc
 from test_gpu_kv_cache import DEV, on, same
 
@@ -50,4 +53,36 @@ def test_children_of_a_row_whose_last_page_is_absent(rows, pages):
     assert t[:4].tolist() == [[2, -1, -1], [2, -1, -1], [3, 0, -1], [3, 1, -1]] and bool((t[4:] == -1).all())
     assert n[:4].tolist() == [20, 20, 25, 25] and c[:6].tolist() == [1, 1, 2, 2, 0, 0] and int(c.sum()) == 6
     same(k, wk.cpu(), "keys"), same(v, wv.cpu(), "values")
+    kc.check_device()
+
+
+def test_caches_of_different_sizes_in_two_threads():
+    """Each call lets its kernel have shared memory and launches: another thread's smaller call
+    in between must not take that away."""
+    lib = N.lib()
+    calls = []
+    for pages in (19000, 7000):
+        state = on(np.full((4, 4), -1, np.int32), np.zeros(4, np.int32), np.zeros(pages, np.int32), np.ones(4, np.int32))
+        out = [t.clone() for t in state[:3]]
+        nb = lib.qs_cache_workspace_bytes(4, pages)
+        ws = torch.empty(nb, dtype=torch.uint8, device=DEV)
+        calls.append((state, out, ws, (16, pages, 4, 4, *(t.data_ptr() for t in (*state, *out, ws)), nb,
+                                       torch.cuda.Stream().cuda_stream)))
+    torch.cuda.synchronize()
+    failed = [0, 0]
+
+    def work(i):
+        for _ in range(4000):
+            if lib.qs_cache_extend(*calls[i][3]) != N.QS_OK:
+                failed[i] += 1
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert failed == [0, 0]
+    for _, (table, lengths, count), _, _ in calls:
+        assert table[:, 0].tolist() == [0, 1, 2, 3] and lengths.tolist() == [1] * 4 and int(count.sum()) == 4
     kc.check_device()
