@@ -32,7 +32,7 @@ def _arguments(name, q, k_pages, v_pages, table, lengths, window, sinks, scale):
     _, heads, q_dim = q.shape
     if q_dim != dim:
         raise ValueError(f"queries of dimension {q_dim} do not match the cache's {dim}")
-    if heads % kv_heads:
+    if not kv_heads or heads % kv_heads:
         raise ValueError(f"{heads} query heads do not share {kv_heads} key heads evenly")
     if window is None:
         window = 0

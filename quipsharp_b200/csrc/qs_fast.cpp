@@ -124,7 +124,7 @@ PyObject *attend(PyObject *const *in) {
   qs_kv_pool pool;
   PLAIN(q->dim() == 3 && q->scalar_type() == k->scalar_type() && pool_of(*k, *v, 4, &pool) && in_pieces(*q));
   const int64_t rows = table->size(0), width = table->size(1), tokens = q->size(0), heads = q->size(1), dim = q->size(2);
-  PLAIN(dim == pool.dim && dim > 0 && heads % pool.heads == 0 && lengths->size(0) == rows &&
+  PLAIN(dim == pool.dim && dim > 0 && pool.heads > 0 && heads % pool.heads == 0 && lengths->size(0) == rows &&
         (many ? cu->size(0) == rows + 1 : tokens == rows));
   double scale = 1.0 / std::sqrt(static_cast<double>(dim));
   if (in[8] != Py_None) {

@@ -108,3 +108,12 @@ def test_tokens_before_the_first_row_are_zero(first, new, past):
     check((out[mine], lse[mine]), exact(q[mine], k, v, table, n, new, 0, 0), torch.float16, True)
     for rest in (slice(0, first), slice(first + sum(new), total)):
         assert not out[rest].any() and torch.isneginf(lse[rest]).all()
+
+
+def test_pools_without_a_key_head_are_refused():
+    k = torch.zeros(4, 0, 16, 64, device=DEV, dtype=torch.float16)
+    q = torch.zeros(2, 4, 64, device=DEV, dtype=torch.float16)
+    table, n = (torch.zeros(s, dtype=torch.int32, device=DEV) for s in ((2, 3), (2,)))
+    for call in (lambda: at.decode_attention(q, k, k, table, n), lambda: at.window_attention(q, k, k, table, n, offsets([1, 1]))):
+        with pytest.raises(ValueError, match="0 key heads"):
+            call()
