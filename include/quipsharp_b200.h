@@ -66,8 +66,10 @@ const char *qs_last_error(void);
  * limit: a stalled pipeline ends the kernel with this flag set instead of
  * hanging the GPU.  Also reports, and clears, what the cache operators found
  * on the device since the last call: QS_ERR_PAGES (no free page, or a table row
- * outgrown) and QS_ERR_INDEX (a parent or token count out of range).  No
- * counterpart in the reference (pure Python). */
+ * outgrown) and QS_ERR_INDEX (a parent or token count out of range).  One call
+ * reports and clears one kind; call again for others.  The flags belong to the
+ * device: they are of all caches and streams on it.  No counterpart in the
+ * reference (pure Python). */
 int qs_device_status(qs_stream_t stream);
 
 /* Limit, in nanoseconds, of the bounded waits between the warps of the

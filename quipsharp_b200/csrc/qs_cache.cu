@@ -28,6 +28,8 @@ __device__ int g_cache_error;
 
 __device__ __forceinline__ void flag_error(int bit) { atomicOr(&g_cache_error, bit); }
 
+__global__ void clear_error_kernel(int bit) { atomicAnd(&g_cache_error, ~bit); }
+
 __device__ __forceinline__ int cluster_rank() {
   uint32_t r;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -550,13 +552,14 @@ int device_sms() {
   return n;
 }
 
-int take_cache_errors(int *bits, cudaStream_t s) {
-  static const int zero = 0;
-  *bits = 0;
-  QS_CUDA_TRY(cudaMemcpyFromSymbolAsync(bits, g_cache_error, sizeof(int), 0, cudaMemcpyDeviceToHost, s));
+int take_cache_error(int *bit, cudaStream_t s) {
+  int bits = 0;
+  QS_CUDA_TRY(cudaMemcpyFromSymbolAsync(&bits, g_cache_error, sizeof(int), 0, cudaMemcpyDeviceToHost, s));
   QS_CUDA_TRY(cudaStreamSynchronize(s));
-  if (*bits) {
-    QS_CUDA_TRY(cudaMemcpyToSymbolAsync(g_cache_error, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s));
+  *bit = bits & kCacheErrPages ? kCacheErrPages : bits;
+  if (*bit) {  // that one alone: what another stream raises meanwhile stays
+    clear_error_kernel<<<1, 1, 0, s>>>(*bit);
+    QS_CUDA_TRY(cudaGetLastError());
     QS_CUDA_TRY(cudaStreamSynchronize(s));
   }
   return QS_OK;

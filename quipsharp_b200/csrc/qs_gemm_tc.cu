@@ -721,12 +721,12 @@ int device_status(cudaStream_t s) {
     return fail(QS_ERR_TIMEOUT, "a bounded wait timed out (prefill matmul pipeline or tensor-parallel shard arrival); "
                 "the results of that launch are invalid");
   }
-  int bits = 0;
-  const int st = take_cache_errors(&bits, s);
+  int bit = 0;
+  const int st = take_cache_error(&bit, s);
   if (st) return st;
-  if (bits & kCacheErrPages)
+  if (bit == kCacheErrPages)
     return fail(QS_ERR_PAGES, "a cache row found no free page, or outgrew its page table row; its new tokens have no page");
-  if (bits & kCacheErrParent) return fail(QS_ERR_INDEX, "a cache row's parent or token count was out of range");
+  if (bit) return fail(QS_ERR_INDEX, "a cache row's parent or token count was out of range");
   return QS_OK;
 }
 

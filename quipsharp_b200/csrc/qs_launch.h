@@ -139,8 +139,8 @@ int launch_cache_extend(int64_t page, int64_t pages, int rows, int width, const 
 int launch_cache_write(const qs_kv_pool &pool, int rows, int width, const int *table, const int *lengths,
                        const int *cu, const void *k, int64_t k_token, int64_t k_head, const void *v, int64_t v_token,
                        int64_t v_head, int64_t tokens, cudaStream_t s);
-// Reads and clears the kCacheErr bits raised on the device (synchronises s).
-int take_cache_errors(int *bits, cudaStream_t s);
+// Reads and clears one of the kCacheErr bits raised on the device (synchronises s).
+int take_cache_error(int *bit, cudaStream_t s);
 int device_sms();  // of the current device
 
 // Arguments of attention over one layer of the cache (strides in elements).

@@ -29,8 +29,10 @@ KV_DTYPES = {torch.float16: N.QS_F16, torch.bfloat16: N.QS_BF16}
 
 def check_device(device=None) -> None:
     """Synchronises the current stream and raises what the kernels found wrong
-    since the last call: RuntimeError when rows found no free page or a bounded
-    wait ran out, IndexError for a parent or token count out of range."""
+    since the last call, on any cache of the device: RuntimeError when rows found
+    no free page or a bounded wait ran out, IndexError for a parent or token count
+    out of range.  One kind at a time: where there are two, the next call raises
+    the other."""
     with torch.cuda.device(device):
         N.check(N.lib().qs_device_status(N.raw_stream(torch.cuda.current_device())))
 
@@ -276,5 +278,6 @@ class PagedKVCache:
         return used
 
     def check(self) -> None:
-        """Raises what the kernels found wrong since the last check (synchronises)."""
+        """Raises what the kernels found wrong since the last check, on any cache of
+        the device (see check_device)."""
         check_device(self.k.device)

@@ -86,3 +86,15 @@ def test_caches_of_different_sizes_in_two_threads():
     for _, (table, lengths, count), _, _ in calls:
         assert table[:, 0].tolist() == [0, 1, 2, 3] and lengths.tolist() == [1] * 4 and int(count.sum()) == 4
     kc.check_device()
+
+
+def test_errors_of_two_kinds_are_both_reported():
+    """One call finds a token count out of range and no free page: two checks raise, a third does not."""
+    args = on(np.array([[0], [-1]], np.int32), np.array([16, 0], np.int32), np.array([1], np.int32), np.array([-1, 5], np.int32))
+    kc.check_device()
+    kc.extend_pages(*args, 16)
+    with pytest.raises(RuntimeError, match="no free page"):
+        kc.check_device()
+    with pytest.raises(IndexError):
+        kc.check_device()
+    kc.check_device()
