@@ -22,7 +22,7 @@ from .kv_cache import _device_of, _int32, kv_pool
 
 
 def _arguments(name, q, k_pages, v_pages, table, lengths, window, sinks, scale):
-    N.refuse_grad(name, q)
+    N.refuse_grad(name, q, k_pages, v_pages)
     if k_pages.dim() != 4 or table.dim() != 2 or q.dim() != 3:
         raise ValueError(f"{name} takes queries (tokens, heads, dim), one layer's pools (pages, heads, page, dim) "
                          "and a table (rows, width)")

@@ -103,6 +103,7 @@ def fork_pages(k: Tensor, v: Tensor, table: Tensor, lengths: Tensor, refcount: T
     got = N.fast().fork_pages(k, v, table, lengths, refcount, parents)
     if got is not None:
         return got
+    N.refuse_grad("fork_pages", k, v)
     dev = _device_of(k, v, table, lengths, refcount, parents)
     if not N.is_current(dev):
         with torch.cuda.device(dev):
@@ -126,6 +127,7 @@ def compact_pages(k: Tensor, v: Tensor, table: Tensor, lengths: Tensor,
     got = N.fast().compact_pages(k, v, table, lengths, refcount)
     if got is not None:
         return got
+    N.refuse_grad("compact_pages", k, v)
     dev = _device_of(k, v, table, lengths, refcount)
     if not N.is_current(dev):
         with torch.cuda.device(dev):
@@ -180,7 +182,7 @@ def write_kv(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tens
     contiguous)."""
     if N.fast().write_kv(k, v, k_pages, v_pages, table, lengths, cu):
         return
-    N.refuse_grad("write_kv", k, v)
+    N.refuse_grad("write_kv", k, v, k_pages, v_pages)
     dev = _device_of(k, v, k_pages, v_pages, table, lengths, cu)
     if not N.is_current(dev):
         with torch.cuda.device(dev):

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from quipsharp_b200 import attention as at
+from quipsharp_b200 import kv_cache as kc
 from test_gpu_attention import DEV, check, exact, make
 
 pytestmark = pytest.mark.gpu
@@ -117,3 +118,23 @@ def test_pools_without_a_key_head_are_refused():
     for call in (lambda: at.decode_attention(q, k, k, table, n), lambda: at.window_attention(q, k, k, table, n, offsets([1, 1]))):
         with pytest.raises(ValueError, match="0 key heads"):
             call()
+
+
+def test_pools_that_require_grad_are_refused():
+    """No gradient reaches a pool: a call that would lose one is refused, as for the queries."""
+    rs = np.random.RandomState(1)
+    k, v, table, n = make(rs, [40, 20], 2, 16, 64, torch.float16)
+    q = torch.randn(2, 4, 64, device=DEV).half()
+    new = torch.randn(2, 2, 64, device=DEV).half()
+    cu = torch.arange(3, dtype=torch.int32, device=DEV)
+    count = torch.ones(len(k), dtype=torch.int32, device=DEV)
+    grad = [x.clone().requires_grad_() for x in (k, v)]
+    for kk, vv in ((grad[0], v), (k, grad[1])):
+        for call in (lambda: at.decode_attention(q, kk, vv, table, n), lambda: at.window_attention(q, kk, vv, table, n, cu),
+                     lambda: kc.write_kv(new, new, kk, vv, table, n),
+                     lambda: kc.fork_pages(kk[None], vv[None], table, n, count, n - n),
+                     lambda: kc.compact_pages(kk[None], vv[None], table, n, count)):
+            with pytest.raises(RuntimeError, match="no backward"):
+                call()
+            with torch.no_grad():
+                call()
