@@ -217,11 +217,13 @@ def is_current(index: int) -> bool:
 
 
 def refuse_grad(name: str, *tensors) -> None:
-    """The decoding operators have no backward pass: refuse inputs whose
-    gradient autograd would silently lose."""
+    """The decoding operators have no backward pass and no forward-mode one:
+    refuse inputs whose gradient or tangent autograd would silently lose."""
     for t in tensors:
         if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{name} has no backward pass; call it under torch.no_grad() or detach its inputs")
+        if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} has no forward-mode derivative; detach its inputs")
 
 
 def rows_of_8(t: torch.Tensor) -> torch.Tensor:

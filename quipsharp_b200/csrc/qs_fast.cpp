@@ -37,6 +37,7 @@ struct Args {
       ok = false;
     }
     if (t.requires_grad() && c10::GradMode::is_enabled()) ok = false;
+    if (t.unsafeGetTensorImpl()->autograd_meta() && t._fw_grad(0).defined()) ok = false;  // a tangent
     return &t;
   }
   const Tensor *ints(PyObject *o, int64_t dims) {

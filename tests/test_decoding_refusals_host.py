@@ -1,8 +1,9 @@
 """More refusals of the decoding operators (no GPU; see test_kv_cache_host)."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
-from quipsharp_b200 import attention
+from quipsharp_b200 import attention, beam
 
 
 def test_pools_without_a_key_head():
@@ -10,3 +11,12 @@ def test_pools_without_a_key_head():
     table, n = torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
     with pytest.raises(ValueError, match="0 key heads"):
         attention._arguments("decode_attention", q, k, k, table, n, None, 0, None)
+
+
+def test_forward_mode_tangents():
+    with fwd.dual_level():
+        x = fwd.make_dual(torch.zeros(1, 2, 9), torch.ones(1, 2, 9))
+        with pytest.raises(RuntimeError, match="no forward-mode"):
+            beam.beam_select(x, torch.zeros(1, 2))
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        beam.beam_select(x, torch.zeros(1, 2))

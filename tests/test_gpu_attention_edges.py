@@ -3,9 +3,11 @@
 import numpy as np
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 from quipsharp_b200 import attention as at
 from quipsharp_b200 import kv_cache as kc
+from quipsharp_b200.beam import beam_select
 from test_gpu_attention import DEV, check, exact, make
 
 pytestmark = pytest.mark.gpu
@@ -138,3 +140,21 @@ def test_pools_that_require_grad_are_refused():
                 call()
             with torch.no_grad():
                 call()
+
+
+def test_forward_mode_tangents_are_refused():
+    rs = np.random.RandomState(2)
+    k, v, table, n = make(rs, [40, 20], 2, 16, 64, torch.float16)
+    q = torch.randn(2, 4, 64, device=DEV).half()
+    cu = torch.arange(3, dtype=torch.int32, device=DEV)
+    x, s = torch.randn(1, 2, 50, device=DEV), torch.zeros(1, 2, device=DEV)
+    with fwd.dual_level():
+        dual = [fwd.make_dual(t, torch.ones_like(t)) for t in (q, k, v, x, s)]
+        for call in (lambda: at.decode_attention(dual[0], k, v, table, n), lambda: at.decode_attention(q, dual[1], v, table, n),
+                     lambda: at.window_attention(dual[0], k, v, table, n, cu),
+                     lambda: at.window_attention(q, k, dual[2], table, n, cu),
+                     lambda: kc.write_kv(dual[0][:, :2], q[:, :2], k, v, table, n),
+                     lambda: beam_select(dual[3], s), lambda: beam_select(x, dual[4])):
+            with pytest.raises(RuntimeError, match="no .*derivative"):
+                call()
+    beam_select(x, s)
