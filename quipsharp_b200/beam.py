@@ -29,6 +29,8 @@ def beam_select(logits: Tensor, scores: Tensor, n: int | None = None, finished: 
     if got is not None:
         return got
     N.refuse_grad("beam_select", logits, scores)
+    if not -(1 << 31) <= pad < 1 << 31:
+        raise ValueError(f"pad must be an int32, got {pad}")
     dev = _device_of(logits, scores, finished)
     if not N.is_current(dev):
         with torch.cuda.device(dev):

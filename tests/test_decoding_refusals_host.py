@@ -20,3 +20,9 @@ def test_forward_mode_tangents():
             beam.beam_select(x, torch.zeros(1, 2))
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         beam.beam_select(x, torch.zeros(1, 2))
+
+
+@pytest.mark.parametrize("pad", [1 << 31, -(1 << 31) - 1, 1 << 40])
+def test_padding_tokens_are_int32(pad):
+    with pytest.raises(ValueError, match="int32"):
+        beam.beam_select(torch.zeros(1, 2, 9), torch.zeros(1, 2), pad=pad)
