@@ -42,8 +42,8 @@ def _arguments(name, q, k_pages, v_pages, table, lengths, window, sinks, scale):
         raise ValueError(f"sinks must not be negative, got {sinks}")
     rows, width = table.shape
     return (N.rows_of_8(q), pool, kv_heads, page, rows, width, _int32("table", table, rows, width),
-            _int32("lengths", lengths, rows), 1.0 / math.sqrt(dim) if scale is None else float(scale), int(window),
-            int(sinks))
+            _int32("lengths", lengths, rows), 1.0 / math.sqrt(dim) if scale is None else float(scale),
+            min(int(window), 1 << 62), min(int(sinks), 1 << 62))
 
 
 def decode_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, *,

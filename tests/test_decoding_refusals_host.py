@@ -26,3 +26,11 @@ def test_forward_mode_tangents():
 def test_padding_tokens_are_int32(pad):
     with pytest.raises(ValueError, match="int32"):
         beam.beam_select(torch.zeros(1, 2, 9), torch.zeros(1, 2), pad=pad)
+
+
+def test_windows_of_any_size():
+    """A number past 64 bits is a very large one, not what is left of it."""
+    q, k = torch.zeros(2, 4, 64, dtype=torch.float16), torch.zeros(4, 2, 16, 64, dtype=torch.float16)
+    table, n = torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    *_, window, sinks = attention._arguments("decode_attention", q, k, k, table, n, (1 << 64) + 5, (1 << 65) + 1, None)
+    assert 1 << 31 < window < 1 << 63 and 1 << 31 < sinks < 1 << 63
