@@ -12,6 +12,7 @@ import importlib.util
 import os
 import struct
 import threading
+import warnings
 
 import torch
 
@@ -158,8 +159,19 @@ def lib():
 _fast = None
 
 
+class _NoFast:
+    """Stands in for the extension: no call is plain, so all go by ctypes."""
+
+    def _not_plain(self, *args):
+        return None
+
+    attend = fork_pages = compact_pages = extend_pages = write_kv = beam_select = _not_plain
+
+
 def fast():
-    """The extension module with the decoding operators' direct calls (csrc/qs_fast.cpp)."""
+    """The extension module with the decoding operators' direct calls (csrc/qs_fast.cpp).
+    Without it (or with one built for another torch) the same kernels are called by ctypes,
+    which takes longer on the host."""
     global _fast
     if _fast is None:
         lib()
@@ -169,8 +181,9 @@ def fast():
             module = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(module)
         except ImportError as e:
-            raise NativeLibraryMissing(f"{path} is missing or was built for another torch ({e}); "
-                                       "run `python -m quipsharp_b200.build_native -f`") from e
+            warnings.warn(f"{path} is missing or was built for another torch ({e}): decoding calls take 6 to 8 us more; "
+                          "run `python -m quipsharp_b200.build_native -f`", RuntimeWarning, stacklevel=3)
+            module = _NoFast()
         _fast = module
     return _fast
 

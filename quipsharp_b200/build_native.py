@@ -166,8 +166,9 @@ def build(verbose: bool = False, force: bool = False) -> str:
     return lib
 
 
-def build_fast(verbose: bool, force: bool) -> str:
-    """The Python extension with the decoding operators' direct calls, linked to the library."""
+def build_fast(verbose: bool, force: bool) -> str | None:
+    """The Python extension with the decoding operators' direct calls, linked to the library;
+    None where there is no compiler or are no headers for it (the calls then go by ctypes)."""
     import sysconfig
 
     import torch
@@ -177,9 +178,17 @@ def build_fast(verbose: bool, force: bool) -> str:
         return out
     inc = os.path.join(os.path.dirname(torch.__file__), "include")
     cuda = os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")
-    cmd = [os.environ.get("CXX") or shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC",
+    cxx, python = os.environ.get("CXX") or "g++", sysconfig.get_paths()["include"]
+    for what, there in (("a C++ compiler", shutil.which(cxx)), ("Python's headers", os.path.exists(os.path.join(python, "Python.h"))),
+                        ("torch's headers", os.path.exists(os.path.join(inc, "ATen", "ATen.h")))):
+        if not there:
+            sys.stderr.write(f"{os.path.basename(out)} is not built, for want of {what}: decoding calls go by ctypes\n")
+            if os.path.exists(out):  # older than what it calls
+                os.remove(out)
+            return None
+    cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC",
            "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           "-I", sysconfig.get_paths()["include"], "-I", inc,
+           "-I", python, "-I", inc,
            "-I", os.path.join(inc, "torch", "csrc", "api", "include"), "-I", cuda,
            src, "-o", out, "-L", LIBDIR, f"-l:{LIBNAME}", "-Wl,-rpath,$ORIGIN",
            # torch's own libraries are loaded by the time this is
