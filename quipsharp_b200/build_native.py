@@ -174,7 +174,10 @@ def build_fast(verbose: bool, force: bool) -> str | None:
     import torch
     src, out = os.path.join(CSRC, "qs_fast.cpp"), os.path.join(LIBDIR, "_fast.so")
     newest = max(os.path.getmtime(src), os.path.getmtime(os.path.join(REPO, "include", "quipsharp_b200.h")))
-    if not force and os.path.exists(out) and os.path.getmtime(out) >= newest:
+    # what it was built for: torch's C++ interface changes between versions
+    stamp, built_for = os.path.join(BUILD, "_fast.built_for"), f"torch {torch.__version__}, Python {sys.version}\n"
+    known = os.path.exists(stamp) and open(stamp).read() == built_for
+    if not force and known and os.path.exists(out) and os.path.getmtime(out) >= newest:
         return out
     inc = os.path.join(os.path.dirname(torch.__file__), "include")
     cuda = os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")
@@ -200,6 +203,7 @@ def build_fast(verbose: bool, force: bool) -> str | None:
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
         raise RuntimeError(f"g++ failed on {src}")
+    _write_if_changed(stamp, built_for)
     return out
 
 

@@ -36,3 +36,20 @@ def test_the_library_is_built_without_what_it_needs(gone, tmp_path, monkeypatch,
         monkeypatch.setattr(sysconfig, "get_paths", lambda: {**paths, "include": str(tmp_path)})
     assert build_native.build_fast(False, True) is None
     assert "ctypes" in capsys.readouterr().err
+
+
+def test_it_is_built_again_for_another_torch(tmp_path, monkeypatch):
+    calls = []
+
+    def run(cmd, **kw):
+        calls.append(cmd)
+        (tmp_path / "_fast.so").write_bytes(b"")
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+
+    monkeypatch.setattr(subprocess, "run", run)
+    monkeypatch.setattr(build_native, "LIBDIR", str(tmp_path))
+    monkeypatch.setattr(build_native, "BUILD", str(tmp_path))
+    for version, builds in ((torch.__version__, 1), (torch.__version__, 1), ("99.0", 2), ("99.0", 2)):
+        monkeypatch.setattr(torch, "__version__", version)
+        assert build_native.build_fast(False, False) == str(tmp_path / "_fast.so")
+        assert len(calls) == builds
