@@ -71,8 +71,7 @@ def decode_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor,
     if tokens != rows:
         raise ValueError(f"decode_attention takes one query token per row: {tokens} tokens, {rows} rows")
     nb = N.workspace_bytes("qs_attn_decode_workspace_bytes", rows, heads, kv_heads, dim, page, width, window, sinks)
-    if nb < 0:
-        raise NotImplementedError(f"head dimension must be a multiple of 8 up to 128, got {dim}")
+    nb = max(nb, 0)  # below: sizes that the library refuses, with its reason
     ws = lengths.new_empty(nb // 4) if nb else None
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = q.new_empty((rows, heads), dtype=torch.float32) if return_lse else None
@@ -106,8 +105,7 @@ def window_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor,
     cu = _int32("cu", cu, rows + 1)
     tokens, heads, dim = q.shape
     nb = N.workspace_bytes("qs_attn_window_workspace_bytes", tokens, rows, heads, kv_heads, dim, page, width, window, sinks)
-    if nb < 0:
-        raise NotImplementedError(f"head dimension must be a multiple of 8 up to 128, got {dim}")
+    nb = max(nb, 0)  # below: sizes that the library refuses, with its reason
     ws = lengths.new_empty(nb // 4) if nb else None
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None

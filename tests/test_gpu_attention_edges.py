@@ -158,3 +158,15 @@ def test_forward_mode_tangents_are_refused():
             with pytest.raises(RuntimeError, match="no .*derivative"):
                 call()
     beam_select(x, s)
+
+
+@pytest.mark.parametrize("page,dim,heads,what", [(512, 64, 4, "page size"), (8, 64, 4, "page size"), (24, 64, 4, "page size"),
+                                                 (16, 136, 4, "head dimension"), (16, 60, 4, "head dimension"),
+                                                 (16, 64, 1 << 21, "too many")])
+def test_refusals_name_what_is_wrong(page, dim, heads, what):
+    k = torch.zeros(2, 2, page, dim, device=DEV, dtype=torch.float16)
+    q = torch.zeros(1, 1, dim, device=DEV, dtype=torch.float16).expand(1, heads, dim)
+    table, n = (torch.zeros(s, dtype=torch.int32, device=DEV) for s in ((1, 3), (1,)))
+    for call in (lambda: at.decode_attention(q, k, k, table, n), lambda: at.window_attention(q, k, k, table, n, offsets([1]))):
+        with pytest.raises(NotImplementedError, match=what):
+            call()
