@@ -170,3 +170,15 @@ def test_refusals_name_what_is_wrong(page, dim, heads, what):
     for call in (lambda: at.decode_attention(q, k, k, table, n), lambda: at.window_attention(q, k, k, table, n, offsets([1]))):
         with pytest.raises(NotImplementedError, match=what):
             call()
+
+
+@pytest.mark.parametrize("axis", [0, 1])
+def test_queries_broadcast_along_an_axis(axis):
+    """A query that all tokens, or all heads, share is read where it is."""
+    rs = np.random.RandomState(5)
+    k, v, table, n = make(rs, [77, 300], 2, 32, 64, torch.float16)
+    q = torch.randn((1, 8, 64) if axis == 0 else (60, 1, 64), device=DEV).half().expand(60, 8, 64)
+    got = at.window_attention(q, k, v, table, n, offsets([20, 40]), return_lse=True)
+    check(got, exact(q, k, v, table, n, [20, 40], 0, 0), torch.float16, True)
+    got = at.decode_attention(q[:2], k, v, table, n, return_lse=True)
+    check(got, exact(q[:2], k, v, table, n, [1, 1], 0, 0), torch.float16, False)
