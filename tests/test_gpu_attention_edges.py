@@ -182,3 +182,35 @@ def test_queries_broadcast_along_an_axis(axis):
     check(got, exact(q, k, v, table, n, [20, 40], 0, 0), torch.float16, True)
     got = at.decode_attention(q[:2], k, v, table, n, return_lse=True)
     check(got, exact(q[:2], k, v, table, n, [1, 1], 0, 0), torch.float16, False)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("new,past,q_heads,kv_heads,page,dim", [
+    (8, 15000, 8, 1, 64, 128), (3, 9000, 6, 2, 16, 96), (70, 2500, 8, 2, 32, 64), (1100, 3000, 4, 1, 128, 128)])
+def test_long_rows_to_their_own_rounding(new, past, q_heads, kv_heads, page, dim, dtype):
+    """Over n keys an output is about n^(-1/2), so the tolerance has to be this case's own.
+    With u as elsewhere, p the softmax and v the values: the output's rounding is u |o|; the
+    n roundings of weights are independent, at most u p each and even within that, so their
+    sum has a deviation below u (sum p^2 v^2 / 3)^(1/2), taken six times; a float16 weight
+    below its normal range is off by 2^-25 at most where the largest is 2^6 or more, so all
+    together by n 2^-31 max |v|; and float32 sums as elsewhere, 1e-4 sum p |v|.  That the
+    tolerance is narrow enough shows in outputs without the values of 256 keys."""
+    rs = np.random.RandomState(new)
+    n = new + past
+    k, v, table, lengths = make(rs, [n], kv_heads, page, dim, dtype)
+    q = torch.randn(new, q_heads, dim, device=DEV).to(dtype)
+    kk, vv = (x[table[0].long()].transpose(1, 2).reshape(-1, kv_heads, dim)[:n].double().repeat_interleave(q_heads // kv_heads, 1)
+              for x in (k, v))
+    s = torch.einsum("thd,nhd->htn", q.double(), kk) * dim ** -0.5
+    p = s.masked_fill(torch.arange(n, device=DEV) > past + torch.arange(new, device=DEV)[:, None], -torch.inf).softmax(-1)
+    o = torch.einsum("htn,nhd->thd", p, vv)
+    deviation = (torch.einsum("htn,nhd->thd", p * p, vv * vv) / 3).sqrt()
+    u = 2.0 ** -11 if dtype is torch.float16 else 2.0 ** -8
+    tol = u * o.abs() + 6 * u * deviation + 1e-4 * torch.einsum("htn,nhd->thd", p, vv.abs())
+    if dtype is torch.float16:
+        tol += n * 2.0 ** -31 * vv.abs().max()
+    for at_key in (0, n // 2 // 256 * 256, past - 256):
+        part = slice(at_key, at_key + 256)
+        assert bool((torch.einsum("htn,nhd->thd", p[..., part], vv[part]).abs() > tol).any(-1).float().mean() > 0.9)
+    err = (at.window_attention(q, k, v, table, lengths, offsets([new])).double() - o).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
