@@ -58,8 +58,10 @@ constexpr float kBias = 6.f;
 // Of 64 weights with the reference kept.  None of them may overflow float16; a first tile
 // with few keys seen leaves a low reference, from which this has room for 2^3 with scores
 // of ordinary spread (bias 8: 2^1, and chunks under a window took 93 us for 84).
+// Bfloat16 weights hold more, but their products with large values go into float32 sums: with
+// 2^30 those stay finite up to values of 1e26 and a thousand such tiles.
 template <typename T>
-constexpr float kMaxSum = std::is_same<T, __half>::value ? 60000.f : 1e30f;
+constexpr float kMaxSum = std::is_same<T, __half>::value ? 60000.f : 0x1p30f;
 constexpr int kHalf = kTile * 128;    // bytes of 128 rows of 64 values
 constexpr uint64_t kDrainNs = kDefaultWaitNs;
 

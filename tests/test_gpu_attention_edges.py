@@ -214,3 +214,22 @@ def test_long_rows_to_their_own_rounding(new, past, q_heads, kv_heads, page, dim
         assert bool((torch.einsum("htn,nhd->thd", p[..., part], vv[part]).abs() > tol).any(-1).float().mean() > 0.9)
     err = (at.window_attention(q, k, v, table, lengths, offsets([new])).double() - o).abs()
     assert bool((err <= tol).all()), float((err / tol).max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("new,heads", [(1, 2), (40, 2), (300, 80)])  # the last has whole rows, not shares of the keys
+def test_scores_that_grow_along_the_row_and_large_values(new, heads, dtype):
+    """Scores that rise by 80 over the row: the weights' reference lags behind them, and must
+    not lag so far that a weight times a large value passes float32's range."""
+    rs = np.random.RandomState(new)
+    n, dim = 1500, 64
+    k, v, table, lengths = make(rs, [n], heads, 16, dim, dtype)
+    v *= 1e20 if dtype is torch.bfloat16 else 1e3
+    for place in range(n):
+        k[int(table[0, place // 16]), :, place % 16, 0] = 40.0 * place / n  # times 16 / 8: up to 80
+    q = torch.randn(new, heads, dim, device=DEV).to(dtype)
+    q[:, :, 0] = 16.0
+    want = exact(q, k, v, table, lengths, [new], 0, 0)
+    check(at.window_attention(q, k, v, table, lengths, offsets([new]), return_lse=True), want, dtype, True)
+    one = [x[-1:] for x in want]
+    check(at.decode_attention(q[-1:], k, v, table, lengths, return_lse=True), one, dtype, False)
