@@ -377,7 +377,7 @@ __device__ __forceinline__ void amend_row(const WindowArgs &w, const Job &j, int
   const AttnArgs &a = w.a;
   const int ahead = t * w.tokens_per_tile + r / w.share, token = j.t0 + ahead, pos = j.pos0 + ahead;
   const int last = min(pos, j.keys - 1);
-  const int low = a.window > 0 && pos > a.window ? static_cast<int>(pos - a.window) : -1;
+  const int low = a.window > 0 && pos >= a.window ? static_cast<int>(pos - a.window) : -1;
   const int head = j.head * w.share + r % w.share, pieces = a.dim / 8, slots = (1 << a.page_shift) - 1;
   const int *table = a.table + static_cast<int64_t>(j.row) * a.width;
   auto seen = [&](int key) { return key <= last && (key > low || key < a.sinks); };

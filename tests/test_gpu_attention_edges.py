@@ -216,6 +216,25 @@ def test_long_rows_to_their_own_rounding(new, past, q_heads, kv_heads, page, dim
     assert bool((err <= tol).all()), float((err / tol).max())
 
 
+@pytest.mark.parametrize("window", [1, 4, 31, 32, 64, 70])
+def test_values_not_seen_at_every_place_of_a_window(window):
+    """The token whose window begins at the row's second key, and its neighbours, too."""
+    rs = np.random.RandomState(window)
+    n, dim = 150, 64
+    k, v, table, lengths = make(rs, [n], 1, 16, dim, torch.float16)
+    q = torch.randn(n, 4, dim, device=DEV).half()
+    want = exact(q, k, v, table, lengths, [n], window, 0)
+    pos = torch.arange(n, device=DEV)
+    for place in (0, 1, window - 1, window, window + 1, 2 * window, n - 1):
+        w = v.clone()
+        w[int(table[0, place // 16]), :, place % 16, 5] = float("nan")
+        out = at.window_attention(q, k, w, table, lengths, offsets([n]), window=window, return_lse=True)
+        hit = torch.zeros(n, 4, dim, dtype=torch.bool, device=DEV)
+        hit[:, :, 5] = ((place <= pos) & (place > pos - window))[:, None]
+        assert out[0][hit].isnan().all()
+        check((out[0].masked_fill(hit, 0), out[1]), (want[0].masked_fill(hit, 0), *want[1:]), torch.float16, weights=True)
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("new,heads", [(1, 2), (40, 2), (300, 80)])  # the last has whole rows, not shares of the keys
 def test_scores_that_grow_along_the_row_and_large_values(new, heads, dtype):
