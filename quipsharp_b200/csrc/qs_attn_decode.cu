@@ -17,10 +17,10 @@
 // over each other's shared memory.
 //
 // Bound: the keys and values seen, once, at HBM rate.  Measured: 64 rows of 100 to 16000
-// tokens, 64 query heads over 8 of 128, bfloat16: 318 us for 2.0 GB (6.3 TB/s); 48 rows
-// under a window of 1000, 28 heads over 4 of 64: 13.7 us (46 MB, 3.4 TB/s: 192 segments of
-// unequal length, and a step's latency); one row of 203 tokens 5.2 us, latency alone;
-// one row of 1500, 8 key heads, 6.9.
+// tokens, 64 query heads over 8 of 128, bfloat16: 318 to 330 us for 2.0 GB (6.1 to 6.3 TB/s);
+// 48 rows under a window of 1000, 28 heads over 4 of 64: 13.7 us (46 MB, 3.4 TB/s: 192
+// segments of unequal length, and a step's latency); one row of 203 tokens 5.4 us, latency
+// alone; one row of 1500, 8 key heads, 6.9.
 #include <cmath>
 #include <type_traits>
 

@@ -29,9 +29,11 @@
 // Bound: the exponentials.  A key tile of one query tile takes 128 x 128 of them, 1024
 // cycles of an SM's sixteen a cycle, next to 1024 of the two products (dim 128) and the
 // rest of the softmax's issue.  Measured: a prompt of 8192 tokens, 64 query heads over 8
-// of 128, bfloat16: 960 us (1.15 PFLOP/s); four chunks of 300 to 2000 tokens under a window
-// of 1024: 81 us (0.73 PFLOP/s of visible pairs; ten tiles a job, four of them with masks); up to 9
-// tokens of 3 rows: 10 us, latency alone.
+// of 128, bfloat16: 940 to 967 us (1.14 to 1.17 PFLOP/s, by the clocks that the power limit
+// leaves); four chunks of 300 to 2000 tokens under a window of 1024: 87 us (0.68 PFLOP/s of
+// visible pairs; ten tiles a job, four of them with masks); up to 9 tokens of 3 rows: 10.4 us,
+// latency alone.  (Passes through the public call; the figures of variants below are of the
+// GPU alone, from a graph, where the chunks take 6 us less.)
 //
 // A tile of which 64 keys hold all that its tokens see (a window's edge, the diagonal, first
 // tokens that stay) is computed for those 64 alone.  The loading warp, which has the time,
@@ -113,7 +115,11 @@ __device__ __forceinline__ void tmem_st_32(uint32_t addr, const uint32_t *v) {
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // 64 scores of a row (float32 in raw) to weights 2^(s scale2 + shift), as 16-bit values in
-// raw's first half; returns their sum before that rounding.  The special-function unit
+// raw's first half; returns their sum before that rounding.  The rounding is what the tensor
+// core takes beside 16-bit values, and about as large as the output's own: the prompt's error
+// against 64 bits is 2.0e-3 with it and 1.6e-3 without, drafted float16 tokens' 2.8e-4 and
+// 2.1e-4.  A second product with what it leaves, as in the decode kernel, would add half to
+// the tensor core's time, which is as long as the exponentials' now.  The special-function unit
 // takes 8 cycles for a warp's exponential and bounds it: 533 cycles a warp with two warps
 // on a scheduler.  A quarter of them as polynomials on the multiply-add pipe (26 cycles a
 // pair against 16) took as long.

@@ -10,10 +10,11 @@
 // more); the page contents then move in a second launch over the whole GPU.
 //
 // Nothing here computes: the bound is the bytes moved (the rows copied, once in
-// and once out) plus the two launches.  Measured: a fork of 4 beams over 96 pages 6.5 us,
-// which is latency alone; of 16 groups of 8 beams with 142 MB moved 32 us (4.4 TB/s; 10 of
-// them bookkeeping); a compaction of 1.2 GB moved (both ways) 200 us (6.2 TB/s); 16 ragged
-// chunks of up to 512 tokens taken and written 15 us, most of them two launches' latency.
+// and once out) plus the two launches.  Measured through the public calls: a fork of 4 beams
+// over 96 pages 8.3 us (6.2 on the GPU), which is latency alone; of 16 groups of 8 beams with
+// 142 MB moved 32 us (4.4 TB/s; 10 of them bookkeeping); a compaction of 1.2 GB moved (both
+// ways) 210 to 214 us (5.8 TB/s); 16 ragged chunks of up to 512 tokens taken and written
+// 15 us, most of them two launches' latency.
 #include "qs_common.cuh"
 #include "qs_launch.h"
 
