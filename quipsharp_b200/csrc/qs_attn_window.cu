@@ -201,12 +201,6 @@ constexpr uint32_t idesc_of(int n, bool b_mn_major) {
   return sm100::idesc_f16_f32(kTile, n) | (f << 7) | (f << 10) | ((b_mn_major ? 1u : 0u) << 16);
 }
 
-// Whether a word of two values holds an infinity or NaN.
-template <typename T>
-__device__ __forceinline__ bool strange(uint32_t w) {
-  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-  return (w & e) == e || (w >> 16 & e) == e;
-}
 template <typename T>
 __device__ __forceinline__ float2 floats_of(uint32_t w) {
   if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2 *>(&w));
@@ -373,109 +367,149 @@ __device__ __forceinline__ int first_key(const Job &j, int i) {
 }
 
 // A value that a row does not see has weight 0 in its sum, and 0 x inf is NaN.  So a row
-// (r of query tile t) whose sum is not finite is summed again, key by key, by a whole warp, if
-// a key of its tiles that it does not see has an infinite or NaN value.  By a warp that has
-// nothing else to do: in the softmax warps' epilogue the same code took registers from their
-// loop (a prompt of 8192 tokens 968 -> 1022 us).
+// (r of query tile t) whose sum is not finite is looked at by a whole warp, a few dimensions to
+// a lane: where a key of its tiles that it does not see has an infinite or NaN value, and its
+// own key has none that would explain the output, that dimension is summed again, key by key.
+// By a warp that has nothing else to do: in the softmax warps' epilogue the same code took
+// registers from their loop (a prompt of 8192 tokens 968 -> 1022 us).
 template <typename T, int DP>
-__device__ __forceinline__ void amend_row(const WindowArgs &w, const Job &j, int t, int r, int lane) {
-  constexpr int PER = DP / 32;  // outputs per lane
-  const AttnArgs &a = w.a;
-  const int ahead = t * w.tokens_per_tile + r / w.share, token = j.t0 + ahead, pos = j.pos0 + ahead;
-  const int last = min(pos, j.keys - 1);
-  const int low = a.window > 0 && pos >= a.window ? static_cast<int>(pos - a.window) : -1;
-  const int head = j.head * w.share + r % w.share, pieces = a.dim / 8, slots = (1 << a.page_shift) - 1;
-  const int *table = a.table + static_cast<int64_t>(j.row) * a.width;
-  auto seen = [&](int key) { return key <= last && (key > low || key < a.sinks); };
-  auto page_of = [&](int key) {  // -1 where there is none
-    if (key >= j.keys) return -1;
-    const int p = table[key >> a.page_shift];
-    return p >= 0 && p < a.pages ? p : -1;
-  };
-  const T *keys = static_cast<const T *>(a.k) + j.head * a.ks[1], *values = static_cast<const T *>(a.v) + j.head * a.vs[1];
-  bool unseen = false;
-  for (int i = 0; i < j.tiles; ++i) {
-    const int k0 = first_key(j, i);
-#pragma unroll 1
-    for (int key = k0 + lane; key < k0 + kTile; key += 32) {
-      const int page = seen(key) ? -1 : page_of(key);
-      if (page < 0) continue;
-      const uint4 *v = reinterpret_cast<const uint4 *>(values + page * a.vs[0] + (key & slots) * a.vs[2]);
-#pragma unroll 1
-      for (int c = 0; c < pieces; ++c) {
-        const uint4 x = v[c];
-        unseen |= strange<T>(x.x) || strange<T>(x.y) || strange<T>(x.z) || strange<T>(x.w);
+struct Amend {
+  static constexpr int PER = DP / 32;  // dimensions of a lane
+  const WindowArgs &w;
+  const int lane;
+  int token = -1;       // the last one looked at,
+  uint32_t unseen = 0;  // and this lane's dimensions with such values among the keys that it does not see
+
+  __device__ Amend(const WindowArgs &w_, int lane_) : w(w_), lane(lane_) {}
+
+  static __device__ __forceinline__ uint32_t strange_of(const T *v) {  // a bit for each dimension
+    uint32_t bits = 0;
+#pragma unroll
+    for (int c = 0; c < PER; c += 2) {
+      constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+      const uint32_t x = *reinterpret_cast<const uint32_t *>(v + c);
+      bits |= ((x & e) == e ? 1u : 0u) << c | ((x >> 16 & e) == e ? 2u : 0u) << c;
+    }
+    return bits;
+  }
+
+  __device__ __forceinline__ void row(const Job &j, int t, int r) {
+    const AttnArgs &a = w.a;
+    const int ahead = t * w.tokens_per_tile + r / w.share, pos = j.pos0 + ahead;
+    const int last = min(pos, j.keys - 1), page_mask = (1 << a.page_shift) - 1;
+    const int low = a.window > 0 && pos >= a.window ? static_cast<int>(pos - a.window) : -1;
+    const int head = j.head * w.share + r % w.share;
+    const bool mine = lane * PER < a.dim;  // this lane has dimensions
+    const int64_t at = static_cast<int64_t>(j.t0 + ahead) * a.q_heads + head;
+    const int *table = a.table + static_cast<int64_t>(j.row) * a.width;
+    auto seen = [&](int key) { return key <= last && (key > low || key < a.sinks); };
+    auto page_of = [&](int key) {  // -1 where there is none
+      if (key < 0 || key >= j.keys) return -1;
+      const int p = table[key >> a.page_shift];
+      return p >= 0 && p < a.pages ? p : -1;
+    };
+    auto place = [&](const void *pool, const int64_t (&st)[3], int page, int key) {
+      return static_cast<const T *>(pool) + page * st[0] + j.head * st[1] + (key & page_mask) * st[2];
+    };
+    float *part = w.splits > 1 ? w.part_o + (j.split * a.tokens * a.q_heads + at) * DP + lane * PER : nullptr;
+    T *out = static_cast<T *>(a.out) + at * a.dim + lane * PER;
+    uint32_t bad = 0;  // dimensions whose sum is not finite
+    if (mine) {
+      if (w.splits > 1)
+#pragma unroll
+        for (int c = 0; c < PER; ++c) bad |= (fabsf(part[c]) < INFINITY ? 0u : 1u) << c;
+      else
+        bad = strange_of(out);
+    }
+    // a model gone NaN: the token's own value says it all
+    const int own = seen(last) ? page_of(last) : -1;
+    if (mine && own >= 0) bad &= ~strange_of(place(a.v, a.vs, own, last) + lane * PER);
+    if (!__any_sync(0xffffffffu, bad)) return;
+    if (token != ahead) {  // the heads of a token see the same keys
+      token = ahead;
+      unseen = 0;
+      for (int i = 0; i < j.tiles; ++i) {
+        const int k0 = first_key(j, i);
+        if (k0 + kTile - 1 <= last && (k0 > low || k0 + kTile <= a.sinks)) continue;  // all seen
+        for (int key = k0; key < k0 + kTile; key += 16) {  // of one page
+          const int page = page_of(key);
+          if (page < 0) continue;
+          const T *v = place(a.v, a.vs, page, key) + lane * PER;
+#pragma unroll
+          for (int x = 0; x < 16; ++x)
+            if (mine && key + x < j.keys && !seen(key + x)) unseen |= strange_of(v + x * a.vs[2]);
+        }
       }
     }
-  }
-  if (!__any_sync(0xffffffffu, unseen)) return;  // the row sees what is not finite
-  const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + token * a.q_token + head * a.q_head);
-  const float scale2 = a.scale * kLog2e;
-  float m = -INFINITY, l = 0.f, o[PER] = {};
-  for (int i = 0; i < j.tiles; ++i) {
-    const int k0 = first_key(j, i);
+    bad &= unseen;
+    if (!__any_sync(0xffffffffu, bad)) return;
+
+    const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + static_cast<int64_t>(j.t0 + ahead) * a.q_token +
+                                                     head * a.q_head);
+    const int pieces = a.dim / 8;
+    const float scale2 = a.scale * kLog2e;
+    float m = -INFINITY, l = 0.f, o[PER] = {};
+    for (int i = 0; i < j.tiles; ++i) {
+      const int k0 = first_key(j, i);
 #pragma unroll 1
-    for (int key = k0 + lane; key < k0 + kTile; key += 32) {  // the same number of turns for every lane
-      const int page = seen(key) ? page_of(key) : -1;
-      float s = -INFINITY;
-      if (page >= 0) {
-        const uint4 *k = reinterpret_cast<const uint4 *>(keys + page * a.ks[0] + (key & slots) * a.ks[2]);
-        float dot = 0.f;
-#pragma unroll 1
-        for (int c = 0; c < pieces; ++c) {
-          const uint4 x = q[c], y = k[c];
-          auto add = [&](uint32_t u, uint32_t v) {
-            const float2 f = floats_of<T>(u), g = floats_of<T>(v);
-            dot = fmaf(f.x, g.x, fmaf(f.y, g.y, dot));
-          };
-          add(x.x, y.x), add(x.y, y.y), add(x.z, y.z), add(x.w, y.w);
+      for (int k32 = k0; k32 < k0 + kTile; k32 += 32) {
+        const int key = k32 + lane, page = seen(key) ? page_of(key) : -1;
+        const uint32_t some = __ballot_sync(0xffffffffu, page >= 0);
+        if (!some) continue;
+        float s = -INFINITY;
+        if (page >= 0) {
+          const uint4 *k = reinterpret_cast<const uint4 *>(place(a.k, a.ks, page, key));
+          float dot = 0.f;
+#pragma unroll 4
+          for (int c = 0; c < pieces; ++c) {
+            const uint4 x = q[c], y = k[c];
+            auto add = [&](uint32_t u, uint32_t v) {
+              const float2 f = floats_of<T>(u), g = floats_of<T>(v);
+              dot = fmaf(f.x, g.x, fmaf(f.y, g.y, dot));
+            };
+            add(x.x, y.x), add(x.y, y.y), add(x.z, y.z), add(x.w, y.w);
+          }
+          s = dot * scale2;
         }
-        s = dot * scale2;
-      }
-      float top = s;
+        float top = s;
 #pragma unroll
-      for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-      if (top > m) {
-        const float f = ex2(m - top);
-        l *= f;
+        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        if (top > m) {
+          const float f = ex2(m - top);
+          l *= f;
 #pragma unroll
-        for (int c = 0; c < PER; ++c) o[c] *= f;
-        m = top;
-      }
-      const float p = s == -INFINITY ? 0.f : ex2(s - m);
-      l += p;
-      for (uint32_t some = __ballot_sync(0xffffffffu, page >= 0); some; some &= some - 1) {
-        const int of = __ffs(some) - 1;
-        const float pk = __shfl_sync(0xffffffffu, p, of);
-        const T *v = values + __shfl_sync(0xffffffffu, page, of) * a.vs[0] + ((key - lane + of) & slots) * a.vs[2] + lane * PER;
-        if (lane * PER < a.dim)
+          for (int c = 0; c < PER; ++c) o[c] *= f;
+          m = top;
+        }
+        const float p = s == -INFINITY ? 0.f : ex2(s - m);
+        l += p;
+#pragma unroll 8
+        for (int x = 0; x < 32; ++x) {
+          const float px = __shfl_sync(0xffffffffu, p, x);
+          const int page_x = __shfl_sync(0xffffffffu, page, x);
+          if (page_x < 0 || !mine) continue;
+          const T *v = place(a.v, a.vs, page_x, k32 + x) + lane * PER;
 #pragma unroll
           for (int c = 0; c < PER; c += 2) {
             const float2 f = floats_of<T>(*reinterpret_cast<const uint32_t *>(v + c));
-            o[c] = fmaf(pk, f.x, o[c]);
-            o[c + 1] = fmaf(pk, f.y, o[c + 1]);
+            o[c] = fmaf(px, f.x, o[c]);
+            o[c + 1] = fmaf(px, f.y, o[c + 1]);
           }
+        }
       }
     }
-  }
 #pragma unroll
-  for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-  const int64_t at = static_cast<int64_t>(token) * a.q_heads + head;
-  if (w.splits > 1) {
-    const int64_t to = j.split * a.tokens * a.q_heads + at;
+    for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+    // beside the reference that the other dimensions have, or over the sum
+    const float f = l == 0.f ? 0.f : w.splits > 1 ? ex2(m - w.part_ml[j.split * a.tokens * a.q_heads + at].x) : 1.f / l;
 #pragma unroll
-    for (int c = 0; c < PER; ++c) w.part_o[to * DP + lane * PER + c] = o[c];
-    if (lane == 0) w.part_ml[to] = make_float2(m, l);
-    return;
+    for (int c = 0; c < PER; ++c)
+      if (bad >> c & 1) {
+        if (w.splits > 1) part[c] = o[c] * f;
+        else store1(out + c, o[c] * f);
+      }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-  for (int c = 0; c < PER; c += 2) {
-    uint32_t packed;
-    split16<T>(o[c] * inv, o[c + 1] * inv, packed);
-    if (lane * PER < a.dim) *reinterpret_cast<uint32_t *>(static_cast<T *>(a.out) + at * a.dim + lane * PER + c) = packed;
-  }
-}
+};
 
 template <typename T, int DP, int NQ>
 __global__ void __launch_bounds__(Cfg<DP, NQ>::threads, 1)
@@ -490,6 +524,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   __shared__ uint32_t spans[kSpans][NQ];  // of the last key tiles
   __shared__ __align__(16) uint8_t answer_s[16];
   __shared__ uint32_t bads[2][NQ * 4];  // a job's rows whose sums are not finite, by softmax warp
+  __shared__ uint32_t amended;          // rows summed again so far
   const AttnArgs &a = w.a;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   uint8_t *base = dsm + ((1024u - (smem_u32(dsm) & 1023u)) & 1023u);
@@ -510,6 +545,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   uint32_t *holder = reinterpret_cast<uint32_t *>(base + (NQ + S) * C::tile_bytes + C::out_bytes + C::bars * 8);
 
   if (tid == 0) {
+    amended = 0;
     for (int s = 0; s < S; ++s) {
       sm100::mbar_init(full(s), 1);
       sm100::mbar_init(empty(s), 1);
@@ -544,9 +580,16 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   sm100::tc_fence_after_sync();
   const uint32_t tmem = *holder;
   const int per = NQ * w.tokens_per_tile;
-  auto key_of_tile = [&](const Job &j, int i) {
-    i += j.first;
-    return i < j.sink_tiles ? i * kTile : j.from + (i - j.sink_tiles) * kTile;
+  auto key_of_tile = [&](const Job &j, int i) { return first_key(j, i); };
+  // A wait between jobs, which rows being summed again may hold up: its limit starts anew with
+  // each of them.
+  auto wait_job = [&](uint32_t bar, uint32_t parity) {
+    for (uint32_t before = 0;;) {
+      if (sm100::mbar_wait_warp(bar, parity, w.wait_ns)) return true;
+      const uint32_t now = __shfl_sync(0xffffffffu, *const_cast<volatile uint32_t *>(&amended), 0);
+      if (now == before) return false;
+      before = now;
+    }
   };
 
   if (warp < 4) {
@@ -562,7 +605,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       for (int num = 0; ok; ++num) {
         const int slot = num & 1;
         const Job j = job_of(w, bx, by, bz, per, lane);
-        if (num >= 2) ok = sm100::mbar_wait_warp(job_empty(slot), ((num >> 1) - 1) & 1, w.wait_ns);
+        if (num >= 2) ok = wait_job(job_empty(slot), ((num >> 1) - 1) & 1);
         if (!ok) break;
         if (lane == 0) {
           jobs[slot] = j;
@@ -654,7 +697,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         if (!ok || !next_block(answer, bx, by, bz)) {
           // no block is left: the job after this one says so
           const int last = (num + 1) & 1;
-          if (ok && num >= 1) ok = sm100::mbar_wait_warp(job_empty(last), (((num + 1) >> 1) - 1) & 1, w.wait_ns);
+          if (ok && num >= 1) ok = wait_job(job_empty(last), (((num + 1) >> 1) - 1) & 1);
           if (ok && lane == 0) {
             jobs[last].tiles = -1;
             sm100::mbar_arrive(job_full(last));
@@ -702,7 +745,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       int q_loads = 0, place = 0, step = 0;  // place: of the job's first tile in the ring; step: key tiles so far
       for (int num = 0; ok; ++num) {
         const int slot = num & 1;
-        ok = sm100::mbar_wait_warp(job_full(slot), (num >> 1) & 1, w.wait_ns);
+        ok = wait_job(job_full(slot), (num >> 1) & 1);
         if (!ok) break;
         const int n = __shfl_sync(0xffffffffu, jobs[slot].tiles, 0);
         if (n < 0) break;
@@ -766,11 +809,12 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       if (!sm100::mbar_wait_warp(drain, 0, kDrainNs)) *w.error = 1;
     } else {
       // ---- rows to be summed again, every second softmax warp's each
+      Amend<T, DP> amend(w, lane);
       bool ok = true;
       uint32_t summed_phase = 0;
       for (int num = 0; ok; ++num) {
         const int slot = num & 1;
-        ok = sm100::mbar_wait_warp(job_full(slot), (num >> 1) & 1, w.wait_ns);
+        ok = wait_job(job_full(slot), (num >> 1) & 1);
         if (!ok) break;
         const int n = __shfl_sync(0xffffffffu, jobs[slot].tiles, 0);
         if (n < 0) break;
@@ -780,8 +824,12 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           if (!ok) break;
           for (int from = warp - 2; from < NQ * 4; from += 2) {
             uint32_t bad = *const_cast<volatile uint32_t *>(&bads[slot][from]);
-            for (; bad; bad &= bad - 1) amend_row<T, DP>(w, jobs[slot], from >> 2, (from & 3) * 32 + __ffs(bad) - 1, lane);
+            for (; bad; bad &= bad - 1) {
+              amend.row(jobs[slot], from >> 2, (from & 3) * 32 + __ffs(bad) - 1);
+              if (lane == 0) atomicAdd(&amended, 1u);
+            }
           }
+          amend.token = -1;
         }
         __syncwarp();
         if (lane == 0) sm100::mbar_arrive(job_empty(slot));
@@ -802,7 +850,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     int step = 0, outs = 0;
     for (int num = 0; ok; ++num) {
       const int slot = num & 1;
-      ok = sm100::mbar_wait_warp(job_full(slot), (num >> 1) & 1, w.wait_ns);
+      ok = wait_job(job_full(slot), (num >> 1) & 1);
       if (!ok) break;
       const Job j = jobs[slot];
       const int n = j.tiles;
@@ -976,20 +1024,28 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         }
         __syncwarp();
       };
-      // whether the sums are finite: 0 times them is then 0 (see amend_row)
+      // whether the sums are finite: 0 times them is then 0 (see Amend)
       uint64_t test[4] = {};
       auto look = [&](const uint32_t *o) {
 #pragma unroll
         for (int x = 0; x < 32; x += 2)
           test[x / 2 % 4] = fma2(pack2(__uint_as_float(o[x]), __uint_as_float(o[x + 1])), 0, test[x / 2 % 4]);
       };
+      uint32_t bad = 0;
       auto report = [&] {
-        const float2 z = unpack2(add2(add2(test[0], test[1]), add2(test[2], test[3])));
-        const uint32_t bad = __ballot_sync(0xffffffffu, real && l < INFINITY && !(z.x + z.y == 0.f));
         if (lane == 0) {
           *const_cast<volatile uint32_t *>(&bads[slot][warp - 4]) = bad;
           sm100::mbar_arrive(summed(slot));
         }
+      };
+      auto judge = [&] {  // the usual answer goes out while the outputs are being stored
+        const float2 z = unpack2(add2(add2(test[0], test[1]), add2(test[2], test[3])));
+        bad = __ballot_sync(0xffffffffu, real && l < INFINITY && !(z.x + z.y == 0.f));
+        if (bad == 0) report();
+      };
+      auto stored = [&] {
+        __syncwarp();
+        if (bad) report();
       };
       if (w.splits > 1) {
         const int64_t base = j.split * a.tokens * a.q_heads;
@@ -999,12 +1055,12 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           tmem_ld_32(o_at + c, o);
           sm100::tmem_ld_wait();
           look(o);
+          if (c + 32 == DP) judge();
           send(o, reinterpret_cast<char *>(w.part_o + base * DP + c), DP * 4, 128);
         }
         if (real) w.part_ml[base + at] = make_float2(m == -INFINITY ? -INFINITY : m * scale2 - kBias, l);
         sm100::tc_fence_before_sync();
-        __syncwarp();
-        report();
+        stored();
         continue;
       }
 #pragma unroll
@@ -1015,6 +1071,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         sm100::tmem_ld_wait();
         look(o);
         look(o + 32);
+        if (c + 64 == DP) judge();
 #pragma unroll
         for (int x = 0; x < 32; ++x)
           split16<T>(__uint_as_float(o[2 * x]) * inv, __uint_as_float(o[2 * x + 1]) * inv, o[x]);
@@ -1022,8 +1079,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       }
       sm100::tc_fence_before_sync();  // O is read: the next job's first weights release it
       if (real && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : (m * scale2 - kBias) * kLn2) + logf(l);
-      __syncwarp();
-      report();
+      stored();
     }
     if (!ok) *w.error = 1;
   }

@@ -5,6 +5,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 
+from quipsharp_b200 import _native as N
 from quipsharp_b200 import attention as at
 from quipsharp_b200 import kv_cache as kc
 from quipsharp_b200.beam import beam_select
@@ -252,3 +253,35 @@ def test_scores_that_grow_along_the_row_and_large_values(new, heads, dtype):
     check(at.window_attention(q, k, v, table, lengths, offsets([new]), return_lse=True), want, dtype, True)
     one = [x[-1:] for x in want]
     check(at.decode_attention(q[-1:], k, v, table, lengths, return_lse=True), one, dtype, False)
+
+
+def test_rows_summed_again_do_not_run_into_the_wait_limit():
+    """Many such rows keep their warps far beyond a wait's limit: as long as they come along,
+    the others wait on.  A model whose values are NaN throughout is not summed again at all."""
+    rs = np.random.RandomState(3)
+    new, n, heads, dim = 512, 4096, 64, 128
+    k, v, table, lengths = make(rs, [n], heads, 64, dim, torch.float16)
+    q = torch.randn(new, 8 * heads, dim, device=DEV).half()
+    lib = N.lib()
+
+    def run(values):
+        return at.window_attention(q, k, values, table, lengths, offsets([new]))
+
+    clean, w = run(v), v.clone()
+    place = n - 130  # the tokens before it, in its tile, do not see it
+    w[int(table[0, place // 64]), :, place % 64, 9] = float("inf")
+    kc.check_device()
+    try:
+        assert lib.qs_set_wait_limit_ns(3_000_000) == N.QS_OK
+        got = run(w)
+        kc.check_device()
+        gone = run(torch.full_like(v, float("nan")))
+        kc.check_device()
+    finally:
+        lib.qs_set_wait_limit_ns(0)
+    hit = torch.arange(n - new, n, device=DEV) >= place
+    assert gone.isnan().all() and not got[hit, :, 9].isfinite().any()
+    keep = torch.arange(dim, device=DEV) != 9
+    assert torch.equal(got[..., keep], clean[..., keep])
+    # weights rounded in one sum and not in the other: 2^-11 of the sum of p |v|, below 1, and the outputs' own rounding
+    assert float((got[~hit, :, 9].float() - clean[~hit, :, 9].float()).abs().max()) < 2.0 ** -9
