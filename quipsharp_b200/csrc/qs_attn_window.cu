@@ -30,7 +30,7 @@
 // cycles of an SM's sixteen a cycle, next to 1024 of the two products (dim 128) and the
 // rest of the softmax's issue.  Measured: a prompt of 8192 tokens, 64 query heads over 8
 // of 128, bfloat16: 940 to 967 us (1.14 to 1.17 PFLOP/s, by the clocks that the power limit
-// leaves); four chunks of 300 to 2000 tokens under a window of 1024: 87 us (0.68 PFLOP/s of
+// leaves); four chunks of 300 to 2000 tokens under a window of 1024: 88 us (0.67 PFLOP/s of
 // visible pairs; ten tiles a job, four of them with masks); up to 9 tokens of 3 rows: 10.4 us,
 // latency alone.  (Passes through the public call; the figures of variants below are of the
 // GPU alone, from a graph, where the chunks take 6 us less.)
