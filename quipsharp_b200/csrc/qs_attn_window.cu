@@ -1038,7 +1038,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           sm100::mbar_arrive(summed(slot));
         }
       };
-      auto judge = [&] {  // the usual answer goes out while the outputs are being stored
+      auto tested = [&] {  // the usual answer goes out while the outputs are being stored
         const float2 z = unpack2(add2(add2(test[0], test[1]), add2(test[2], test[3])));
         bad = __ballot_sync(0xffffffffu, real && l < INFINITY && !(z.x + z.y == 0.f));
         if (bad == 0) report();
@@ -1055,7 +1055,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           tmem_ld_32(o_at + c, o);
           sm100::tmem_ld_wait();
           look(o);
-          if (c + 32 == DP) judge();
+          if (c + 32 == DP) tested();
           send(o, reinterpret_cast<char *>(w.part_o + base * DP + c), DP * 4, 128);
         }
         if (real) w.part_ml[base + at] = make_float2(m == -INFINITY ? -INFINITY : m * scale2 - kBias, l);
@@ -1071,7 +1071,7 @@ attn_window_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         sm100::tmem_ld_wait();
         look(o);
         look(o + 32);
-        if (c + 64 == DP) judge();
+        if (c + 64 == DP) tested();
 #pragma unroll
         for (int x = 0; x < 32; ++x)
           split16<T>(__uint_as_float(o[2 * x]) * inv, __uint_as_float(o[2 * x + 1]) * inv, o[x]);

@@ -427,7 +427,8 @@ __global__ void __launch_bounds__(kS, kScanCtas) beam_scan_kernel(ScanArgs a) {
     for (int i = have + tid; i < a.n; i += kS) out[i] = make_uint2(0u, 0u);  // a chunk of fewer than n logits
   } else {
     // More equal or huge logits than fit (a vocabulary masked to one value, say):
-    // n rounds, each the best one after the last pick.
+    // n rounds, each the best one after the last pick (32 x 8 x 128000 bfloat16 logits of
+    // which all but 1000 are masked, n = 16: 680 us, for 28).
     uint2 last = make_uint2(0xffffffffu, 0u);
     for (int r = 0; r < a.n; ++r) {
       uint2 b = make_uint2(0u, 0x7fffffffu);
